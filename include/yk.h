@@ -245,7 +245,9 @@ int yk_track_op(yk_tracker* trk, int stream_index, int pos, int op, int arg, con
 /* sizeof() of the ABI structs, for bindings that mirror them (0: yk_tracker_cfg,
  * 1: yk_tracker_stats, 2: yk_track_out, 3: yk_track_state, 4: yk_view, 5: yk_op,
  * 6: yk_model_desc, 7: yk_bt_cfg, 8: yk_motion, 9: yk_gmd_stats, 10: yk_tensor,
- * 11: yk_track_event); -1 for an unknown id. */
+ * 11: yk_track_event, 12: yk_linear_args, 13: yk_linear_grad_args, 14: yk_layer_norm_args,
+ * 15: yk_layer_norm_grad_args, 16: yk_attention_args, 17: yk_attention_grad_args); -1 for an
+ * unknown id. */
 int64_t yk_struct_size(int which);
 
 /* Append a new track created from a box (AircraftKalmanTracker.__init__, :23-101) to the
@@ -601,17 +603,163 @@ int yk_model_buffer(yk_model* m, int buf, void** dev_ptr);
 /* Synchronous device -> host copy (bindings without their own HIP runtime access). */
 int yk_memcpy_d2h(void* host_dst, const void* dev_src, int64_t bytes);
 
+/* ------------------------------------------------------------------ token operators
+ * The products, norms and attention of a transformer layer over the cells of a feature map (a token
+ * is one NHWC pixel: a row of channels), beside the convolutions a detector program runs.  A
+ * program's YK_K_LINEAR / YK_K_LAYER_NORM / YK_K_ATTENTION ops call the same kernels.  Matrices
+ * are rows of `dtype` elements (YK_ACT_BF16, YK_ACT_F32 or YK_ACT_F16) with a stride between
+ * rows, in elements (an input's may be 0: one row for all); elements of a row are adjacent.  Any
+ * size from 1, any alignment that is a multiple of the element.  Sums,
+ * softmax statistics and norms are float32; an output is rounded once.
+ *
+ * Every call only enqueues kernels on `stream` (hipGraph-capturable); nothing is allocated, so
+ * a call that needs scratch takes it from the caller: *_workspace returns the bytes for the same
+ * arguments (pointers other than the optional ones need not be set), and `ws` must be 16-byte
+ * aligned and stay untouched until the call's kernels have ended.  Outputs must not overlap inputs
+ * (yk_linear's y may be res where strides and rows agree) and scratch belongs to one call in flight. */
+enum yk_token_act { YK_TOK_NONE = 0, YK_TOK_SILU = 1, YK_TOK_GELU = 2, YK_TOK_RELU = 3 }; /* GELU: z * Phi(z) */
+
+/* y[m][n] = act(z[m][n]) + res[m % res_rows][n],  z = x w^T + bias. */
+typedef struct {
+  int32_t dtype, act;       /* yk_act_dtype, yk_token_act                                     */
+  int32_t bias_f32;         /* 1: bias is float32, 0: it is `dtype`                           */
+  int32_t reserved;         /* 0                                                              */
+  int64_t m, n, k;
+  const void* x;            /* [m][k]                                                         */
+  const void* w;            /* [n][k], a linear layer's weight                                */
+  const void* bias;         /* [n] or NULL                                                    */
+  const void* res;          /* [res_rows][n] or NULL; res_rows == m: a plain residual         */
+  void* y;                  /* [m][n]                                                         */
+  void* z;                  /* [m][n] or NULL: act's argument, for the backward pass          */
+  int64_t x_stride, w_stride, res_stride, res_rows, y_stride, z_stride;
+  void* ws;
+  int64_t ws_bytes;
+} yk_linear_args;
+int yk_linear_workspace(const yk_linear_args* a, int64_t* bytes);
+int yk_linear(yk_ctx* ctx, const yk_linear_args* a, void* stream);
+
+/* Gradients of yk_linear: dz = dy act'(z), dx = dz w, dw = dz^T x, dbias = sum over m of dz,
+ * dres[r] = sum of dy[m] over m % res_rows == r.  A NULL output is not computed. */
+typedef struct {
+  int32_t dtype, act, bias_f32, reserved;
+  int64_t m, n, k;
+  const void* dy;           /* [m][n]                                                         */
+  const void* x;            /* [m][k]; may be NULL without dw                                 */
+  const void* w;            /* [n][k]; may be NULL without dx                                 */
+  const void* z;            /* [m][n], yk_linear's z; may be NULL when act is YK_TOK_NONE     */
+  void* dx;                 /* [m][k]                                                         */
+  void* dw;                 /* [n][k]                                                         */
+  void* dbias;              /* [n], float32 or `dtype` by bias_f32                            */
+  void* dres;               /* [res_rows][n]                                                  */
+  int64_t dy_stride, x_stride, w_stride, z_stride, dx_stride, dw_stride, dres_stride, res_rows;
+  void* ws;
+  int64_t ws_bytes;
+} yk_linear_grad_args;
+int yk_linear_backward_workspace(const yk_linear_grad_args* a, int64_t* bytes);
+int yk_linear_backward(yk_ctx* ctx, const yk_linear_grad_args* a, void* stream);
+
+/* y = (x - mean) * rstd * w + b over each row of c elements, rstd = 1 / sqrt(var + eps) with the
+ * biased variance.  w / b NULL: 1 / 0.  mean / rstd (float32 [m]) NULL: not stored. */
+typedef struct {
+  int32_t dtype, param_f32; /* 1: w and b are float32, 0: they are `dtype`                    */
+  int64_t m, c;
+  float eps;
+  int32_t reserved;
+  const void* x;
+  const void* w;
+  const void* b;
+  void* y;
+  float* mean;
+  float* rstd;
+  int64_t x_stride, y_stride;
+} yk_layer_norm_args;
+int yk_layer_norm(yk_ctx* ctx, const yk_layer_norm_args* a, void* stream);
+
+/* Gradients of yk_layer_norm from its mean and rstd.  A NULL output is not computed; dw / db are
+ * float32 or `dtype` by param_f32, and need scratch. */
+typedef struct {
+  int32_t dtype, param_f32;
+  int64_t m, c;
+  const void* dy;
+  const void* x;
+  const void* w;
+  const float* mean;
+  const float* rstd;
+  void* dx;
+  void* dw;
+  void* db;
+  int64_t dy_stride, x_stride, dx_stride;
+  void* ws;
+  int64_t ws_bytes;
+} yk_layer_norm_grad_args;
+int yk_layer_norm_backward_workspace(const yk_layer_norm_grad_args* a, int64_t* bytes);
+int yk_layer_norm_backward(yk_ctx* ctx, const yk_layer_norm_grad_args* a, void* stream);
+
+/* o = softmax(scale q k^T) v per head; head h of q reads key head h / (h_q / h_kv).  Rows of a
+ * head are d <= 128 adjacent elements; *_stride = {batch, row, head} strides in elements.
+ * lengths[b] / q_lengths[b] (int32 on the device, NULL: all): the keys / queries in use, clamped to
+ * [0, nk] / [0, nq]; rows behind them are not read, and their o (and dq, dk, dv) is 0.  causal:
+ * query i sees keys j <= i + length - q_length (the last query sees the last key).  A query that
+ * sees no key gives o = 0, lse = -infinity and has no gradient. */
+typedef struct {
+  int32_t dtype, causal;
+  int32_t b, h_q, h_kv, d;
+  int64_t nq, nk;
+  float scale;
+  int32_t reserved;
+  const void* q;            /* [b][nq][h_q][d]                                                */
+  const void* k;            /* [b][nk][h_kv][d]                                               */
+  const void* v;
+  const int32_t* q_lengths;
+  const int32_t* lengths;
+  void* o;                  /* as q                                                           */
+  float* lse;               /* [b][h_q][nq]: ln of the softmax's denominator, or NULL         */
+  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
+  void* ws;
+  int64_t ws_bytes;
+} yk_attention_args;
+int yk_attention_workspace(const yk_attention_args* a, int64_t* bytes);
+int yk_attention(yk_ctx* ctx, const yk_attention_args* a, void* stream);
+
+/* Gradients of yk_attention: the probabilities are computed again from q, k and lse. */
+typedef struct {
+  int32_t dtype, causal;
+  int32_t b, h_q, h_kv, d;
+  int64_t nq, nk;
+  float scale;
+  int32_t reserved;
+  const void* go;           /* gradient of o                                                  */
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* o;
+  const float* lse;
+  const int32_t* q_lengths;
+  const int32_t* lengths;
+  void* dq;
+  void* dk;
+  void* dv;
+  int64_t go_stride[3], q_stride[3], k_stride[3], v_stride[3], o_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+  void* ws;
+  int64_t ws_bytes;
+} yk_attention_grad_args;
+int yk_attention_backward_workspace(const yk_attention_grad_args* a, int64_t* bytes);
+int yk_attention_backward(yk_ctx* ctx, const yk_attention_grad_args* a, void* stream);
+
 /* Host-side layout check, compiled into the caller with the caller's view of the structs: 0 when
  * the loaded library has this header's ABI version and every struct size, else YK_ERR_STATE.
  * Call it once before any other entry point. */
 static inline int yk_abi_check(void) {
-  const int64_t want[12] = {(int64_t)sizeof(yk_tracker_cfg), (int64_t)sizeof(yk_tracker_stats),
+  const int64_t want[18] = {(int64_t)sizeof(yk_tracker_cfg), (int64_t)sizeof(yk_tracker_stats),
                             (int64_t)sizeof(yk_track_out), (int64_t)sizeof(yk_track_state),
                             (int64_t)sizeof(yk_view), (int64_t)sizeof(yk_op), (int64_t)sizeof(yk_model_desc),
                             (int64_t)sizeof(yk_bt_cfg), (int64_t)sizeof(yk_motion), (int64_t)sizeof(yk_gmd_stats),
-                            (int64_t)sizeof(yk_tensor), (int64_t)sizeof(yk_track_event)};
+                            (int64_t)sizeof(yk_tensor), (int64_t)sizeof(yk_track_event),
+                            (int64_t)sizeof(yk_linear_args), (int64_t)sizeof(yk_linear_grad_args),
+                            (int64_t)sizeof(yk_layer_norm_args), (int64_t)sizeof(yk_layer_norm_grad_args),
+                            (int64_t)sizeof(yk_attention_args), (int64_t)sizeof(yk_attention_grad_args)};
   if (yk_abi_version() != YK_ABI_VERSION) return YK_ERR_STATE;
-  for (int i = 0; i < 12; ++i)
+  for (int i = 0; i < 18; ++i)
     if (yk_struct_size(i) != want[i]) return YK_ERR_STATE;
   return YK_OK;
 }

@@ -10,7 +10,7 @@ CPU fallback: without the library or a GPU every entry point raises ``YKError``.
 ``compat/`` holds ``kalman`` and ``ultralytics`` shim packages: put that directory on
 sys.path and the reference driver's imports resolve to this package unchanged.
 """
-from . import arch, frames, model, predictor, shard, synth, tracker, visualize, weights  # noqa: F401
+from . import arch, frames, model, ops, predictor, shard, synth, tracker, visualize, weights  # noqa: F401
 from ._lib import YKError, exported_symbols  # noqa: F401
 from .tracker import (  # noqa: F401
     AircraftKalmanTracker,

@@ -135,6 +135,54 @@ def weights_struct(sd: dict):
     return w, keep
 
 
+def _fields(*groups):
+    """ctypes fields from (type, "name name ...") groups."""
+    return [(n, t) for t, names in groups for n in names.split()]
+
+
+# token operators (yk_linear_args ... yk_attention_grad_args)
+_i64 = C.c_int64
+_s3 = _i64 * 3
+
+
+class LinearArgs(C.Structure):
+    _fields_ = _fields((_i32, "dtype act bias_f32 reserved"), (_i64, "m n k"), (_vp, "x w bias res y z"),
+                       (_i64, "x_stride w_stride res_stride res_rows y_stride z_stride"), (_vp, "ws"), (_i64, "ws_bytes"))
+
+
+class LinearGradArgs(C.Structure):
+    _fields_ = _fields((_i32, "dtype act bias_f32 reserved"), (_i64, "m n k"), (_vp, "dy x w z dx dw dbias dres"),
+                       (_i64, "dy_stride x_stride w_stride z_stride dx_stride dw_stride dres_stride res_rows"), (_vp, "ws"),
+                       (_i64, "ws_bytes"))
+
+
+class LayerNormArgs(C.Structure):
+    _fields_ = _fields((_i32, "dtype param_f32"), (_i64, "m c"), (C.c_float, "eps"), (_i32, "reserved"),
+                       (_vp, "x w b y mean rstd"), (_i64, "x_stride y_stride"))
+
+
+class LayerNormGradArgs(C.Structure):
+    _fields_ = _fields((_i32, "dtype param_f32"), (_i64, "m c"), (_vp, "dy x w mean rstd dx dw db"),
+                       (_i64, "dy_stride x_stride dx_stride"), (_vp, "ws"), (_i64, "ws_bytes"))
+
+
+class AttentionArgs(C.Structure):
+    _fields_ = _fields((_i32, "dtype causal b h_q h_kv d"), (_i64, "nq nk"), (C.c_float, "scale"), (_i32, "reserved"),
+                       (_vp, "q k v q_lengths lengths o lse"), (_s3, "q_stride k_stride v_stride o_stride"), (_vp, "ws"),
+                       (_i64, "ws_bytes"))
+
+
+class AttentionGradArgs(C.Structure):
+    _fields_ = _fields((_i32, "dtype causal b h_q h_kv d"), (_i64, "nq nk"), (C.c_float, "scale"), (_i32, "reserved"),
+                       (_vp, "go q k v o lse q_lengths lengths dq dk dv"),
+                       (_s3, "go_stride q_stride k_stride v_stride o_stride dq_stride dk_stride dv_stride"), (_vp, "ws"),
+                       (_i64, "ws_bytes"))
+
+
+TOKEN_ARGS = {"yk_linear": LinearArgs, "yk_linear_backward": LinearGradArgs, "yk_layer_norm": LayerNormArgs,
+              "yk_layer_norm_backward": LayerNormGradArgs, "yk_attention": AttentionArgs,
+              "yk_attention_backward": AttentionGradArgs}
+
 _SIGS = {
     "yk_abi_version": ([], C.c_int),
     "yk_last_error": ([], C.c_char_p),
@@ -209,6 +257,9 @@ _SIGS = {
     "yk_nms_candidates": ([_vp, C.c_int, C.c_float, C.c_int, _vp, _vp, _vp, _vp], C.c_int),
     "yk_model_nms_stats": ([_vp, _vp, C.c_int, _vp], C.c_int),
     "yk_model_check": ([_vp, _vp], C.c_int),
+    **{fn: ([_vp, C.POINTER(t), _vp], C.c_int) for fn, t in TOKEN_ARGS.items()},
+    **{fn + "_workspace": ([C.POINTER(t), C.POINTER(C.c_int64)], C.c_int) for fn, t in TOKEN_ARGS.items()
+       if t is not LayerNormArgs},
 }
 
 _lock = threading.Lock()
@@ -245,7 +296,8 @@ def lib() -> C.CDLL:
             raise YKError(f"libyk.so ABI version {L.yk_abi_version()}, this package expects {ABI_VERSION}")
         sizes = {0: C.sizeof(TrackerCfg), 1: STATS_DTYPE.itemsize, 2: TRACK_OUT_DTYPE.itemsize,
                  3: TRACK_STATE_DTYPE.itemsize, 7: C.sizeof(BtCfg), 8: MOTION_DTYPE.itemsize,
-                 9: GMD_STATS_DTYPE.itemsize, 10: C.sizeof(Tensor), 11: TRACK_EVENT_DTYPE.itemsize}
+                 9: GMD_STATS_DTYPE.itemsize, 10: C.sizeof(Tensor), 11: TRACK_EVENT_DTYPE.itemsize,
+                 **{12 + i: C.sizeof(t) for i, t in enumerate(TOKEN_ARGS.values())}}
         for k, v in sizes.items():
             if L.yk_struct_size(k) != v:
                 raise YKError(f"ABI struct {k} size mismatch: C {L.yk_struct_size(k)} vs python {v}")

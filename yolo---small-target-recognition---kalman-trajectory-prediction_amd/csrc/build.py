@@ -29,6 +29,9 @@ BUILD = os.path.join(HERE, ("_build_diag_" + hashlib.sha1(" ".join(DEFINES).enco
                      else "_build")
 ARCH = os.environ.get("YK_OFFLOAD_ARCH", "gfx950")
 
+# some forms of the packed float32 instructions give wrong results on gfx950
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 # (source, extra flags).  The tracker must not contract a*b+c into FMA: it reproduces
 # numpy's separately rounded float64 arithmetic (see tracker.hip header).
 SOURCES = [
@@ -39,8 +42,12 @@ SOURCES = [
     ("detector.hip", []),
     ("bytetrack.hip", ["-ffp-contract=off"]),
     ("gmd.hip", ["-ffp-contract=off"]),
+    ("linear.hip", NO_PACKED_F32),
+    ("layer_norm.hip", NO_PACKED_F32),
+    ("attention.hip", NO_PACKED_F32),
 ]
 HEADERS = ["yk_internal.h", "yk_host.h", os.path.join("..", "..", "include", "yk.h"), os.path.join("..", "..", "include", "yk_diag.h")]
+OWN_HEADERS = {s: ["token_common.h"] for s in ("linear.hip", "layer_norm.hip", "attention.hip")}
 
 
 def _hipcc() -> str:
@@ -79,7 +86,7 @@ def _compile(src: str, extra: list[str], force: bool) -> str:
     obj = os.path.join(BUILD, os.path.splitext(src)[0] + ".o")
     flags = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function",
              "-I", os.path.join(REPO, "include")] + DEFINES + extra
-    hdrs = [os.path.join(HERE, h) for h in HEADERS]
+    hdrs = [os.path.join(HERE, h) for h in HEADERS + OWN_HEADERS.get(src, [])]
     stamp = obj + ".sha"
     dig = _digest([path] + hdrs, flags)
     if not force and os.path.exists(obj) and os.path.exists(stamp) and open(stamp).read() == dig:

@@ -1,0 +1,645 @@
+// Matrix product with bias, activation and residual in its epilogue, and its gradients
+// (include/yk.h, yk_linear).
+//
+//   forward   y  = act(x w^T + bias) + res[m % res_rows]     [m][k] x [n][k]
+//   backward  dz = dy act'(z);  dx = dz w;  dw = dz^T x;  dbias = column sums of dz;
+//             dres[r] = sum of dy over the rows m % res_rows == r
+//
+// All three products are C[m][n] = sum over k of X(m, k) W(n, k), where either operand may lie
+// transposed in memory (rows of k): forward (plain, plain), dx (plain, transposed), dw (both).  The W
+// side is the MFMA's A operand, so a lane ends with 4 consecutive n of one m.
+#include "token_common.h"
+
+namespace yk {
+namespace tok {
+
+struct GemmArgs {
+  const char* x;
+  const char* w;
+  const void* bias;
+  const char* res;
+  char* y;
+  char* z;
+  float* part;  // split sums: [splits][m][n] float32, or NULL
+  int64_t x_stride, w_stride, res_stride, y_stride, z_stride;
+  int m, n, k, res_rows, act, bias_f32, dtype;
+  int tiles_m, tiles_n, k_split;  // k_split: K elements per blockIdx.y
+};
+
+// bias, activation, residual and the stores of 4 consecutive n of one m
+template <class Tr>
+__device__ __forceinline__ void epilogue(const GemmArgs& a, int64_t m, int n, f32x4 v) {
+  using T = typename Tr::T;
+  const int left = a.n - n;
+  if (left <= 0) return;
+  if (a.bias) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) v[i] += load_param(a.bias, n + i, a.bias_f32, a.dtype);
+  }
+  if (a.z) {
+    T* z = (T*)a.z + m * a.z_stride + n;
+    if (left >= 4) {
+      store4<Tr>(z, v);
+    } else {
+      for (int i = 0; i < left; ++i) z[i] = from_f32<Tr>(v[i]);
+    }
+  }
+  if (a.act != YK_TOK_NONE) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = act_f32(v[i], a.act);
+  }
+  T* y = (T*)a.y + m * a.y_stride + n;
+  const T* res = a.res ? (const T*)a.res + (a.res_rows == a.m ? m : m % a.res_rows) * a.res_stride + n : nullptr;
+  if (left >= 4) {
+    if (res) v += load4<Tr>(res);
+    store4<Tr>(y, v);
+  } else {
+    for (int i = 0; i < left; ++i) y[i] = from_f32<Tr>(v[i] + (res ? to_f32<Tr>(res[i]) : 0.f));
+  }
+}
+
+// One operand's tile in LDS: kRows rows (of m or n) x 128 bytes of K, as 16-byte chunks.
+//   plain       [row][8 chunks of k]; chunk c of row r lies at c ^ (r & 7), so the 16 rows a
+//               fragment read touches fall on different banks
+//   transposed  [k][kRows]; the 16 rows of a fragment are one segment (32 / 64 bytes) of a k row;
+//               segment s of k row kk lies at s ^ twist(kk), which spreads the k rows one read
+//               touches over the banks; 16-bit fragments come through ds_read_b64_tr_b16
+template <class Tr, bool kTrans, int kRows>
+struct Tile {
+  using T = typename Tr::T;
+  static constexpr int kK = 128 / Tr::kBytes;         // K elements of a tile
+  static constexpr int kEpc = 16 / Tr::kBytes;        // elements of a chunk
+  static constexpr int kChunks = kRows * 8;
+  static constexpr int kPerRow = kTrans ? kRows / kEpc : 8;  // chunks of a stored row
+  static constexpr int kSegs = kRows / 16;
+  static constexpr int kSegChunks = Tr::kBytes;       // 16 elements = 32 / 64 bytes
+  static constexpr int kBytesAll = kRows * 128;
+
+  static __device__ __forceinline__ int twist(int kk) {
+    return (Tr::kBytes == 4 ? kk >> 3 : (kk & 3) | ((kk >> 1) & 4)) & (kSegs - 1);
+  }
+  // stored row and first element of chunk j
+  static __device__ __forceinline__ void locate(int j, int& row, int& col) {
+    row = j / kPerRow;
+    const int p = j % kPerRow;
+    if constexpr (kTrans) col = (((p / kSegChunks) ^ twist(row)) * kSegChunks + p % kSegChunks) * kEpc;
+    else col = (p ^ (row & 7)) * kEpc;
+  }
+
+  // K elements 32 * step + 8 * (lane / 16) .. + 7 of row 16 * t + lane % 16
+  static __device__ __forceinline__ typename Tr::V8 frag(const char* lds, int t, int step, int lane) {
+    const int l = lane & 15, g = lane >> 4;
+    if constexpr (!kTrans) {
+      const char* row = lds + (t * 16 + l) * 128;
+      if constexpr (Tr::kBytes == 2) {
+        return *(const typename Tr::V8*)(row + (((step * 4 + g) ^ (l & 7)) << 4));
+      } else {
+        const f32x4 lo = *(const f32x4*)(row + (((2 * g) ^ (l & 7)) << 4));
+        const f32x4 hi = *(const f32x4*)(row + (((2 * g + 1) ^ (l & 7)) << 4));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+    } else if constexpr (Tr::kBytes == 2) {
+      const int kk = step * 32 + g * 8 + (l >> 2);
+      typedef __attribute__((address_space(3))) s16x4* lp;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lp)(lds + kk * (kRows * 2) + ((t ^ twist(kk)) << 5) + (l & 3) * 8));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lp)(lds + (kk + 4) * (kRows * 2) + ((t ^ twist(kk + 4)) << 5) + (l & 3) * 8));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      f32x8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int kk = g * 8 + e;
+        v[e] = *(const float*)(lds + kk * (kRows * 4) + ((t ^ twist(kk)) << 6) + l * 4);
+      }
+      return v;
+    }
+  }
+};
+
+// The loads of one operand's tiles by 256 threads.  kAsync: straight from memory to LDS through a
+// buffer descriptor, whose range check turns a chunk outside the matrix into zeros; needs 16-byte
+// aligned rows and whole chunks.  Otherwise through registers, any alignment.
+template <class Tr, bool kTrans, int kRows, bool kAsync>
+struct Loader {
+  using Tl = Tile<Tr, kTrans, kRows>;
+  using T = typename Tr::T;
+  static constexpr int kN = Tl::kChunks / 256;
+  const T* base;       // first stored row / column of this workgroup's tiles
+  int64_t stride;
+  int rows, cols;      // stored rows / columns left from there
+  u32x4 reg[kAsync ? 1 : kN];
+
+  __device__ __forceinline__ void init(const char* p, int64_t s, int r0, int m, int k0, int k1) {
+    stride = s;
+    if constexpr (kTrans) {
+      base = (const T*)p + (int64_t)k0 * s + r0;
+      rows = k1 - k0;
+      cols = m - r0;
+    } else {
+      base = (const T*)p + (int64_t)r0 * s + k0;
+      rows = m - r0;
+      cols = k1 - k0;
+    }
+  }
+  __device__ __forceinline__ void advance() {
+    if constexpr (kTrans) {
+      base += Tl::kK * stride;
+      rows -= Tl::kK;
+    } else {
+      base += Tl::kK;
+      cols -= Tl::kK;
+    }
+  }
+  __device__ __forceinline__ void issue(char* lds) {
+    const int tid = threadIdx.x;
+    if constexpr (kAsync) {
+      const int64_t span = ((int64_t)(rows - 1) * stride + cols) * Tr::kBytes;
+      const int bytes = rfl((int)(span < 0x7ffffff0 ? span : 0x7ffffff0));
+      const size_t b = (size_t)base;
+      const size_t ub = ((size_t)(unsigned)rfl((int)(b >> 32)) << 32) | (unsigned)rfl((int)b);
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)ub, (short)0, bytes, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        int row, col;
+        Tl::locate(i * 256 + tid, row, col);
+        const unsigned off = row < rows && col < cols ? (unsigned)((row * (int)stride + col) * Tr::kBytes) : 0x80000000u;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rsrc, (__attribute__((address_space(3))) void*)(lds + (i * 256 + rfl(tid & ~63)) * 16), 16, off, 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        int row, col;
+        Tl::locate(i * 256 + tid, row, col);
+        reg[i] = row < rows ? load16<Tr>(base + row * stride + col, cols - col) : u32x4{0, 0, 0, 0};
+      }
+    }
+  }
+  __device__ __forceinline__ void commit(char* lds) {
+    if constexpr (!kAsync) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) *(u32x4*)(lds + (i * 256 + threadIdx.x) * 16) = reg[i];
+    }
+  }
+};
+
+template <class Tr, bool kXT, bool kWT, int kTile, bool kAsync>
+__global__ __launch_bounds__(256) void gemm_kernel(GemmArgs a) {
+  using XTile = Tile<Tr, kXT, kTile>;
+  using WTile = Tile<Tr, kWT, kTile>;
+  constexpr int kF = kTile / 32;  // 16-wide fragments of a wave's quarter, per side
+  constexpr int kSteps = XTile::kK / 32;
+  __shared__ __attribute__((aligned(16))) char lds[2][2][XTile::kBytesAll];
+  const int lane = threadIdx.x & 63, wave = rfl(threadIdx.x >> 6);
+  // tiles in groups of 8 along m, m fastest: a group's x tiles and the w tile in use stay in the XCD's L2
+  const int item = xcd_item(blockIdx.x, a.tiles_m * a.tiles_n);
+  const int per = 8 * a.tiles_n, grp = item / per, in = item - grp * per;
+  const int gm = a.tiles_m - grp * 8 < 8 ? a.tiles_m - grp * 8 : 8;
+  const int tn = in / gm, tm = grp * 8 + in - tn * gm;
+  const int k0 = blockIdx.y * a.k_split, k1 = a.k - k0 < a.k_split ? a.k : k0 + a.k_split;
+  Loader<Tr, kXT, kTile, kAsync> lx;
+  Loader<Tr, kWT, kTile, kAsync> lw;
+  lx.init(a.x, a.x_stride, tm * kTile, a.m, k0, k1);
+  lw.init(a.w, a.w_stride, tn * kTile, a.n, k0, k1);
+  const int wm = (wave & 1) * kF, wn = (wave >> 1) * kF;  // first fragment of this wave
+  f32x4 acc[kF][kF];
+#pragma unroll
+  for (int i = 0; i < kF; ++i)
+#pragma unroll
+    for (int j = 0; j < kF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int nk = (k1 - k0 + XTile::kK - 1) / XTile::kK;
+  lx.issue(lds[0][0]);
+  lw.issue(lds[0][1]);
+  lx.commit(lds[0][0]);
+  lw.commit(lds[0][1]);
+  __syncthreads();
+  for (int kt = 0; kt < nk; ++kt) {
+    const int cur = kt & 1;
+    if (kt + 1 < nk) {
+      lx.advance();
+      lw.advance();
+      lx.issue(lds[cur ^ 1][0]);
+      lw.issue(lds[cur ^ 1][1]);
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      typename Tr::V8 wf[kF], xf[kF];
+#pragma unroll
+      for (int i = 0; i < kF; ++i) wf[i] = WTile::frag(lds[cur][1], wn + i, s, lane);
+#pragma unroll
+      for (int j = 0; j < kF; ++j) xf[j] = XTile::frag(lds[cur][0], wm + j, s, lane);
+#pragma unroll
+      for (int i = 0; i < kF; ++i)
+#pragma unroll
+        for (int j = 0; j < kF; ++j) acc[i][j] = mma<Tr>(wf[i], xf[j], acc[i][j]);
+    }
+    if (kt + 1 < nk) {
+      lx.commit(lds[cur ^ 1][0]);
+      lw.commit(lds[cur ^ 1][1]);
+    }
+    __syncthreads();
+  }
+
+  const int l = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int j = 0; j < kF; ++j) {
+    const int64_t m = (int64_t)tm * kTile + (wm + j) * 16 + l;
+    if (m >= a.m) continue;
+#pragma unroll
+    for (int i = 0; i < kF; ++i) {
+      const int n = tn * kTile + (wn + i) * 16 + g * 4;
+      if (a.part) {
+        float* p = a.part + ((int64_t)blockIdx.y * a.m + m) * a.n + n;
+        if (a.n - n >= 4) {
+          store4<F32>(p, acc[i][j]);
+        } else {
+          for (int e = 0; e < a.n - n; ++e) p[e] = acc[i][j][e];
+        }
+      } else {
+        epilogue<Tr>(a, m, n, acc[i][j]);
+      }
+    }
+  }
+}
+
+// Sum of the split products in order, then the epilogue: 4 consecutive n per thread.
+template <class Tr>
+__global__ __launch_bounds__(256) void split_sum_kernel(GemmArgs a, int splits) {
+  const int n4 = (a.n + 3) / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t m = i / n4;
+  if (m >= a.m) return;
+  const int n = (int)(i - m * n4) * 4, left = a.n - n;
+  f32x4 v{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; ++s) {
+    const float* p = a.part + ((int64_t)s * a.m + m) * a.n + n;
+    if (left >= 4) {
+      v += load4<F32>(p);
+    } else {
+      for (int e = 0; e < left; ++e) v[e] += p[e];
+    }
+  }
+  epilogue<Tr>(a, m, n, v);
+}
+
+// Few rows (m <= 16 kMT): the weight is read once, straight into fragments, by workgroups of 16
+// output channels whose 8 waves split K 64 elements at a time; their sums meet in LDS.
+template <class Tr, int kMT>
+__global__ __launch_bounds__(512) void rows_kernel(GemmArgs a) {
+  using T = typename Tr::T;
+  constexpr int kWaves = 8, kEpc = 16 / Tr::kBytes, kPer = 8 / kEpc;  // loads of a fragment
+  __shared__ f32x4 sum[kWaves][kMT][64];
+  const int lane = threadIdx.x & 63, wave = rfl(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const T* w = (const T*)a.w + (int64_t)(n0 + l) * a.w_stride;
+  const bool wl = n0 + l < a.n;
+  f32x4 acc[kMT];
+#pragma unroll
+  for (int j = 0; j < kMT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int k0 = wave * 64; k0 < a.k; k0 += kWaves * 64) {
+    u32x4 wf[2][kPer], xf[kMT][2][kPer];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int p = 0; p < kPer; ++p) {
+        const int k = k0 + s * 32 + g * 8 + p * kEpc;
+        wf[s][p] = wl ? load16<Tr>(w + k, a.k - k) : u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < kMT; ++j) {
+          const int m = j * 16 + l;
+          xf[j][s][p] = m < a.m ? load16<Tr>((const T*)a.x + m * a.x_stride + k, a.k - k) : u32x4{0, 0, 0, 0};
+        }
+      }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int j = 0; j < kMT; ++j)
+        acc[j] = mma<Tr>(__builtin_bit_cast(typename Tr::V8, wf[s]), __builtin_bit_cast(typename Tr::V8, xf[j][s]), acc[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < kMT; ++j) sum[wave][j][lane] = acc[j];
+  __syncthreads();
+  if (wave >= kMT) return;
+  f32x4 v = sum[0][wave][lane];
+#pragma unroll
+  for (int s = 1; s < kWaves; ++s) v += sum[s][wave][lane];
+  const int m = wave * 16 + l;
+  if (m < a.m) epilogue<Tr>(a, m, n0 + g * 4, v);
+}
+
+struct ColArgs {
+  const char* dy;
+  const char* z;   // with act: dz = dy act'(z) is stored and summed; else dy is summed
+  char* dz;
+  void* out;       // with one row group: the sums themselves
+  float* part;     // [groups][r][n]
+  int64_t dy_stride, z_stride, out_stride;
+  int m, n, r, groups, act, out_f32, dtype, chunk_blocks;
+};
+
+// Sums over the rows m % r == residue, for each column; a workgroup holds 32 chunks of columns x 8
+// rows of one residue, blockIdx.y a group of them.
+template <class Tr>
+__global__ __launch_bounds__(256) void cols_kernel(ColArgs a) {
+  using T = typename Tr::T;
+  constexpr int kEpc = 16 / Tr::kBytes;
+  __shared__ float lds[8][32 * kEpc];
+  const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
+  const int res = blockIdx.x / a.chunk_blocks, cb = blockIdx.x - res * a.chunk_blocks;
+  const int c0 = (cb * 32 + lane) * kEpc;
+  const int n = a.n - c0;
+  float acc[kEpc];
+#pragma unroll
+  for (int e = 0; e < kEpc; ++e) acc[e] = 0.f;
+  if (n > 0) {
+    for (int64_t row = res + ((int64_t)blockIdx.y * 8 + sub) * a.r; row < a.m; row += (int64_t)gridDim.y * 8 * a.r) {
+      const u32x4 u = load16<Tr>((const T*)a.dy + row * a.dy_stride + c0, n);
+      T d[kEpc];
+      __builtin_memcpy(d, &u, 16);
+      if (a.act != YK_TOK_NONE) {
+        const u32x4 uz = load16<Tr>((const T*)a.z + row * a.z_stride + c0, n);
+        T zv[kEpc];
+        __builtin_memcpy(zv, &uz, 16);
+        float f[kEpc];
+#pragma unroll
+        for (int e = 0; e < kEpc; ++e) f[e] = to_f32<Tr>(d[e]) * act_slope(to_f32<Tr>(zv[e]), a.act);
+#pragma unroll
+        for (int e = 0; e < kEpc; ++e) {
+          acc[e] += f[e];
+          d[e] = from_f32<Tr>(f[e]);
+        }
+        // dz is rounded to the operands' type: it is an operand of two matrix products
+        T* o = (T*)a.dz + row * a.n + c0;
+        if (n >= kEpc) {
+          u32x4 v;
+          __builtin_memcpy(&v, d, 16);
+          *(u32x4_any*)o = v;
+        } else {
+          for (int e = 0; e < n; ++e) o[e] = d[e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < kEpc; ++e) acc[e] += to_f32<Tr>(d[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kEpc; ++e) lds[sub][lane * kEpc + e] = acc[e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * kEpc; i += 256) {
+    const int c = cb * 32 * kEpc + i;
+    if (c >= a.n) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) v += lds[s][i];
+    if (a.part) a.part[((int64_t)blockIdx.y * a.r + res) * a.n + c] = v;
+    else if (a.out) store_param(a.out, res * a.out_stride + c, v, a.out_f32, a.dtype);
+  }
+}
+
+// The row groups' sums added in order: 64 (residue, column) pairs x 16 group ranges.
+__global__ __launch_bounds__(1024) void cols_sum_kernel(ColArgs a) {
+  __shared__ float lds[16][64];
+  const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
+  const int64_t all = (int64_t)a.r * a.n, i = (int64_t)blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (i < all)
+    for (int p = g; p < a.groups; p += 16) s += a.part[p * all + i];
+  lds[g][lane] = s;
+  __syncthreads();
+  if (g == 0 && i < all) {
+    float v = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v += lds[j][lane];
+    const int64_t row = i / a.n;
+    store_param(a.out, row * a.out_stride + (i - row * a.n), v, a.out_f32, a.dtype);
+  }
+}
+
+// ---- launch rules -----------------------------------------------------------------------------
+struct Plan {
+  int tile, splits, k_split;
+};
+constexpr int kCUs = 256;
+
+// 128 x 128 tiles where they fill the CUs, else 64 x 64; a product with too few tiles splits K
+inline Plan plan_gemm(int64_t m, int64_t n, int64_t k, int bytes) {
+  const int64_t kk = 128 / bytes;
+  Plan p;
+  p.tile = cdiv(m, 128) * cdiv(n, 128) >= kCUs ? 128 : 64;
+  const int64_t tiles = cdiv(m, p.tile) * cdiv(n, p.tile), steps = cdiv(k, kk);
+  int64_t s = 1;
+  if (tiles < kCUs) {
+    s = cdiv(2 * kCUs, tiles);
+    if (s > steps / 4) s = steps / 4;
+    if (s > 64) s = 64;
+    if (s < 1) s = 1;
+  }
+  const int64_t per = cdiv(steps, s);
+  p.splits = (int)cdiv(steps, per);
+  p.k_split = (int)(per * kk);
+  return p;
+}
+inline int64_t gemm_scratch(int64_t m, int64_t n, int64_t k, int bytes) {
+  const Plan p = plan_gemm(m, n, k, bytes);
+  return p.splits > 1 ? (int64_t)p.splits * m * n * 4 : 0;
+}
+constexpr int kFewRows = 64;
+
+template <class Tr, bool kXT, bool kWT, int kTile>
+void launch_gemm_t(const GemmArgs& a, int splits, bool async, hipStream_t st) {
+  const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), (unsigned)splits);
+  if (async) hipLaunchKernelGGL((gemm_kernel<Tr, kXT, kWT, kTile, true>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((gemm_kernel<Tr, kXT, kWT, kTile, false>), grid, dim3(256), 0, st, a);
+}
+
+// rows of 16-byte chunks whose offsets inside a tile stay below 2^31
+inline bool aligned_rows(const void* p, int64_t stride, int64_t cols, int bytes) {
+  return (uintptr_t)p % 16 == 0 && stride * bytes % 16 == 0 && cols * bytes % 16 == 0 && stride * bytes < (1 << 23);
+}
+
+// part: scratch of gemm_scratch bytes, or NULL (then K is not split)
+template <class Tr, bool kXT, bool kWT>
+void launch_gemm(GemmArgs a, float* part, hipStream_t st) {
+  Plan p = plan_gemm(a.m, a.n, a.k, Tr::kBytes);
+  if (!part) p.splits = 1;
+  if (p.splits == 1) p.k_split = a.k;
+  a.part = p.splits > 1 ? part : nullptr;
+  a.k_split = p.k_split;
+  a.tiles_m = (int)cdiv(a.m, p.tile);
+  a.tiles_n = (int)cdiv(a.n, p.tile);
+  const bool async = aligned_rows(a.x, a.x_stride, kXT ? a.m : a.k, Tr::kBytes) &&
+                     aligned_rows(a.w, a.w_stride, kWT ? a.n : a.k, Tr::kBytes);
+  if (p.tile == 128) launch_gemm_t<Tr, kXT, kWT, 128>(a, p.splits, async, st);
+  else launch_gemm_t<Tr, kXT, kWT, 64>(a, p.splits, async, st);
+  if (p.splits > 1)
+    hipLaunchKernelGGL(split_sum_kernel<Tr>, dim3((unsigned)cdiv((int64_t)a.m * cdiv(a.n, 4), 256)), dim3(256), 0, st, a,
+                       p.splits);
+}
+
+template <class Tr>
+void run_linear(const GemmArgs& a, float* part, hipStream_t st) {
+  if (a.m <= kFewRows) {
+    const dim3 grid((unsigned)cdiv(a.n, 16));
+    if (a.m <= 16) hipLaunchKernelGGL((rows_kernel<Tr, 1>), grid, dim3(512), 0, st, a);
+    else if (a.m <= 32) hipLaunchKernelGGL((rows_kernel<Tr, 2>), grid, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((rows_kernel<Tr, 4>), grid, dim3(512), 0, st, a);
+    return;
+  }
+  launch_gemm<Tr, false, false>(a, part, st);
+}
+
+// Row groups of the column sums: enough workgroups for the chip, at least 32 rows each
+inline int col_groups(int64_t m, int64_t n, int64_t r, int bytes) {
+  const int64_t wgs = r * cdiv(n, 32 * (16 / bytes)), rows = cdiv(m, r);
+  int64_t g = cdiv(4 * kCUs, wgs);
+  if (g > cdiv(rows, 32)) g = cdiv(rows, 32);
+  return (int)(g < 1 ? 1 : g > 512 ? 512 : g);
+}
+template <class Tr>
+void run_cols(ColArgs c, float* part, hipStream_t st) {
+  c.groups = col_groups(c.m, c.n, c.r, Tr::kBytes);
+  c.chunk_blocks = (int)cdiv(c.n, 32 * (16 / Tr::kBytes));
+  c.part = c.out && c.groups > 1 ? part : nullptr;
+  hipLaunchKernelGGL(cols_kernel<Tr>, dim3((unsigned)(c.chunk_blocks * (int64_t)c.r), (unsigned)c.groups), dim3(256), 0, st, c);
+  if (c.part)
+    hipLaunchKernelGGL(cols_sum_kernel, dim3((unsigned)cdiv((int64_t)c.r * c.n, 64)), dim3(1024), 0, st, c);
+}
+
+template <class Tr>
+void run_linear_grad(const yk_linear_grad_args& g, hipStream_t st) {
+  const bool act = g.act != YK_TOK_NONE;
+  char* ws = (char*)g.ws;
+  char* dz = (char*)g.dy;
+  int64_t dz_stride = g.dy_stride;
+  if (act) {
+    dz = ws;
+    dz_stride = g.n;
+    ws += cdiv(g.m * g.n * Tr::kBytes, 16) * 16;
+  }
+  float* part = (float*)ws;  // one region: the kernels that use it follow each other on the stream
+  if (act || g.dbias) {
+    ColArgs c{(const char*)g.dy, (const char*)g.z, dz, g.dbias, nullptr, g.dy_stride, g.z_stride, g.n, (int)g.m,
+              (int)g.n, 1, 1, g.act, g.bias_f32 || Tr::kBytes == 4, g.dtype, 1};
+    run_cols<Tr>(c, part, st);
+  }
+  if (g.dres) {
+    ColArgs c{(const char*)g.dy, nullptr, nullptr, g.dres, nullptr, g.dy_stride, 0, g.dres_stride, (int)g.m,
+              (int)g.n, (int)g.res_rows, 1, YK_TOK_NONE, Tr::kBytes == 4, g.dtype, 1};
+    run_cols<Tr>(c, part, st);
+  }
+  if (g.dx) {
+    GemmArgs a{};
+    a.x = dz, a.x_stride = dz_stride;
+    a.w = (const char*)g.w, a.w_stride = g.w_stride;
+    a.y = (char*)g.dx, a.y_stride = g.dx_stride;
+    a.m = (int)g.m, a.n = (int)g.k, a.k = (int)g.n, a.dtype = g.dtype;
+    launch_gemm<Tr, false, true>(a, part, st);
+  }
+  if (g.dw) {
+    GemmArgs a{};
+    a.x = dz, a.x_stride = dz_stride;
+    a.w = (const char*)g.x, a.w_stride = g.x_stride;
+    a.y = (char*)g.dw, a.y_stride = g.dw_stride;
+    a.m = (int)g.n, a.n = (int)g.k, a.k = (int)g.m, a.dtype = g.dtype;
+    launch_gemm<Tr, true, true>(a, part, st);
+  }
+}
+
+int check_linear(const char* fn, int dtype, int act, int64_t m, int64_t n, int64_t k) {
+  YK_CHECK_ARG(tok_bytes(dtype), std::string(fn) + ": dtype must be YK_ACT_BF16, YK_ACT_F32 or YK_ACT_F16");
+  YK_CHECK_ARG(act >= YK_TOK_NONE && act <= YK_TOK_RELU, std::string(fn) + ": bad activation");
+  YK_CHECK_ARG(m >= 0 && m < (1 << 30) && n >= 1 && n < (1 << 30) && k >= 1 && k < (1 << 30),
+               std::string(fn) + ": sizes out of range (m in [0, 2^30), n and k in [1, 2^30))");
+  YK_CHECK_ARG(cdiv(m, 64) * cdiv(n, 64) < (int64_t(1) << 31) && cdiv(m, 64) * cdiv(k, 64) < (int64_t(1) << 31) &&
+                   cdiv(n, 64) * cdiv(k, 64) < (int64_t(1) << 31),
+               std::string(fn) + ": more tiles than a launch holds");
+  return YK_OK;
+}
+
+}  // namespace tok
+}  // namespace yk
+
+using namespace yk::tok;
+
+extern "C" {
+
+int yk_linear_workspace(const yk_linear_args* a, int64_t* bytes) {
+  YK_CHECK_ARG(a && bytes, "yk_linear_workspace: NULL argument");
+  if (const int rc = check_linear("yk_linear_workspace", a->dtype, a->act, a->m, a->n, a->k)) return rc;
+  *bytes = a->m <= kFewRows ? 0 : gemm_scratch(a->m, a->n, a->k, tok_bytes(a->dtype));
+  return YK_OK;
+}
+
+int yk_linear(yk_ctx* ctx, const yk_linear_args* a, void* stream) {
+  YK_CHECK_ARG(ctx && a, "yk_linear: NULL argument");
+  if (const int rc = check_linear("yk_linear", a->dtype, a->act, a->m, a->n, a->k)) return rc;
+  if (a->m == 0) return YK_OK;
+  YK_CHECK_ARG(a->x && a->w && a->y, "yk_linear: x, w and y must be set");
+  YK_CHECK_ARG(!a->res || (a->res_rows >= 1 && a->res_rows <= a->m), "yk_linear: res_rows must be in [1, m]");
+  YK_CHECK_ARG(a->x_stride >= 0 && a->w_stride >= 0 && (!a->res || a->res_stride >= 0) &&
+                   (a->m == 1 || (a->y_stride >= a->n && (!a->z || a->z_stride >= a->n))),
+               "yk_linear: a negative row stride, or an output's is shorter than its row");
+  int64_t need = 0;
+  if (const int rc = yk_linear_workspace(a, &need)) return rc;
+  YK_CHECK_ARG(need == 0 || !a->ws || (a->ws_bytes >= need && (uintptr_t)a->ws % 16 == 0),
+               "yk_linear: ws must be yk_linear_workspace bytes, 16-byte aligned (or NULL: K is not split)");
+  yk::DeviceGuard g(ctx->device);
+  GemmArgs k{(const char*)a->x, (const char*)a->w, a->bias, (const char*)a->res, (char*)a->y, (char*)a->z, nullptr,
+             a->x_stride, a->w_stride, a->res_stride, a->y_stride, a->z_stride, (int)a->m, (int)a->n, (int)a->k,
+             (int)a->res_rows, a->act, a->bias_f32 || a->dtype == YK_ACT_F32, a->dtype, 0, 0, 0};
+  float* part = need ? (float*)a->ws : nullptr;
+  const hipStream_t st = (hipStream_t)stream;
+  if (a->dtype == YK_ACT_F32) run_linear<F32>(k, part, st);
+  else if (a->dtype == YK_ACT_BF16) run_linear<B16>(k, part, st);
+  else run_linear<H16>(k, part, st);
+  return launched("yk_linear");
+}
+
+int yk_linear_backward_workspace(const yk_linear_grad_args* a, int64_t* bytes) {
+  YK_CHECK_ARG(a && bytes, "yk_linear_backward_workspace: NULL argument");
+  if (const int rc = check_linear("yk_linear_backward_workspace", a->dtype, a->act, a->m, a->n, a->k)) return rc;
+  YK_CHECK_ARG(!a->dres || (a->res_rows >= 1 && a->res_rows <= a->m), "yk_linear_backward_workspace: res_rows must be in [1, m]");
+  const int e = tok_bytes(a->dtype);
+  int64_t part = 0;
+  auto grow = [&](int64_t b) { part = b > part ? b : part; };
+  if (a->m) {
+    if (a->dbias) grow(col_groups(a->m, a->n, 1, e) * a->n * 4);
+    if (a->dres) grow((int64_t)col_groups(a->m, a->n, a->res_rows, e) * a->res_rows * a->n * 4);
+    if (a->dx) grow(gemm_scratch(a->m, a->k, a->n, e));
+    if (a->dw) grow(gemm_scratch(a->n, a->k, a->m, e));
+    if (a->act != YK_TOK_NONE) part += cdiv(a->m * a->n * e, 16) * 16;
+  }
+  *bytes = part;
+  return YK_OK;
+}
+
+int yk_linear_backward(yk_ctx* ctx, const yk_linear_grad_args* a, void* stream) {
+  YK_CHECK_ARG(ctx && a, "yk_linear_backward: NULL argument");
+  if (const int rc = check_linear("yk_linear_backward", a->dtype, a->act, a->m, a->n, a->k)) return rc;
+  if (!a->dx && !a->dw && !a->dbias && !a->dres) return YK_OK;
+  YK_CHECK_ARG(a->m >= 1, "yk_linear_backward: m must be >= 1");
+  YK_CHECK_ARG(a->dy && (a->act == YK_TOK_NONE || a->z) && (!a->dx || a->w) && (!a->dw || a->x),
+               "yk_linear_backward: an input that the requested gradients need is NULL");
+  YK_CHECK_ARG(a->dy_stride >= 0 && a->x_stride >= 0 && a->w_stride >= 0 && a->z_stride >= 0 &&
+                   (!a->dx || a->m == 1 || a->dx_stride >= a->k) && (!a->dw || a->n == 1 || a->dw_stride >= a->k) &&
+                   (!a->dres || a->res_rows == 1 || a->dres_stride >= a->n),
+               "yk_linear_backward: a negative row stride, or an output's is shorter than its row");
+  int64_t need = 0;
+  if (const int rc = yk_linear_backward_workspace(a, &need)) return rc;
+  YK_CHECK_ARG(need == 0 || (a->ws && a->ws_bytes >= need && (uintptr_t)a->ws % 16 == 0),
+               "yk_linear_backward: ws must be yk_linear_backward_workspace bytes, 16-byte aligned");
+  yk::DeviceGuard g(ctx->device);
+  const hipStream_t st = (hipStream_t)stream;
+  if (a->dtype == YK_ACT_F32) run_linear_grad<F32>(*a, st);
+  else if (a->dtype == YK_ACT_BF16) run_linear_grad<B16>(*a, st);
+  else run_linear_grad<H16>(*a, st);
+  return launched("yk_linear_backward");
+}
+
+}  // extern "C"

@@ -68,6 +68,12 @@ int64_t yk_struct_size(int which) {
     case 9: return (int64_t)sizeof(yk_gmd_stats);
     case 10: return (int64_t)sizeof(yk_tensor);
     case 11: return (int64_t)sizeof(yk_track_event);
+    case 12: return (int64_t)sizeof(yk_linear_args);
+    case 13: return (int64_t)sizeof(yk_linear_grad_args);
+    case 14: return (int64_t)sizeof(yk_layer_norm_args);
+    case 15: return (int64_t)sizeof(yk_layer_norm_grad_args);
+    case 16: return (int64_t)sizeof(yk_attention_args);
+    case 17: return (int64_t)sizeof(yk_attention_grad_args);
     default: return -1;
   }
 }
