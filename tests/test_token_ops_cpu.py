@@ -40,7 +40,7 @@ AGRAD = dict(ATT, go=64, lse=64, dq=64, dk=64, dv=64)
     ("yk_linear", LIN, dict(y=None)), ("yk_linear", LIN, dict(y_stride=39)), ("yk_linear", LIN, dict(x_stride=-30)),
     ("yk_linear", LIN, dict(res=64, res_rows=0, res_stride=40)), ("yk_linear", LIN, dict(res=64, res_rows=101, res_stride=40)),
     ("yk_linear", LIN, dict(m=1 << 29, n=1 << 29, y_stride=1 << 29)),
-    ("yk_linear", dict(LIN, k=4096, x_stride=4096, w_stride=4096), dict(ws=64, ws_bytes=16)),
+    ("yk_linear", dict(LIN, k=4096, x_stride=4096, w_stride=4096), dict(ws=68, ws_bytes=16)),
     ("yk_linear_backward", GRAD, dict(dtype=2)), ("yk_linear_backward", GRAD, dict(m=0)),
     ("yk_linear_backward", GRAD, dict(act=2)), ("yk_linear_backward", GRAD, dict(w=None)),
     ("yk_linear_backward", GRAD, dict(dx_stride=29)), ("yk_linear_backward", GRAD, dict(dres=64, res_rows=101)),
@@ -91,6 +91,18 @@ def test_workspace_sizes():
     rc, n = need("yk_attention", **{**ATT, "nq": 1, "nk": 20480})
     assert rc == 0 and n > 0
     assert need("yk_attention_backward", **AGRAD) == (0, 2 * 2 * 4 * 9 * 4)
+
+
+def test_packed_arguments_match_the_structs():
+    """ops.py hands the argument structs over as packed bytes: same size, same place of the scratch."""
+    ops = pkg().ops
+    for fn, s in (("yk_linear", ops._LINEAR), ("yk_linear_backward", ops._LINEAR_GRAD), ("yk_layer_norm_backward", ops._NORM_GRAD),
+                  ("yk_attention", ops._ATTENTION), ("yk_attention_backward", ops._ATTENTION_GRAD)):
+        t = L.TOKEN_ARGS[fn]
+        assert s.size == t.ws.offset and s.size + ops._WS.size == C.sizeof(t), fn
+    assert ops._NORM.size == C.sizeof(L.LayerNormArgs)
+    a = L.LinearArgs.from_buffer_copy(ops._LINEAR.pack(*range(1, 20)) + ops._WS.pack(20, 21))
+    assert [getattr(a, n) for n, _ in a._fields_] == list(range(1, 22))
 
 
 def test_no_gpu_tensors():

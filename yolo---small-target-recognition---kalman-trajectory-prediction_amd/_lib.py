@@ -257,9 +257,9 @@ _SIGS = {
     "yk_nms_candidates": ([_vp, C.c_int, C.c_float, C.c_int, _vp, _vp, _vp, _vp], C.c_int),
     "yk_model_nms_stats": ([_vp, _vp, C.c_int, _vp], C.c_int),
     "yk_model_check": ([_vp, _vp], C.c_int),
-    **{fn: ([_vp, C.POINTER(t), _vp], C.c_int) for fn, t in TOKEN_ARGS.items()},
-    **{fn + "_workspace": ([C.POINTER(t), C.POINTER(C.c_int64)], C.c_int) for fn, t in TOKEN_ARGS.items()
-       if t is not LayerNormArgs},
+    # (the argument struct by address: ops.py hands over packed bytes)
+    **{fn: ([_vp, _vp, _vp], C.c_int) for fn in TOKEN_ARGS},
+    **{fn + "_workspace": ([_vp, C.POINTER(C.c_int64)], C.c_int) for fn in TOKEN_ARGS if fn != "yk_layer_norm"},
 }
 
 _lock = threading.Lock()

@@ -20,8 +20,6 @@
 namespace yk {
 namespace tok {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
-
 struct AttnArgs {
   const char *q, *k, *v, *o, *go;
   char *out, *dq, *dk, *dv;

@@ -26,36 +26,44 @@ struct GemmArgs {
   int tiles_m, tiles_n, k_split;  // k_split: K elements per blockIdx.y
 };
 
-// bias, activation, residual and the stores of 4 consecutive n of one m
+// z, activation, residual and the stores of 8 consecutive n of one m, from sums that hold the bias
 template <class Tr>
-__device__ __forceinline__ void epilogue(const GemmArgs& a, int64_t m, int n, f32x4 v) {
+__device__ __forceinline__ void epilogue(const GemmArgs& a, int64_t m, int n, float* v) {
   using T = typename Tr::T;
   const int left = a.n - n;
-  if (left <= 0) return;
-  if (a.bias) {
+  T* y = (T*)a.y + m * a.y_stride + n;
+  T* z = a.z ? (T*)a.z + m * a.z_stride + n : nullptr;
+  const T* res = a.res ? (const T*)a.res + (a.res_rows == a.m ? m : m % a.res_rows) * a.res_stride + n : nullptr;
+  if (left >= 8) {
+    if (z) store8<Tr>(z, v);
+    if (a.act != YK_TOK_NONE) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < left) v[i] += load_param(a.bias, n + i, a.bias_f32, a.dtype);
-  }
-  if (a.z) {
-    T* z = (T*)a.z + m * a.z_stride + n;
-    if (left >= 4) {
-      store4<Tr>(z, v);
-    } else {
-      for (int i = 0; i < left; ++i) z[i] = from_f32<Tr>(v[i]);
+      for (int e = 0; e < 8; ++e) v[e] = act_f32(v[e], a.act);
+    }
+    if (res) add8<Tr>(res, v);
+    store8<Tr>(y, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (e >= left) continue;
+      if (z) z[e] = from_f32<Tr>(v[e]);
+      const float r = act_f32(v[e], a.act);
+      y[e] = from_f32<Tr>(res ? r + to_f32<Tr>(res[e]) : r);
     }
   }
-  if (a.act != YK_TOK_NONE) {
+}
+__device__ __forceinline__ void bias8(const GemmArgs& a, int n, float* b) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = act_f32(v[i], a.act);
-  }
-  T* y = (T*)a.y + m * a.y_stride + n;
-  const T* res = a.res ? (const T*)a.res + (a.res_rows == a.m ? m : m % a.res_rows) * a.res_stride + n : nullptr;
-  if (left >= 4) {
-    if (res) v += load4<Tr>(res);
-    store4<Tr>(y, v);
+  for (int e = 0; e < 8; ++e) b[e] = 0.f;
+  if (!a.bias) return;
+  if (a.n - n >= 8) {
+    if (a.bias_f32) add8<F32>((const float*)a.bias + n, b);
+    else if (a.dtype == YK_ACT_BF16) add8<B16>((const unsigned short*)a.bias + n, b);
+    else add8<H16>((const _Float16*)a.bias + n, b);
   } else {
-    for (int i = 0; i < left; ++i) y[i] = from_f32<Tr>(v[i] + (res ? to_f32<Tr>(res[i]) : 0.f));
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (n + e < a.n) b[e] = load_param(a.bias, n + e, a.bias_f32, a.dtype);
   }
 }
 
@@ -119,17 +127,19 @@ struct Tile {
   }
 };
 
-// The loads of one operand's tiles by 256 threads.  kAsync: straight from memory to LDS through a
+// The loads of one operand's tiles by kThreads threads.  kAsync: straight from memory to LDS through a
 // buffer descriptor, whose range check turns a chunk outside the matrix into zeros; needs 16-byte
 // aligned rows and whole chunks.  Otherwise through registers, any alignment.
-template <class Tr, bool kTrans, int kRows, bool kAsync>
+template <class Tr, bool kTrans, int kRows, int kThreads, bool kAsync>
 struct Loader {
   using Tl = Tile<Tr, kTrans, kRows>;
   using T = typename Tr::T;
-  static constexpr int kN = Tl::kChunks / 256;
+  static constexpr int kN = Tl::kChunks / kThreads;
+  static constexpr unsigned kOut = 0x80000000u;  // past every descriptor's range
   const T* base;       // first stored row / column of this workgroup's tiles
   int64_t stride;
   int rows, cols;      // stored rows / columns left from there
+  unsigned off[kAsync ? kN : 1];  // byte offset of each chunk, kOut where m (n) ends before it
   u32x4 reg[kAsync ? 1 : kN];
 
   __device__ __forceinline__ void init(const char* p, int64_t s, int r0, int m, int k0, int k1) {
@@ -142,6 +152,14 @@ struct Loader {
       base = (const T*)p + (int64_t)r0 * s + k0;
       rows = m - r0;
       cols = k1 - k0;
+    }
+    if constexpr (kAsync) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        int row, col;
+        Tl::locate(i * kThreads + threadIdx.x, row, col);
+        off[i] = (kTrans ? col < cols : row < rows) ? (unsigned)((row * (int)stride + col) * Tr::kBytes) : kOut;
+      }
     }
   }
   __device__ __forceinline__ void advance() {
@@ -156,24 +174,29 @@ struct Loader {
   __device__ __forceinline__ void issue(char* lds) {
     const int tid = threadIdx.x;
     if constexpr (kAsync) {
-      const int64_t span = ((int64_t)(rows - 1) * stride + cols) * Tr::kBytes;
+      // (nothing left: every chunk lands as zeros)
+      const int64_t span = rows > 0 && cols > 0 ? ((int64_t)(rows - 1) * stride + cols) * Tr::kBytes : 0;
       const int bytes = rfl((int)(span < 0x7ffffff0 ? span : 0x7ffffff0));
       const size_t b = (size_t)base;
       const size_t ub = ((size_t)(unsigned)rfl((int)(b >> 32)) << 32) | (unsigned)rfl((int)b);
       const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)ub, (short)0, bytes, 0x00020000);
+      const bool tail = (kTrans ? rows : cols) < Tl::kK;  // K ends inside this tile
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
-        int row, col;
-        Tl::locate(i * 256 + tid, row, col);
-        const unsigned off = row < rows && col < cols ? (unsigned)((row * (int)stride + col) * Tr::kBytes) : 0x80000000u;
+        unsigned o = off[i];
+        if (tail) {
+          int row, col;
+          Tl::locate(i * kThreads + tid, row, col);
+          if ((kTrans ? row : col) >= (kTrans ? rows : cols)) o = kOut;
+        }
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rsrc, (__attribute__((address_space(3))) void*)(lds + (i * 256 + rfl(tid & ~63)) * 16), 16, off, 0, 0, 0);
+            rsrc, (__attribute__((address_space(3))) void*)(lds + (i * kThreads + rfl(tid & ~63)) * 16), 16, o, 0, 0, 0);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
         int row, col;
-        Tl::locate(i * 256 + tid, row, col);
+        Tl::locate(i * kThreads + tid, row, col);
         reg[i] = row < rows ? load16<Tr>(base + row * stride + col, cols - col) : u32x4{0, 0, 0, 0};
       }
     }
@@ -181,18 +204,32 @@ struct Loader {
   __device__ __forceinline__ void commit(char* lds) {
     if constexpr (!kAsync) {
 #pragma unroll
-      for (int i = 0; i < kN; ++i) *(u32x4*)(lds + (i * 256 + threadIdx.x) * 16) = reg[i];
+      for (int i = 0; i < kN; ++i) *(u32x4*)(lds + (i * kThreads + threadIdx.x) * 16) = reg[i];
     }
   }
 };
 
-template <class Tr, bool kXT, bool kWT, int kTile, bool kAsync>
-__global__ __launch_bounds__(256) void gemm_kernel(GemmArgs a) {
-  using XTile = Tile<Tr, kXT, kTile>;
-  using WTile = Tile<Tr, kWT, kTile>;
-  constexpr int kF = kTile / 32;  // 16-wide fragments of a wave's quarter, per side
+// Until this wave's loads but the last kLeft have landed, and its LDS reads are done; then until all
+// waves are there.
+template <int kLeft>
+__device__ __forceinline__ void loads_landed() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLeft) : "memory");
+  __builtin_amdgcn_s_barrier();
+}
+
+// kTM x kTN tile of C by kWM x kWN waves.  kAsync: kStages - 1 tiles of K in flight, one barrier per
+// tile; a buffer is filled again after the barrier that follows its last read.
+template <class Tr, bool kXT, bool kWT, int kTM, int kTN, int kWM, int kWN, int kStages, bool kAsync>
+__global__ __launch_bounds__(64 * kWM * kWN) void gemm_kernel(GemmArgs a) {
+  using XTile = Tile<Tr, kXT, kTM>;
+  using WTile = Tile<Tr, kWT, kTN>;
+  constexpr int kThreads = 64 * kWM * kWN;
+  constexpr int kFM = kTM / (16 * kWM), kFN = kTN / (16 * kWN);  // 16-wide fragments of a wave, per side
   constexpr int kSteps = XTile::kK / 32;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][XTile::kBytesAll];
+  // one array for both operands' tiles: with two, the compiler waits for every load in flight before
+  // it reads either
+  constexpr int kBuf = XTile::kBytesAll + WTile::kBytesAll;
+  __shared__ __attribute__((aligned(16))) char lds[kStages][kBuf];
   const int lane = threadIdx.x & 63, wave = rfl(threadIdx.x >> 6);
   // tiles in groups of 8 along m, m fastest: a group's x tiles and the w tile in use stay in the XCD's L2
   const int item = xcd_item(blockIdx.x, a.tiles_m * a.tiles_n);
@@ -200,87 +237,136 @@ __global__ __launch_bounds__(256) void gemm_kernel(GemmArgs a) {
   const int gm = a.tiles_m - grp * 8 < 8 ? a.tiles_m - grp * 8 : 8;
   const int tn = in / gm, tm = grp * 8 + in - tn * gm;
   const int k0 = blockIdx.y * a.k_split, k1 = a.k - k0 < a.k_split ? a.k : k0 + a.k_split;
-  Loader<Tr, kXT, kTile, kAsync> lx;
-  Loader<Tr, kWT, kTile, kAsync> lw;
-  lx.init(a.x, a.x_stride, tm * kTile, a.m, k0, k1);
-  lw.init(a.w, a.w_stride, tn * kTile, a.n, k0, k1);
-  const int wm = (wave & 1) * kF, wn = (wave >> 1) * kF;  // first fragment of this wave
-  f32x4 acc[kF][kF];
+  Loader<Tr, kXT, kTM, kThreads, kAsync> lx;
+  Loader<Tr, kWT, kTN, kThreads, kAsync> lw;
+  lx.init(a.x, a.x_stride, tm * kTM, a.m, k0, k1);
+  lw.init(a.w, a.w_stride, tn * kTN, a.n, k0, k1);
+  const int wm = wave % kWM * kFM, wn = wave / kWM * kFN;  // first fragment of this wave
+  f32x4 acc[kFN][kFM];
 #pragma unroll
-  for (int i = 0; i < kF; ++i)
+  for (int i = 0; i < kFN; ++i)
 #pragma unroll
-    for (int j = 0; j < kF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < kFM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   const int nk = (k1 - k0 + XTile::kK - 1) / XTile::kK;
-  lx.issue(lds[0][0]);
-  lw.issue(lds[0][1]);
-  lx.commit(lds[0][0]);
-  lw.commit(lds[0][1]);
-  __syncthreads();
-  for (int kt = 0; kt < nk; ++kt) {
-    const int cur = kt & 1;
-    if (kt + 1 < nk) {
-      lx.advance();
-      lw.advance();
-      lx.issue(lds[cur ^ 1][0]);
-      lw.issue(lds[cur ^ 1][1]);
-    }
+  // one tile of K; `between`: the next tile's loads, behind the first LDS reads
+  auto compute = [&](const char* buf, auto&& between) {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      typename Tr::V8 wf[kF], xf[kF];
+      typename Tr::V8 wf[kFN], xf[kFM];
 #pragma unroll
-      for (int i = 0; i < kF; ++i) wf[i] = WTile::frag(lds[cur][1], wn + i, s, lane);
+      for (int i = 0; i < kFN; ++i) wf[i] = WTile::frag(buf + XTile::kBytesAll, wn + i, s, lane);
 #pragma unroll
-      for (int j = 0; j < kF; ++j) xf[j] = XTile::frag(lds[cur][0], wm + j, s, lane);
+      for (int j = 0; j < kFM; ++j) xf[j] = XTile::frag(buf, wm + j, s, lane);
+      if (s == 0) between();
 #pragma unroll
-      for (int i = 0; i < kF; ++i)
+      for (int j = 0; j < kFM; ++j)
 #pragma unroll
-        for (int j = 0; j < kF; ++j) acc[i][j] = mma<Tr>(wf[i], xf[j], acc[i][j]);
+        for (int i = 0; i < kFN; ++i) acc[i][j] = mma<Tr>(wf[i], xf[j], acc[i][j]);
     }
-    if (kt + 1 < nk) {
-      lx.commit(lds[cur ^ 1][0]);
-      lw.commit(lds[cur ^ 1][1]);
+  };
+  if constexpr (kAsync) {
+    constexpr int kLoads = decltype(lx)::kN + decltype(lw)::kN;
+    auto issue = [&](int buf) {
+      lx.issue(lds[buf]);
+      lw.issue(lds[buf] + XTile::kBytesAll);
+      lx.advance();
+      lw.advance();
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(i);
+    int cur = 0, fill = kStages - 1;
+    for (int kt = 0; kt < nk; ++kt) {
+      loads_landed<(kStages - 2) * kLoads>();
+      compute(lds[cur], [&] { issue(fill); });
+      fill = cur;
+      cur = cur + 1 == kStages ? 0 : cur + 1;
     }
+    loads_landed<0>();
+  } else {
+    lx.issue(lds[0]);
+    lw.issue(lds[0] + XTile::kBytesAll);
+    lx.commit(lds[0]);
+    lw.commit(lds[0] + XTile::kBytesAll);
     __syncthreads();
+    for (int kt = 0; kt < nk; ++kt) {
+      const int cur = kt & 1;
+      if (kt + 1 < nk) {
+        lx.advance();
+        lw.advance();
+        lx.issue(lds[cur ^ 1]);
+        lw.issue(lds[cur ^ 1] + XTile::kBytesAll);
+      }
+      compute(lds[cur], [] {});
+      if (kt + 1 < nk) {
+        lx.commit(lds[cur ^ 1]);
+        lw.commit(lds[cur ^ 1] + XTile::kBytesAll);
+      }
+      __syncthreads();
+    }
   }
 
-  const int l = lane & 15, g = lane >> 4;
+  // The accumulators pass through LDS 32 rows at a time (each wave in a part of its own), so that
+  // a lane finishes 8 neighbouring n and a row's stores and residual reads are whole lines.
+  constexpr int kPass = 2, kPitch = kFN * 16 + 4, kCh = kFN * 2, kStepRows = 64 / kCh;
+  static_assert(kFM % kPass == 0 && kWM * kWN * kPass * 16 * kPitch * 4 <= kStages * kBuf, "the rows in transit fit the tiles' LDS");
+  float* buf = (float*)&lds[0][0] + wave * kPass * 16 * kPitch;
+  const int l = lane & 15, g = lane >> 4, c = lane % kCh, n = tn * kTN + wn * 16 + c * 8;
+  float b[8];
+  bias8(a, n, b);
 #pragma unroll
-  for (int j = 0; j < kF; ++j) {
-    const int64_t m = (int64_t)tm * kTile + (wm + j) * 16 + l;
-    if (m >= a.m) continue;
+  for (int j0 = 0; j0 < kFM; j0 += kPass) {
 #pragma unroll
-    for (int i = 0; i < kF; ++i) {
-      const int n = tn * kTile + (wn + i) * 16 + g * 4;
+    for (int j = 0; j < kPass; ++j)
+#pragma unroll
+      for (int i = 0; i < kFN; ++i) *(f32x4*)(buf + (j * 16 + l) * kPitch + i * 16 + g * 4) = acc[i][j0 + j];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int h = 0; h < kPass * 16 / kStepRows; ++h) {
+      const int row = h * kStepRows + lane / kCh;
+      const int64_t m = (int64_t)tm * kTM + (wm + j0) * 16 + row;
+      const f32x4 lo = *(const f32x4*)(buf + row * kPitch + c * 8), hi = *(const f32x4*)(buf + row * kPitch + c * 8 + 4);
+      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      if (m >= a.m || n >= a.n) continue;
       if (a.part) {
         float* p = a.part + ((int64_t)blockIdx.y * a.m + m) * a.n + n;
-        if (a.n - n >= 4) {
-          store4<F32>(p, acc[i][j]);
+        if (a.n - n >= 8) {
+          store8<F32>(p, v);
         } else {
-          for (int e = 0; e < a.n - n; ++e) p[e] = acc[i][j][e];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e < a.n) p[e] = v[e];
         }
       } else {
-        epilogue<Tr>(a, m, n, acc[i][j]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += b[e];
+        epilogue<Tr>(a, m, n, v);
       }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
-// Sum of the split products in order, then the epilogue: 4 consecutive n per thread.
+// Sum of the split products in order, then the epilogue: 8 consecutive n per thread.
 template <class Tr>
 __global__ __launch_bounds__(256) void split_sum_kernel(GemmArgs a, int splits) {
-  const int n4 = (a.n + 3) / 4;
+  const int n8 = (a.n + 7) / 8;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t m = i / n4;
+  const int64_t m = i / n8;
   if (m >= a.m) return;
-  const int n = (int)(i - m * n4) * 4, left = a.n - n;
-  f32x4 v{0.f, 0.f, 0.f, 0.f};
+  const int n = (int)(i - m * n8) * 8, left = a.n - n;
+  float v[8];
+  bias8(a, n, v);
   for (int s = 0; s < splits; ++s) {
     const float* p = a.part + ((int64_t)s * a.m + m) * a.n + n;
-    if (left >= 4) {
-      v += load4<F32>(p);
+    if (left >= 8) {
+      add8<F32>(p, v);
     } else {
-      for (int e = 0; e < left; ++e) v[e] += p[e];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < left) v[e] += p[e];
     }
   }
   epilogue<Tr>(a, m, n, v);
@@ -292,7 +378,7 @@ template <class Tr, int kMT>
 __global__ __launch_bounds__(512) void rows_kernel(GemmArgs a) {
   using T = typename Tr::T;
   constexpr int kWaves = 8, kEpc = 16 / Tr::kBytes, kPer = 8 / kEpc;  // loads of a fragment
-  __shared__ f32x4 sum[kWaves][kMT][64];
+  __shared__ __attribute__((aligned(16))) float sum[kWaves][16 * kMT][20];
   const int lane = threadIdx.x & 63, wave = rfl(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16;
   const T* w = (const T*)a.w + (int64_t)(n0 + l) * a.w_stride;
@@ -322,14 +408,17 @@ __global__ __launch_bounds__(512) void rows_kernel(GemmArgs a) {
         acc[j] = mma<Tr>(__builtin_bit_cast(typename Tr::V8, wf[s]), __builtin_bit_cast(typename Tr::V8, xf[j][s]), acc[j]);
   }
 #pragma unroll
-  for (int j = 0; j < kMT; ++j) sum[wave][j][lane] = acc[j];
+  for (int j = 0; j < kMT; ++j) *(f32x4*)&sum[wave][j * 16 + l][g * 4] = acc[j];
   __syncthreads();
-  if (wave >= kMT) return;
-  f32x4 v = sum[0][wave][lane];
+  const int m = threadIdx.x >> 1, n = n0 + (threadIdx.x & 1) * 8;
+  if (m >= a.m || n >= a.n) return;  // (m < 16 kMT: a.m is at most that)
+  float v[8];
+  bias8(a, n, v);
 #pragma unroll
-  for (int s = 1; s < kWaves; ++s) v += sum[s][wave][lane];
-  const int m = wave * 16 + l;
-  if (m < a.m) epilogue<Tr>(a, m, n0 + g * 4, v);
+  for (int s = 0; s < kWaves; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += sum[s][m][n - n0 + e];
+  epilogue<Tr>(a, m, n, v);
 }
 
 struct ColArgs {
@@ -427,63 +516,103 @@ struct Plan {
 };
 constexpr int kCUs = 256;
 
-// 128 x 128 tiles where they fill the CUs, else 64 x 64; a product with too few tiles splits K
-inline Plan plan_gemm(int64_t m, int64_t n, int64_t k, int bytes) {
-  const int64_t kk = 128 / bytes;
-  Plan p;
-  p.tile = cdiv(m, 128) * cdiv(n, 128) >= kCUs ? 128 : 64;
-  const int64_t tiles = cdiv(m, p.tile) * cdiv(n, p.tile), steps = cdiv(k, kk);
-  int64_t s = 1;
-  if (tiles < kCUs) {
-    s = cdiv(2 * kCUs, tiles);
-    if (s > steps / 4) s = steps / 4;
-    if (s > 64) s = 64;
-    if (s < 1) s = 1;
+// Time of a product by tile size, from sweeps of tile and split on this card (microseconds; a step
+// is 64 of K for the 16-bit types, 32 for float32): `alone` per step for the only workgroup of
+// its CU (its loads' latency), `shared` per step and workgroup where `per_cu` of them share it
+// (the CU's load rate; the MFMAs for float32), `ends` / `ends_shared` for the first loads and the
+// epilogue.  16-bit, 4096 x 1024 x 4096: 128-tiles 49 us, 64-tiles 50, 256-tiles 95 (64 of them on
+// 256 CUs); 40960 x 4096 x 1024: 360 / 394 (256 / 128); 1000^3: 8.8 / 13.7 (64 / 128); float32
+// 10240 x 2048 x 512: 186 / 203 (64 / 128).
+struct TileTime {
+  int tile, per_cu;
+  double alone, shared, ends, ends_shared;
+};
+constexpr TileTime kTimes16[] = {{256, 1, 1.5, 1.5, 12, 12}, {128, 2, 0.7, 0.44, 4.5, 2.6}, {64, 4, 0.35, 0.19, 2.5, 0.8}};
+constexpr TileTime kTimes32[] = {{128, 2, 2.15, 2.05, 5, 3.5}, {64, 4, 0.72, 0.52, 2.5, 1}};
+
+// The tile and the split of K that the table says are fastest.  trans: operands that lie transposed
+// (their fragments take twice the LDS reads, which shows where a workgroup is alone: 2048 x 512 x
+// 10240, both transposed, 256 64-tiles: 103 us, split in 4: 45).  A split costs a launch and its
+// float32 sums once written and once read.
+inline Plan plan_gemm(int64_t m, int64_t n, int64_t k, int bytes, int trans, bool async) {
+  const int64_t kk = 128 / bytes, steps = cdiv(k, kk);
+  Plan best{64, 1, 0};
+  double best_t = 1e30;
+  const TileTime* times = bytes == 2 ? kTimes16 : kTimes32;
+  for (int i = bytes == 2 && !async ? 1 : 0; i < (bytes == 2 ? 3 : 2); ++i) {  // (256: no variant through registers)
+    const TileTime& t = times[i];
+    const int64_t tiles = cdiv(m, t.tile) * cdiv(n, t.tile);
+    for (int64_t s = 1; s == 1 || (s <= 64 && steps >= 4 * s && tiles * s <= kCUs * t.per_cu); s += s < 4 ? 1 : s / 2) {
+      const int64_t per = cdiv(steps, s), wgs = cdiv(tiles * cdiv(steps, per), kCUs);
+      auto turn = [&](int64_t r) {  // r workgroups at once on a CU
+        return r == 0 ? 0.0 : per * fmax(t.alone * (1 + 0.4 * trans), r * t.shared) + fmax(t.ends, r * t.ends_shared);
+      };
+      double us = (wgs / t.per_cu) * turn(t.per_cu) + turn(wgs % t.per_cu);
+      if (s > 1) us += 4 + (double)m * n * s * 8 / 8e6;
+      if (us < best_t) {
+        best_t = us;
+        best = Plan{t.tile, (int)cdiv(steps, per), (int)(per * kk)};
+      }
+    }
   }
-  const int64_t per = cdiv(steps, s);
-  p.splits = (int)cdiv(steps, per);
-  p.k_split = (int)(per * kk);
-  return p;
+  return best;
 }
-inline int64_t gemm_scratch(int64_t m, int64_t n, int64_t k, int bytes) {
-  const Plan p = plan_gemm(m, n, k, bytes);
-  return p.splits > 1 ? (int64_t)p.splits * m * n * 4 : 0;
+inline int64_t gemm_scratch(int64_t m, int64_t n, int64_t k, int bytes, int trans) {
+  int64_t need = 0;  // whether the rows are aligned is known with the pointers only
+  for (int async = 0; async < 2; ++async) {
+    const Plan p = plan_gemm(m, n, k, bytes, trans, async);
+    const int64_t b = p.splits > 1 ? (int64_t)p.splits * m * n * 4 : 0;
+    need = b > need ? b : need;
+  }
+  return need;
 }
 constexpr int kFewRows = 64;
 
-template <class Tr, bool kXT, bool kWT, int kTile>
-void launch_gemm_t(const GemmArgs& a, int splits, bool async, hipStream_t st) {
+template <class Tr, bool kXT, bool kWT, bool kAsync>
+void launch_tiles(const GemmArgs& a, int tile, int splits, hipStream_t st) {
   const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), (unsigned)splits);
-  if (async) hipLaunchKernelGGL((gemm_kernel<Tr, kXT, kWT, kTile, true>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((gemm_kernel<Tr, kXT, kWT, kTile, false>), grid, dim3(256), 0, st, a);
+  if constexpr (Tr::kBytes == 2 && kAsync) {
+    if (tile == 256) {
+      hipLaunchKernelGGL((gemm_kernel<Tr, kXT, kWT, 256, 256, 2, 4, 2, true>), grid, dim3(512), 0, st, a);
+      return;
+    }
+  }
+  if (tile == 128) hipLaunchKernelGGL((gemm_kernel<Tr, kXT, kWT, 128, 128, 2, 2, 2, kAsync>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((gemm_kernel<Tr, kXT, kWT, 64, 64, 2, 2, 2, kAsync>), grid, dim3(256), 0, st, a);
 }
 
-// rows of 16-byte chunks whose offsets inside a tile stay below 2^31
+// rows of 16-byte chunks whose offsets inside a tile stay below 2^31 (256 rows of less than 2^23 bytes)
 inline bool aligned_rows(const void* p, int64_t stride, int64_t cols, int bytes) {
   return (uintptr_t)p % 16 == 0 && stride * bytes % 16 == 0 && cols * bytes % 16 == 0 && stride * bytes < (1 << 23);
 }
 
-// part: scratch of gemm_scratch bytes, or NULL (then K is not split)
 template <class Tr, bool kXT, bool kWT>
-void launch_gemm(GemmArgs a, float* part, hipStream_t st) {
-  Plan p = plan_gemm(a.m, a.n, a.k, Tr::kBytes);
-  if (!part) p.splits = 1;
+Plan plan_for(const GemmArgs& a, bool& async) {
+  async = aligned_rows(a.x, a.x_stride, kXT ? a.m : a.k, Tr::kBytes) &&
+          aligned_rows(a.w, a.w_stride, kWT ? a.n : a.k, Tr::kBytes);
+  return plan_gemm(a.m, a.n, a.k, Tr::kBytes, kXT + kWT, async);
+}
+
+// part: `room` bytes of scratch; without enough of it K is not split
+template <class Tr, bool kXT, bool kWT>
+void launch_gemm(GemmArgs a, void* part, int64_t room, hipStream_t st) {
+  bool async;
+  Plan p = plan_for<Tr, kXT, kWT>(a, async);
+  if (p.splits > 1 && (!part || room < (int64_t)p.splits * a.m * a.n * 4)) p.splits = 1;
   if (p.splits == 1) p.k_split = a.k;
-  a.part = p.splits > 1 ? part : nullptr;
+  a.part = p.splits > 1 ? (float*)part : nullptr;
   a.k_split = p.k_split;
   a.tiles_m = (int)cdiv(a.m, p.tile);
   a.tiles_n = (int)cdiv(a.n, p.tile);
-  const bool async = aligned_rows(a.x, a.x_stride, kXT ? a.m : a.k, Tr::kBytes) &&
-                     aligned_rows(a.w, a.w_stride, kWT ? a.n : a.k, Tr::kBytes);
-  if (p.tile == 128) launch_gemm_t<Tr, kXT, kWT, 128>(a, p.splits, async, st);
-  else launch_gemm_t<Tr, kXT, kWT, 64>(a, p.splits, async, st);
+  if (async) launch_tiles<Tr, kXT, kWT, true>(a, p.tile, p.splits, st);
+  else launch_tiles<Tr, kXT, kWT, false>(a, p.tile, p.splits, st);
   if (p.splits > 1)
-    hipLaunchKernelGGL(split_sum_kernel<Tr>, dim3((unsigned)cdiv((int64_t)a.m * cdiv(a.n, 4), 256)), dim3(256), 0, st, a,
+    hipLaunchKernelGGL(split_sum_kernel<Tr>, dim3((unsigned)cdiv((int64_t)a.m * cdiv(a.n, 8), 256)), dim3(256), 0, st, a,
                        p.splits);
 }
 
 template <class Tr>
-void run_linear(const GemmArgs& a, float* part, hipStream_t st) {
+void run_linear(const GemmArgs& a, void* part, int64_t room, hipStream_t st) {
   if (a.m <= kFewRows) {
     const dim3 grid((unsigned)cdiv(a.n, 16));
     if (a.m <= 16) hipLaunchKernelGGL((rows_kernel<Tr, 1>), grid, dim3(512), 0, st, a);
@@ -491,7 +620,7 @@ void run_linear(const GemmArgs& a, float* part, hipStream_t st) {
     else hipLaunchKernelGGL((rows_kernel<Tr, 4>), grid, dim3(512), 0, st, a);
     return;
   }
-  launch_gemm<Tr, false, false>(a, part, st);
+  launch_gemm<Tr, false, false>(a, part, room, st);
 }
 
 // Row groups of the column sums: enough workgroups for the chip, at least 32 rows each
@@ -523,6 +652,7 @@ void run_linear_grad(const yk_linear_grad_args& g, hipStream_t st) {
     ws += cdiv(g.m * g.n * Tr::kBytes, 16) * 16;
   }
   float* part = (float*)ws;  // one region: the kernels that use it follow each other on the stream
+  const int64_t room = g.ws ? g.ws_bytes - (ws - (char*)g.ws) : 0;
   if (act || g.dbias) {
     ColArgs c{(const char*)g.dy, (const char*)g.z, dz, g.dbias, nullptr, g.dy_stride, g.z_stride, g.n, (int)g.m,
               (int)g.n, 1, 1, g.act, g.bias_f32 || Tr::kBytes == 4, g.dtype, 1};
@@ -539,7 +669,7 @@ void run_linear_grad(const yk_linear_grad_args& g, hipStream_t st) {
     a.w = (const char*)g.w, a.w_stride = g.w_stride;
     a.y = (char*)g.dx, a.y_stride = g.dx_stride;
     a.m = (int)g.m, a.n = (int)g.k, a.k = (int)g.n, a.dtype = g.dtype;
-    launch_gemm<Tr, false, true>(a, part, st);
+    launch_gemm<Tr, false, true>(a, part, room, st);
   }
   if (g.dw) {
     GemmArgs a{};
@@ -547,7 +677,7 @@ void run_linear_grad(const yk_linear_grad_args& g, hipStream_t st) {
     a.w = (const char*)g.x, a.w_stride = g.x_stride;
     a.y = (char*)g.dw, a.y_stride = g.dw_stride;
     a.m = (int)g.n, a.n = (int)g.k, a.k = (int)g.m, a.dtype = g.dtype;
-    launch_gemm<Tr, true, true>(a, part, st);
+    launch_gemm<Tr, true, true>(a, part, room, st);
   }
 }
 
@@ -572,7 +702,7 @@ extern "C" {
 int yk_linear_workspace(const yk_linear_args* a, int64_t* bytes) {
   YK_CHECK_ARG(a && bytes, "yk_linear_workspace: NULL argument");
   if (const int rc = check_linear("yk_linear_workspace", a->dtype, a->act, a->m, a->n, a->k)) return rc;
-  *bytes = a->m <= kFewRows ? 0 : gemm_scratch(a->m, a->n, a->k, tok_bytes(a->dtype));
+  *bytes = a->m <= kFewRows ? 0 : gemm_scratch(a->m, a->n, a->k, tok_bytes(a->dtype), 0);
   return YK_OK;
 }
 
@@ -585,19 +715,16 @@ int yk_linear(yk_ctx* ctx, const yk_linear_args* a, void* stream) {
   YK_CHECK_ARG(a->x_stride >= 0 && a->w_stride >= 0 && (!a->res || a->res_stride >= 0) &&
                    (a->m == 1 || (a->y_stride >= a->n && (!a->z || a->z_stride >= a->n))),
                "yk_linear: a negative row stride, or an output's is shorter than its row");
-  int64_t need = 0;
-  if (const int rc = yk_linear_workspace(a, &need)) return rc;
-  YK_CHECK_ARG(need == 0 || !a->ws || (a->ws_bytes >= need && (uintptr_t)a->ws % 16 == 0),
-               "yk_linear: ws must be yk_linear_workspace bytes, 16-byte aligned (or NULL: K is not split)");
+  YK_CHECK_ARG(!a->ws || (a->ws_bytes >= 0 && (uintptr_t)a->ws % 16 == 0),
+               "yk_linear: ws must be 16-byte aligned (NULL or too short: K is not split)");
   yk::DeviceGuard g(ctx->device);
   GemmArgs k{(const char*)a->x, (const char*)a->w, a->bias, (const char*)a->res, (char*)a->y, (char*)a->z, nullptr,
              a->x_stride, a->w_stride, a->res_stride, a->y_stride, a->z_stride, (int)a->m, (int)a->n, (int)a->k,
              (int)a->res_rows, a->act, a->bias_f32 || a->dtype == YK_ACT_F32, a->dtype, 0, 0, 0};
-  float* part = need ? (float*)a->ws : nullptr;
   const hipStream_t st = (hipStream_t)stream;
-  if (a->dtype == YK_ACT_F32) run_linear<F32>(k, part, st);
-  else if (a->dtype == YK_ACT_BF16) run_linear<B16>(k, part, st);
-  else run_linear<H16>(k, part, st);
+  if (a->dtype == YK_ACT_F32) run_linear<F32>(k, a->ws, a->ws_bytes, st);
+  else if (a->dtype == YK_ACT_BF16) run_linear<B16>(k, a->ws, a->ws_bytes, st);
+  else run_linear<H16>(k, a->ws, a->ws_bytes, st);
   return launched("yk_linear");
 }
 
@@ -611,8 +738,8 @@ int yk_linear_backward_workspace(const yk_linear_grad_args* a, int64_t* bytes) {
   if (a->m) {
     if (a->dbias) grow(col_groups(a->m, a->n, 1, e) * a->n * 4);
     if (a->dres) grow((int64_t)col_groups(a->m, a->n, a->res_rows, e) * a->res_rows * a->n * 4);
-    if (a->dx) grow(gemm_scratch(a->m, a->k, a->n, e));
-    if (a->dw) grow(gemm_scratch(a->n, a->k, a->m, e));
+    if (a->dx) grow(gemm_scratch(a->m, a->k, a->n, e, 1));
+    if (a->dw) grow(gemm_scratch(a->n, a->k, a->m, e, 2));
     if (a->act != YK_TOK_NONE) part += cdiv(a->m * a->n * e, 16) * 16;
   }
   *bytes = part;

@@ -102,6 +102,31 @@ __device__ __forceinline__ f32x4 load4(const typename Tr::T* p) {
   }
 }
 
+// 8 elements between registers and any address
+template <class Tr>
+__device__ __forceinline__ void store8(typename Tr::T* p, const float* v) {
+  if constexpr (Tr::kBytes == 4) {
+    *(u32x4_any*)p = __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]});
+    *(u32x4_any*)(p + 4) = __builtin_bit_cast(u32x4, f32x4{v[4], v[5], v[6], v[7]});
+  } else {
+    typename Tr::T t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = from_f32<Tr>(v[e]);
+    u32x4 u;
+    __builtin_memcpy(&u, t, 16);
+    *(u32x4_any*)p = u;
+  }
+}
+template <class Tr>
+__device__ __forceinline__ void add8(const typename Tr::T* p, float* v) {
+  const f32x4 lo = load4<Tr>(p), hi = load4<Tr>(p + 4);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] += lo[e];
+    v[4 + e] += hi[e];
+  }
+}
+
 // 16 bytes (kEpc elements) of a row, elements at or past n0 zero: one load where they are all
 // there, element loads at the row's end
 template <class Tr>
@@ -151,26 +176,48 @@ __device__ __forceinline__ void store_param(void* p, int64_t i, float v, int is_
   else ((_Float16*)p)[i] = (_Float16)v;
 }
 
-// act(z) and act'(z) in float32.  GELU is z Phi(z) with Phi(z) = (1 + erf(z / sqrt 2)) / 2.
+// 2^x and 1 / x: one instruction each, off by about one unit in the last place
+__device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float rcp_f(float x) { return __builtin_amdgcn_rcpf(x); }
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
+
+// Phi(-|z|) and e^(-z^2 / 2): Phi's tail as in Abramowitz and Stegun 7.1.26 (Hastings), a polynomial
+// in t = 1 / (1 + p |z| / sqrt 2) times that exponential, off by less than 7.5e-8 of 1.  14
+// instructions against some 40 of erff, whose two ranges a wave walks both; the product z Phi(z)
+// is then off by less than 2 float32 roundings of z.
+__device__ __forceinline__ float normal_tail(float z, float& e) {
+  const float t = rcp_f(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
+  e = exp2_f(z * z * (-0.5f * kLog2e));
+  float p = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+  p = fmaf(p, t, 0.5f * 1.421413741f);
+  p = fmaf(p, t, 0.5f * -0.284496736f);
+  p = fmaf(p, t, 0.5f * 0.254829592f);
+  return p * t * e;
+}
+
+// act(z) and act'(z) in float32.  GELU is z Phi(z).
 __device__ __forceinline__ float act_f32(float z, int act) {
-  switch (act) {
-    case YK_TOK_SILU: return z / (1.f + expf(-z));
-    case YK_TOK_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case YK_TOK_RELU: return z > 0.f ? z : z != z ? z : 0.f;
-    default: return z;
+  if (act == YK_TOK_GELU) {
+    float e;
+    const float q = normal_tail(z, e);
+    return z * (z < 0.f ? q : 1.f - q);
   }
+  if (act == YK_TOK_SILU) return z * rcp_f(1.f + exp2_f(z * -kLog2e));
+  if (act == YK_TOK_RELU) return z > 0.f ? z : z != z ? z : 0.f;
+  return z;
 }
 __device__ __forceinline__ float act_slope(float z, int act) {
-  switch (act) {
-    case YK_TOK_SILU: {
-      const float s = 1.f / (1.f + expf(-z));
-      return s * (1.f + z * (1.f - s));
-    }
-    case YK_TOK_GELU:
-      return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
-    case YK_TOK_RELU: return z > 0.f ? 1.f : 0.f;
-    default: return 1.f;
+  if (act == YK_TOK_GELU) {
+    float e;
+    const float q = normal_tail(z, e);
+    return fmaf(z * 0.39894228040143268f, e, z < 0.f ? q : 1.f - q);
   }
+  if (act == YK_TOK_SILU) {
+    const float s = rcp_f(1.f + exp2_f(z * -kLog2e));
+    return s * fmaf(z, 1.f - s, 1.f);
+  }
+  if (act == YK_TOK_RELU) return z > 0.f ? 1.f : 0.f;
+  return 1.f;
 }
 
 __device__ __forceinline__ int rfl(int v) { return __builtin_amdgcn_readfirstlane(v); }

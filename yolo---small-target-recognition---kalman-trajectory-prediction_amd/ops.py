@@ -14,6 +14,7 @@ A tensor's last dimension must be contiguous; what precedes it must step evenly 
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -21,81 +22,120 @@ from . import _lib as L
 
 ACTS = {"none": 0, "silu": 1, "gelu": 2, "relu": 3}
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 3}  # yk_act_dtype
+_F32 = torch.float32
+_empty, _empty_like, _grad_enabled = torch.empty, torch.empty_like, torch.is_grad_enabled
+
+# The C argument structs as packed bytes (a ctypes struct costs three times as long to fill); the
+# last two fields, scratch and its size, are appended once the size is known.
+_LINEAR = struct.Struct("4i 3q 6Q 6q")
+_LINEAR_GRAD = struct.Struct("4i 3q 8Q 8q")
+_NORM = struct.Struct("2i 2q f i 6Q 2q")
+_NORM_GRAD = struct.Struct("2i 2q 8Q 3q")
+_ATTENTION = struct.Struct("6i 2q f i 7Q 12q")
+_ATTENTION_GRAD = struct.Struct("6i 2q f i 11Q 24q")
+_WS = struct.Struct("Q q")
+_scratch: dict = {}  # (entry point, sizes) -> bytes of scratch
 
 
-def _tensor(t, name, like=None, dtypes=None):
+def _input(t, name):
+    """The operator's first tensor: sets the type and the GPU.  Returns (yk_act_dtype, device index)."""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires grad: no autograd graph is built here (detach it, or torch.no_grad())")
-    if like is None:
-        if t.dtype not in _DTYPES:
-            raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-        if t.device.type != "cuda":
-            raise L.YKError(f"{name} is on {t.device}: the token operators run on an AMD GPU only (no CPU fallback)")
-    else:
-        if t.device != like.device:
-            raise ValueError(f"{name} is on {t.device}, expected {like.device}")
-        if t.dtype not in (dtypes or (like.dtype,)):
-            raise ValueError(f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes or (like.dtype,))}")
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if not t.is_cuda:
+        raise L.YKError(f"{name} is on {t.device}: the token operators run on an AMD GPU only (no CPU fallback)")
+    if t.requires_grad and _grad_enabled():
+        _needs_no_grad(name)
+    return code, t.get_device()
+
+
+def _needs_no_grad(name):
+    raise ValueError(f"{name} requires grad: no autograd graph is built here (detach it, or torch.no_grad())")
+
+
+def _like(t, name, dev, dtype, other=None):
+    """Another tensor of the call: on the same GPU, of the given type (or the other one)."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{dev}")
+    if t.dtype is not dtype and t.dtype is not other:
+        raise ValueError(f"{name} has dtype {t.dtype}, expected {dtype}" + (f" or {other}" if other else ""))
+    if t.requires_grad and _grad_enabled():
+        _needs_no_grad(name)
     return t
 
 
 def _rows(t, name, cols=None):
     """(rows, columns, row stride) of a tensor as a matrix of its last dimension."""
-    if t.dim() < 1 or t.shape[-1] < 1:
+    shape = t.shape
+    if not shape or shape[-1] < 1:
         raise ValueError(f"{name} must have a last dimension of at least 1")
-    c = t.shape[-1]
+    c = shape[-1]
     if cols is not None and c != cols:
         raise ValueError(f"{name} has {c} columns, expected {cols}")
-    if c > 1 and t.stride(-1) != 1:
+    if t.is_contiguous():
+        return t.numel() // c, c, c
+    strides = t.stride()
+    if c > 1 and strides[-1] != 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
-    rows, stride = 1, c
-    first = True
-    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    rows, stride = 1, None
+    for n, s in zip(shape[-2::-1], strides[-2::-1]):
         if n == 1:
             continue
-        if first:
-            stride, first = s, False
+        if stride is None:
+            stride = s
         elif s != stride * rows:
-            raise ValueError(f"{name}: rows must be evenly spaced (shape {tuple(t.shape)}, strides {t.stride()})")
+            raise ValueError(f"{name}: rows must be evenly spaced (shape {tuple(shape)}, strides {strides})")
         rows *= n
-    return rows, c, stride
+    return rows, c, c if stride is None else stride
 
 
-def _vector(t, name, n, like):
-    """A parameter of n elements: the tensors' dtype or float32, contiguous."""
-    _tensor(t, name, like, (like.dtype, torch.float32))
-    if t.shape != (n,) or not (n == 1 or t.is_contiguous()):
+def _vector(t, name, n, dev, dtype):
+    """A parameter of n elements, contiguous, of the tensors' type or float32: (address, 1 if float32)."""
+    _like(t, name, dev, dtype, _F32)
+    if t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous vector of {n} elements, got {tuple(t.shape)}")
-    return t
+    return t.data_ptr(), int(t.dtype is _F32)
 
 
-def _p(t):
-    return None if t is None else t.data_ptr()
-
-
-def _call(fn, args, like):
-    dev = like.device.index
+def _call(fn, packed, dev, sizes=None):
+    """Enqueue an entry point on the device's current stream, with the scratch that `sizes` (all its
+    size depends on) needs."""
     lib = L.lib()
-    ws = None
-    if fn != "yk_layer_norm":
-        need = C.c_int64()
-        rc = getattr(lib, fn + "_workspace")(C.byref(args), C.byref(need))
-        if rc:
-            L.check(rc, fn)
-        if need.value:
-            ws = torch.empty(need.value, dtype=torch.uint8, device=like.device)
-            args.ws, args.ws_bytes = ws.data_ptr(), need.value
-    rc = getattr(lib, fn)(L.context(dev), C.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+    if sizes is not None:
+        need = _scratch.get((fn, sizes))
+        if need is None:
+            n = C.c_int64()
+            L.check(getattr(lib, fn + "_workspace")(packed + _WS.pack(0, 0), C.byref(n)), fn)
+            if len(_scratch) >= 4096:
+                _scratch.clear()
+            need = _scratch[(fn, sizes)] = n.value
+        if need:
+            ws = _empty(need, dtype=torch.uint8, device=torch.device("cuda", dev))
+            packed += _WS.pack(ws.data_ptr(), need)
+        else:
+            packed += _WS.pack(0, 0)
+    rc = getattr(lib, fn)(L.context(dev), packed, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         L.check(rc, fn)
 
 
 def _act(name):
-    if name not in ACTS:
+    code = ACTS.get(name)
+    if code is None:
         raise ValueError(f"act must be one of {sorted(ACTS)}, got {name!r}")
-    return ACTS[name]
+    return code
+
+
+def _residual(residual, m, n, dev, dtype):
+    """(address, rows, row stride) of linear()'s residual."""
+    r, _, rs = _rows(_like(residual, "residual", dev, dtype), "residual", n)
+    if not 1 <= r <= max(m, 1):
+        raise ValueError(f"residual has {r} rows, x has {m}: expected 1 to that many")
+    return residual.data_ptr(), r, rs
 
 
 def linear(x, weight, bias=None, *, act="none", residual=None, return_preact=False):
@@ -105,74 +145,78 @@ def linear(x, weight, bias=None, *, act="none", residual=None, return_preact=Fal
     or "relu"; residual [..., N] with any R <= rows(x) rows, row m of the result taking row m % R (R
     tokens shared by the images of a batch).  Returns [..., N], with return_preact also act's
     argument, which linear_backward needs unless act is "none"."""
-    _tensor(x, "x")
+    dt, dev = _input(x, "x")
+    dtype = x.dtype
     m, k, xs = _rows(x, "x")
-    _tensor(weight, "weight", x)
-    if weight.dim() != 2:
+    n, _, ws = _rows(_like(weight, "weight", dev, dtype), "weight", k)
+    if weight.dim() != 2 or n < 1:
         raise ValueError("weight must be [N, K]")
-    n, _, ws = _rows(weight, "weight", k)
-    if n < 1:
-        raise ValueError("weight must have at least one row")
-    a = L.LinearArgs(dtype=_DTYPES[x.dtype], act=_act(act), m=m, n=n, k=k, x=_p(x), w=_p(weight), x_stride=xs, w_stride=ws)
-    if bias is not None:
-        a.bias, a.bias_f32 = _p(_vector(bias, "bias", n, x)), bias.dtype == torch.float32
-    if residual is not None and m:
-        r, _, rs = _rows(_tensor(residual, "residual", x), "residual", n)
-        if not 1 <= r <= m:
-            raise ValueError(f"residual has {r} rows, x has {m}: expected 1 to that many")
-        a.res, a.res_rows, a.res_stride = _p(residual), r, rs
-    y = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=x.device)
-    z = torch.empty_like(y) if return_preact else None
-    a.y, a.y_stride, a.z, a.z_stride = _p(y), n, _p(z), n
+    a = _act(act)
+    b, bf = (0, 0) if bias is None else _vector(bias, "bias", n, dev, dtype)
+    r, rows, rs = (0, 0, 0) if residual is None or not m else _residual(residual, m, n, dev, dtype)
+    y = x.new_empty((*x.shape[:-1], n))
+    z = _empty_like(y) if return_preact else None
     if m:
-        _call("yk_linear", a, x)
+        _call("yk_linear", _LINEAR.pack(dt, a, bf, 0, m, n, k, x.data_ptr(), weight.data_ptr(), b, r, y.data_ptr(),
+                                        0 if z is None else z.data_ptr(), xs, ws, rs, rows, n, n),
+              dev, (dt, m, n, k))
     return (y, z) if return_preact else y
 
 
 def linear_backward(dy, x, weight, bias=None, *, act="none", preact=None, residual=None):
     """Gradients of linear() from dy [..., N]: (dx, dweight, dbias, dresidual), the last two None
     without bias / residual.  preact is linear's second result (needed unless act is "none");
-    residual's shape and dtype are what counts of it.  Where it has a row per row of x its gradient
-    is dy itself."""
-    _tensor(x, "x")
+    residual's shape and dtype are what counts of it.  Where it has dy's shape its gradient is dy
+    itself."""
+    dt, dev = _input(x, "x")
+    dtype = x.dtype
     m, k, xs = _rows(x, "x")
-    n, _, ws = _rows(_tensor(weight, "weight", x), "weight", k)
-    md, _, ds = _rows(_tensor(dy, "dy", x), "dy", n)
+    n, _, ws = _rows(_like(weight, "weight", dev, dtype), "weight", k)
+    md, _, ds = _rows(_like(dy, "dy", dev, dtype), "dy", n)
     if weight.dim() != 2 or md != m:
         raise ValueError("weight must be [N, K] and dy have a row for every row of x")
-    a = L.LinearGradArgs(dtype=_DTYPES[x.dtype], act=_act(act), m=m, n=n, k=k, dy=_p(dy), x=_p(x), w=_p(weight),
-                         dy_stride=ds, x_stride=xs, w_stride=ws)
-    if a.act:
+    a = _act(act)
+    z, zs = 0, 0
+    if a:
         if preact is None:
             raise ValueError(f"act {act!r} needs preact, the second result of linear(..., return_preact=True)")
-        mz, _, zs = _rows(_tensor(preact, "preact", x), "preact", n)
+        mz, _, zs = _rows(_like(preact, "preact", dev, dtype), "preact", n)
         if mz != m:
             raise ValueError("preact must have a row for every row of x")
-        a.z, a.z_stride = _p(preact), zs
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device)
+        z = preact.data_ptr()
+    dx, dw = x.new_empty(x.shape), x.new_empty(weight.shape)
     db = dres = None
+    pb = bf = pr = rows = 0
     if bias is not None:
-        _vector(bias, "bias", n, x)
-        db = torch.empty(n, dtype=bias.dtype, device=x.device)
-        a.dbias, a.bias_f32 = _p(db), bias.dtype == torch.float32
+        _, bf = _vector(bias, "bias", n, dev, dtype)
+        db = bias.new_empty(n)
+        pb = db.data_ptr()
     if residual is not None:
-        r, _, _ = _rows(_tensor(residual, "residual", x), "residual", n)
-        if not 1 <= r <= max(m, 1):
-            raise ValueError(f"residual has {r} rows, x has {m}: expected 1 to that many")
-        if r == m and residual.shape == dy.shape:
-            dres = dy
+        _, rows, _ = _residual(residual, m, n, dev, dtype)
+        if residual.shape == dy.shape:
+            dres, rows = dy, 0
         else:
-            dres = torch.empty(residual.shape, dtype=x.dtype, device=x.device)
-            a.dres, a.dres_stride, a.res_rows = _p(dres), n, r
-    if not m:
+            dres = x.new_empty(residual.shape)
+            pr = dres.data_ptr()
+    if m:
+        _call("yk_linear_backward",
+              _LINEAR_GRAD.pack(dt, a, bf, 0, m, n, k, dy.data_ptr(), x.data_ptr(), weight.data_ptr(), z, dx.data_ptr(),
+                                dw.data_ptr(), pb, pr, ds, xs, ws, zs, k, k, n, rows),
+              dev, (dt, a, m, n, k, pb != 0, rows))
+    else:
         for t in (dw, db, dres):
             if t is not None:
                 t.zero_()
-        return dx, dw, db, dres
-    a.dx, a.dw, a.dx_stride, a.dw_stride = _p(dx), _p(dw), k, k
-    _call("yk_linear_backward", a, x)
     return dx, dw, db, dres
+
+
+def _norm_params(weight, bias, c, dev, dtype):
+    """(address of weight, of bias, 1 if they are float32)"""
+    w, wf = (0, 0) if weight is None else _vector(weight, "weight", c, dev, dtype)
+    b, bf = (0, wf) if bias is None else _vector(bias, "bias", c, dev, dtype)
+    if weight is not None and bf != wf:
+        raise ValueError("weight and bias must have one dtype")
+    return w, b, bf
 
 
 def layer_norm(x, weight=None, bias=None, *, eps=1e-5, return_stats=False):
@@ -180,78 +224,65 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, return_stats=False):
 
     weight / bias [C]: both in x's dtype or both float32; None: 1 / 0.  With return_stats also
     mean and 1 / sqrt(var + eps), float32 of x's leading shape, for layer_norm_backward."""
-    _tensor(x, "x")
+    dt, dev = _input(x, "x")
     m, c, xs = _rows(x, "x")
-    a = L.LayerNormArgs(dtype=_DTYPES[x.dtype], m=m, c=c, eps=eps, x=_p(x), x_stride=xs, y_stride=c)
-    _norm_params(a, weight, bias, c, x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a.y = _p(y)
-    mean = rstd = None
-    if return_stats:
-        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        rstd = torch.empty_like(mean)
-        a.mean, a.rstd = _p(mean), _p(rstd)
+    w, b, pf = _norm_params(weight, bias, c, dev, x.dtype)
     if not eps >= 0:
         raise ValueError("eps must be >= 0")
+    y = x.new_empty(x.shape)
+    mean = rstd = None
+    if return_stats:
+        mean = x.new_empty(x.shape[:-1], dtype=_F32)
+        rstd = _empty_like(mean)
     if m:
-        _call("yk_layer_norm", a, x)
+        _call("yk_layer_norm", _NORM.pack(dt, pf, m, c, eps, 0, x.data_ptr(), w, b, y.data_ptr(),
+                                          mean.data_ptr() if return_stats else 0, rstd.data_ptr() if return_stats else 0,
+                                          xs, c), dev)
     return (y, mean, rstd) if return_stats else y
-
-
-def _norm_params(a, weight, bias, c, x):
-    given = [t for t in (weight, bias) if t is not None]
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None:
-            _vector(t, name, c, x)
-    if len(given) == 2 and weight.dtype != bias.dtype:
-        raise ValueError("weight and bias must have one dtype")
-    a.w, a.param_f32 = _p(weight), bool(given) and given[0].dtype == torch.float32
-    if bias is not None and hasattr(a, "b"):
-        a.b = _p(bias)
 
 
 def layer_norm_backward(dy, x, weight, mean, rstd):
     """Gradients of layer_norm() from dy, x and its mean and rstd: (dx, dweight, dbias), the last
     two in weight's dtype (float32 where weight is None)."""
-    _tensor(x, "x")
+    dt, dev = _input(x, "x")
     m, c, xs = _rows(x, "x")
-    md, _, ds = _rows(_tensor(dy, "dy", x), "dy", c)
+    md, _, ds = _rows(_like(dy, "dy", dev, x.dtype), "dy", c)
     for t, name in ((mean, "mean"), (rstd, "rstd")):
-        _tensor(t, name, x, (torch.float32,))
-        if t.numel() != m or not t.is_contiguous():
+        if _like(t, name, dev, _F32).numel() != m or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous tensor with an element for every row of x")
     if md != m:
         raise ValueError("dy must have a row for every row of x")
-    a = L.LayerNormGradArgs(dtype=_DTYPES[x.dtype], m=m, c=c, dy=_p(dy), x=_p(x), mean=_p(mean), rstd=_p(rstd),
-                            dy_stride=ds, x_stride=xs, dx_stride=c)
-    _norm_params(a, weight, None, c, x)
-    pd = torch.float32 if weight is None else weight.dtype
-    a.param_f32 = pd == torch.float32
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dw, db = torch.empty(c, dtype=pd, device=x.device), torch.empty(c, dtype=pd, device=x.device)
-    a.dx, a.dw, a.db = _p(dx), _p(dw), _p(db)
-    _call("yk_layer_norm_backward", a, x)
+    w, _, pf = _norm_params(weight, None, c, dev, x.dtype)
+    dw = x.new_empty(c, dtype=_F32) if weight is None else weight.new_empty(c)
+    dx, db = x.new_empty(x.shape), _empty_like(dw)
+    _call("yk_layer_norm_backward",
+          _NORM_GRAD.pack(dt, int(dw.dtype is _F32), m, c, dy.data_ptr(), x.data_ptr(), w, mean.data_ptr(), rstd.data_ptr(),
+                          dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ds, xs, c),
+          dev, (dt, m, c))
     return dx, dw, db
 
 
-def _heads(t, name, like, shape=None):
-    _tensor(t, name, like)
-    if t.dim() != 4 or (shape is not None and tuple(t.shape) != shape):
-        raise ValueError(f"{name} must be [batch, tokens, heads, size]" +
-                         (f" = {list(shape)}" if shape is not None else "") + f", got {list(t.shape)}")
-    if t.shape[3] > 1 and t.stride(3) != 1:
+def _heads(t, name, shape):
+    """Strides of [batch, tokens, heads, size]."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be [batch, tokens, heads, size] = {list(shape)}, got {list(t.shape)}")
+    s = t.stride()
+    if s[3] != 1 and shape[3] > 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
-    return t.stride()[:3]
+    return s[:3]
 
 
-def _attention_args(cls, q, k, v, scale, causal, q_lengths, lengths):
-    qs = _heads(q, "q", None)
+def _attention_args(q, k, v, scale, causal, q_lengths, lengths):
+    """(device, sizes that open the C struct, addresses of q k v, of the lengths, strides of q k v)"""
+    dt, dev = _input(q, "q")
+    dtype = q.dtype
+    _like(k, "k", dev, dtype)
+    _like(v, "v", dev, dtype)
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError(f"q and k must be [batch, tokens, heads, size], got {list(q.shape)} and {list(k.shape)}")
     b, nq, h, d = q.shape
-    ks = _heads(k, "k", q)
-    nk, hk = k.shape[1], k.shape[2]
-    vs = _heads(v, "v", q, (b, nk, hk, d))
-    if k.shape[0] != b or k.shape[3] != d:
-        raise ValueError(f"k must be [{b}, tokens, heads, {d}], got {list(k.shape)}")
+    nk, hk = k.shape[1:3]
+    qs, ks, vs = _heads(q, "q", q.shape), _heads(k, "k", (b, nk, hk, d)), _heads(v, "v", (b, nk, hk, d))
     if h < 1 or hk < 1 or h % hk:
         raise ValueError(f"q's heads ({h}) must be a multiple of k's ({hk})")
     if not 1 <= d <= 128:
@@ -259,15 +290,14 @@ def _attention_args(cls, q, k, v, scale, causal, q_lengths, lengths):
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0 < scale < float("inf"):
         raise ValueError("scale must be positive and finite")
-    for t, name in ((q_lengths, "q_lengths"), (lengths, "lengths")):
+    lens = [0, 0]
+    for i, (t, name) in enumerate(((q_lengths, "q_lengths"), (lengths, "lengths"))):
         if t is not None:
-            _tensor(t, name, q, (torch.int32,))
-            if t.shape != (b,) or not t.is_contiguous():
+            if _like(t, name, dev, torch.int32).shape != (b,) or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous int32 tensor [{b}]")
-    s3 = C.c_int64 * 3
-    return cls(dtype=_DTYPES[q.dtype], causal=bool(causal), b=b, h_q=h, h_kv=hk, d=d, nq=nq, nk=nk, scale=scale,
-               q=_p(q), k=_p(k), v=_p(v), q_lengths=_p(q_lengths), lengths=_p(lengths), q_stride=s3(*qs), k_stride=s3(*ks),
-               v_stride=s3(*vs))
+            lens[i] = t.data_ptr()
+    return dev, (dt, int(bool(causal)), b, h, hk, d, nq, nk, scale, 0), (q.data_ptr(), k.data_ptr(), v.data_ptr()), lens, \
+        (*qs, *ks, *vs)
 
 
 def attention(q, k, v, *, scale=None, causal=False, lengths=None, q_lengths=None, return_lse=False):
@@ -279,29 +309,28 @@ def attention(q, k, v, *, scale=None, causal=False, lengths=None, q_lengths=None
     sees keys j <= i + length - q_length, so one new token sees its whole cache.  A query that sees
     no key gives 0.  Returns o like q, with return_lse also ln of the softmax's denominators,
     float32 [B, H, Nq] (-inf where no key is seen), for attention_backward."""
-    a = _attention_args(L.AttentionArgs, q, k, v, scale, causal, q_lengths, lengths)
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    a.o, a.o_stride = _p(o), (C.c_int64 * 3)(*o.stride()[:3])
-    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=q.device) if return_lse else None
-    a.lse = _p(lse)
+    dev, head, qkv, lens, strides = _attention_args(q, k, v, scale, causal, q_lengths, lengths)
+    o = q.new_empty(q.shape)
+    lse = q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=_F32) if return_lse else None
     if o.numel():
-        _call("yk_attention", a, q)
+        _call("yk_attention", _ATTENTION.pack(*head, *qkv, *lens, o.data_ptr(), lse.data_ptr() if return_lse else 0, *strides,
+                                              *o.stride()[:3]), dev, head)
     return (o, lse) if return_lse else o
 
 
 def attention_backward(do, q, k, v, o, lse, *, scale=None, causal=False, lengths=None, q_lengths=None):
     """Gradients of attention() with the same arguments, from do and its two results: (dq, dk, dv),
     dk and dv summed over the heads that share a key head, 0 behind the lengths."""
-    a = _attention_args(L.AttentionGradArgs, q, k, v, scale, causal, q_lengths, lengths)
-    s3 = C.c_int64 * 3
-    a.go_stride, a.o_stride = s3(*_heads(do, "do", q, tuple(q.shape))), s3(*_heads(o, "o", q, tuple(q.shape)))
-    _tensor(lse, "lse", q, (torch.float32,))
-    if lse.shape != (q.shape[0], q.shape[2], q.shape[1]) or not lse.is_contiguous():
+    dev, head, qkv, lens, strides = _attention_args(q, k, v, scale, causal, q_lengths, lengths)
+    gs = _heads(_like(do, "do", dev, q.dtype), "do", q.shape)
+    os = _heads(_like(o, "o", dev, q.dtype), "o", q.shape)
+    if _like(lse, "lse", dev, _F32).shape != (q.shape[0], q.shape[2], q.shape[1]) or not lse.is_contiguous():
         raise ValueError("lse must be attention's second result, contiguous [B, H, Nq]")
-    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     if not q.numel() or not k.numel():
         return dq.zero_(), dk.zero_(), dv.zero_()
-    a.go, a.o, a.lse, a.dq, a.dk, a.dv = _p(do), _p(o), _p(lse), _p(dq), _p(dk), _p(dv)
-    a.dq_stride, a.dk_stride, a.dv_stride = s3(*dq.stride()[:3]), s3(*dk.stride()[:3]), s3(*dv.stride()[:3])
-    _call("yk_attention_backward", a, q)
+    _call("yk_attention_backward",
+          _ATTENTION_GRAD.pack(*head, do.data_ptr(), *qkv, o.data_ptr(), lse.data_ptr(), *lens, dq.data_ptr(), dk.data_ptr(),
+                               dv.data_ptr(), *gs, *strides, *os, *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3]),
+          dev, head)
     return dq, dk, dv
