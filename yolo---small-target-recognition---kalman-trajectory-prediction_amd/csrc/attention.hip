@@ -91,72 +91,165 @@ __device__ __forceinline__ typename Tr::V8 pack8(f32x4 lo, f32x4 hi) {
   }
 }
 
-// kBN x kDP block of rows in LDS (kDP = d padded to 32, zero filled), rows 16 bytes apart beyond
-// their data so that the 16 rows of a fragment start on different banks.
+// kBN x kDP block of rows in LDS (kDP = d padded to 32, zero filled) in 16-byte chunks.  Chunk c of a
+// row lies at c ^ (row >> kShift) within its group of kGroup chunks, so that the 16 rows of a
+// fragment, whichever way it is read, fall on different banks.
 template <class Tr, int kDP>
 struct Block {
   using T = typename Tr::T;
   static constexpr int kBN = 128 / Tr::kBytes;  // 64 rows of 16-bit, 32 of float32
   static constexpr int kEpc = 16 / Tr::kBytes;
-  static constexpr int kPitch = kDP * Tr::kBytes + 16;
+  static constexpr int kRow = kDP * Tr::kBytes;
   static constexpr int kRowChunks = kDP / kEpc;
   static constexpr int kN = kDP / 32;           // chunks per thread of 256
-  static constexpr int kBytesAll = kBN * kPitch;
+  static constexpr int kBytesAll = kBN * kRow;
+  static constexpr int kGroup = kRow % 256 == 0 ? 16 : kRow % 128 == 0 ? 8 : 4;
+  static constexpr int kShift = kGroup == 16 ? 0 : kGroup == 8 ? 1 : 2;
 
+  static __device__ __forceinline__ int place(int row, int c) {  // (its own inverse in c)
+    return (c & ~(kGroup - 1)) | ((c ^ (row >> kShift)) & (kGroup - 1));
+  }
   // A operand: row 16 t + l, elements 32 s + 8 g ..
   static __device__ __forceinline__ typename Tr::V8 row_frag(const char* lds, int t, int s, int lane) {
     const int l = lane & 15, g = lane >> 4;
-    return *(const typename Tr::V8*)__builtin_assume_aligned(lds + (t * 16 + l) * kPitch + (s * 32 + g * 8) * Tr::kBytes, 16);
+    const char* row = lds + (t * 16 + l) * kRow;
+    if constexpr (Tr::kBytes == 2) {
+      return *(const typename Tr::V8*)(row + place(l, s * 4 + g) * 16);
+    } else {
+      const f32x4 lo = *(const f32x4*)(row + place(l, s * 8 + 2 * g) * 16);
+      const f32x4 hi = *(const f32x4*)(row + place(l, s * 8 + 2 * g + 1) * 16);
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
   }
   // A operand, transposed: element 16 dt + l of rows 32 u + {4g .. 4g+3, 16+4g .. 16+4g+3}
   static __device__ __forceinline__ typename Tr::V8 col_frag(const char* lds, int dt, int u, int lane) {
     const int l = lane & 15, g = lane >> 4;
     if constexpr (Tr::kBytes == 2) {
-      const char* p = lds + (u * 32 + 4 * g + (l >> 2)) * kPitch + dt * 32 + (l & 3) * 8;
+      const int row = 4 * g + (l >> 2);
+      const char* p = lds + (u * 32 + row) * kRow + place(row, dt * 2 + ((l & 3) >> 1)) * 16 + (l & 1) * 8;
       typedef __attribute__((address_space(3))) s16x4* lp;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)p);
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 16 * kPitch));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 16 * kRow));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
       typename Tr::V8 v;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        v[e] = *(const float*)(lds + (u * 32 + (e & 4) * 4 + 4 * g + (e & 3)) * kPitch + (dt * 16 + l) * 4);
+      for (int e = 0; e < 8; ++e) {
+        const int row = u * 32 + (e & 4) * 4 + 4 * g + (e & 3);
+        v[e] = *(const float*)(lds + row * kRow + place(row, dt * 4 + (l >> 2)) * 16 + (l & 3) * 4);
+      }
       return v;
     }
   }
 };
 
-template <class Tr, int kDP>
-struct Stage {  // a block on its way from memory to LDS, by 256 threads
+// A stream of blocks of rows from memory to LDS by 256 threads: the packed rows of a group of
+// heads, or (group 1) the keys of a head.  kAsync: without registers, through a buffer descriptor
+// that moves with the block, whose range check turns what is not there into zeros; needs whole,
+// 16-byte aligned chunks and a group that divides the block (feed_async).
+template <class Tr, int kDP, bool kAsync>
+struct Feed {
   using Bl = Block<Tr, kDP>;
   using T = typename Tr::T;
-  u32x4 reg[Bl::kN];
-  // rows first .. of a key head's keys, below `limit`
-  __device__ __forceinline__ void load_keys(const T* base, int64_t stride, int first, int limit, int d) {
+  static constexpr unsigned kOut = 0x80000000u;
+  const T* base;  // row `first`'s query, head 0 of the group (kAsync); row 0 (else)
+  int64_t st1, st2;
+  int group, d, first;
+  unsigned off[kAsync ? Bl::kN : 1];
+  u32x4 reg[kAsync ? 1 : Bl::kN];
+
+  __device__ __forceinline__ void init(const char* p, const int64_t* st, int b, int head0, int grp, int dd, int first_row) {
+    group = grp, d = dd, first = first_row;
+    st1 = st[1], st2 = st[2];
+    base = (const T*)p + b * st[0] + head0 * st[2];
+    if constexpr (kAsync) {
+      base += (int64_t)query_of(first, group) * st1;
 #pragma unroll
-    for (int i = 0; i < Bl::kN; ++i) {
-      const int j = i * 256 + threadIdx.x, row = j / Bl::kRowChunks, c = (j % Bl::kRowChunks) * Bl::kEpc;
-      reg[i] = load16_if<Tr>(base + (int64_t)(first + row) * stride + c, base, d - c, first + row < limit, d % Bl::kEpc == 0);
+      for (int i = 0; i < Bl::kN; ++i) {
+        const int j = i * 256 + threadIdx.x, row = j / Bl::kRowChunks, c = Bl::place(row, j % Bl::kRowChunks) * Bl::kEpc;
+        const int q = query_of(row, group);
+        off[i] = c < d ? (unsigned)((q * (int)st1 + (row - q * group) * (int)st2 + c) * Tr::kBytes) : kOut;
+      }
     }
   }
-  // packed rows first .. of (b, hk), below `limit`
-  __device__ __forceinline__ void load_rows(const T* base, const int64_t* st, int b, int hk, int group, int first,
-                                            int limit, int d) {
+  // the block that begins at `first`, rows at and past `limit` zero
+  __device__ __forceinline__ void issue(char* lds, int limit) {
+    if constexpr (kAsync) {
+      const size_t b = (size_t)base;
+      const size_t ub = ((size_t)(unsigned)rfl((int)(b >> 32)) << 32) | (unsigned)rfl((int)b);
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)ub, (short)0, 0x7ffffff0, 0x00020000);
+      const bool tail = first + Bl::kBN > limit;
 #pragma unroll
-    for (int i = 0; i < Bl::kN; ++i) {
-      const int j = i * 256 + threadIdx.x, row = j / Bl::kRowChunks, c = (j % Bl::kRowChunks) * Bl::kEpc;
-      reg[i] = load16_if<Tr>(row_ptr(base, st, b, hk, group, first + row) + c, base, d - c, first + row < limit, d % Bl::kEpc == 0);
+      for (int i = 0; i < Bl::kN; ++i) {
+        unsigned o = off[i];
+        if (tail && first + (int)((i * 256 + threadIdx.x) / Bl::kRowChunks) >= limit) o = kOut;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rsrc, (__attribute__((address_space(3))) void*)(lds + (i * 256 + rfl(threadIdx.x & ~63)) * 16), 16, o, 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < Bl::kN; ++i) {
+        const int j = i * 256 + threadIdx.x, row = first + j / Bl::kRowChunks, c = (j % Bl::kRowChunks) * Bl::kEpc;
+        const int q = query_of(row, group);
+        reg[i] = load16_if<Tr>(base + q * st1 + (row - q * group) * st2 + c, base, d - c, row < limit, d % Bl::kEpc == 0);
+      }
     }
   }
-  __device__ __forceinline__ void store(char* lds) const {
+  __device__ __forceinline__ void advance() {
+    first += Bl::kBN;
+    if constexpr (kAsync) base += (int64_t)(group == 1 ? Bl::kBN : Bl::kBN / group) * st1;
+  }
+  __device__ __forceinline__ void commit(char* lds) const {
+    if constexpr (!kAsync) {
 #pragma unroll
-    for (int i = 0; i < Bl::kN; ++i) {
-      const int j = i * 256 + threadIdx.x, row = j / Bl::kRowChunks, c = j % Bl::kRowChunks;
-      *(u32x4*)(lds + row * Bl::kPitch + c * 16) = reg[i];
+      for (int i = 0; i < Bl::kN; ++i) {
+        const int j = i * 256 + threadIdx.x, row = j / Bl::kRowChunks, c = j % Bl::kRowChunks;
+        *(u32x4*)(lds + row * Bl::kRow + Bl::place(row, c) * 16) = reg[i];
+      }
     }
   }
 };
+
+// Until this wave's loads have landed and its LDS reads are done; then until all waves are there.
+__device__ __forceinline__ void block_landed() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+}
+
+// Runs `body(buffer)` over the blocks of two feeds, [first, end) in rows; `buf`: kBuffers of them, the
+// next block on its way while one is worked on, one barrier per block.  extra(buffer, first) loads what else
+// belongs to a block (kAsync: straight to LDS).
+template <class Tr, int kDP, bool kAsync, class F, class X, class B>
+__device__ __forceinline__ void for_blocks(F& f0, F& f1, int first, int end, int limit, char* buf, int stride, X&& extra, B&& body) {
+  constexpr int kBN = Block<Tr, kDP>::kBN, kHalf = Block<Tr, kDP>::kBytesAll;
+  if (first >= end) return;
+  auto issue = [&](char* p, int r) {
+    f0.issue(p, limit);
+    f1.issue(p + kHalf, limit);
+    extra(p + 2 * kHalf, r);
+    f0.advance();
+    f1.advance();
+  };
+  int cur = 0;
+  issue(buf, first);
+  if constexpr (!kAsync) {
+    f0.commit(buf);
+    f1.commit(buf + kHalf);
+  }
+  for (int r = first; r < end; r += kBN) {
+    block_landed();
+    char* next = buf + (cur ^ 1) * stride;
+    if (r + kBN < end) issue(next, r + kBN);
+    body(buf + cur * stride, r);
+    if constexpr (!kAsync) {
+      if (r + kBN < end) {
+        f0.commit(next);
+        f1.commit(next + kHalf);
+      }
+    }
+    cur ^= 1;
+  }
+}
 
 // 4 elements d0 .. of an output row
 template <class Tr>
@@ -170,11 +263,15 @@ __device__ __forceinline__ void store_out(typename Tr::T* p, int d0, int d, f32x
   }
 }
 
-// One column's running softmax over a block of kT score tiles (raw scores in st; p comes back in
-// it), keys beyond `lim` left out.  m is the running maximum of score * scale * log2 e, l this
-// lane's share of the denominator.  Returns the factor for what was accumulated before.
-template <int kT>
-__device__ __forceinline__ float softmax_step(f32x4* st, int key0, int lim, bool mask, float sl2, float& m, float& l) {
+// One column's running softmax over a block of kT score tiles: raw scores in st, p comes back in
+// it, keys beyond `lim` left out (mask: some lane has any).  m is the reference of the column's
+// exponents, in score * scale * log2 e: not the running maximum itself but at most kLag below
+// it, so that most blocks need neither the other lanes' maxima nor a rescaling (p then reaches 2^kLag,
+// which costs no accuracy).  l: this lane's share of the denominator, from p as it is before any
+// rounding.  rescale(f): what else was accumulated so far times f.
+constexpr float kLag = 8.f;
+template <int kT, class R>
+__device__ __forceinline__ void softmax_step(f32x4* st, int key0, int lim, bool mask, float sl2, float& m, float& l, R&& rescale) {
   const int g = (threadIdx.x & 63) >> 4;
   if (mask) {
 #pragma unroll
@@ -184,36 +281,50 @@ __device__ __forceinline__ float softmax_step(f32x4* st, int key0, int lim, bool
   }
   float mx = -INFINITY;
 #pragma unroll
-  for (int t = 0; t < kT; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, st[t][i]);
-  mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-  const float mn = fmaxf(m, mx * sl2);
-  const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every p is exp2(-inf) = 0
-  const float alpha = __builtin_amdgcn_exp2f(m - ref);
-  float s = 0.f;
+  for (int t = 0; t < kT; ++t) mx = fmaxf(fmaxf(fmaxf(mx, st[t][0]), fmaxf(st[t][1], st[t][2])), st[t][3]);
+  mx *= sl2;
+  if (__any(mx > m + kLag)) {
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float mn = fmaxf(m, mx);
+    const float f = exp2_f(m - (mn == -INFINITY ? 0.f : mn));
+    l *= f;
+    rescale(f);
+    m = mn;
+  }
+  const float ref = m == -INFINITY ? 0.f : m;  // nothing seen yet: every p is exp2(-inf) = 0
 #pragma unroll
   for (int t = 0; t < kT; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float p = __builtin_amdgcn_exp2f(fmaf(st[t][i], sl2, -ref));
-      st[t][i] = p;
-      s += p;
+      st[t][i] = exp2_f(fmaf(st[t][i], sl2, -ref));
+      l += st[t][i];
     }
-  l = l * alpha + s;
-  m = mn;
-  return alpha;
 }
 
-// Forward: 4 waves of 16 kNT rows, key blocks through LDS, the next one's loads in flight meanwhile.
-template <class Tr, int kDP, int kNT>
+// A column's sum over the lanes that share it.
+__device__ __forceinline__ float column_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+// Keys that a block of rows [r0, r0 + n) sees: its last row in use sees most.
+__device__ __forceinline__ int key_end(const AttnArgs& a, const Seq& s, int r0, int n) {
+  if (query_of(r0, a.group) >= s.qlen) return 0;
+  if (!a.causal) return s.klen;
+  int i = query_of((r0 + n < a.rows ? r0 + n : a.rows) - 1, a.group);
+  i = i < s.qlen ? i : s.qlen - 1;
+  return i + s.off + 1;
+}
+
+// Forward: 4 waves of 16 kNT rows.
+template <class Tr, int kDP, int kNT, bool kAsync>
 __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a, int row_blocks) {
   using T = typename Tr::T;
   using V8 = typename Tr::V8;
   using Bl = Block<Tr, kDP>;
-  constexpr int kKT = Bl::kBN / 16, kS = kDP / 32, kDT = kDP / 16, kRows = 64 * kNT;
-  __shared__ __attribute__((aligned(16))) char lk[Bl::kBytesAll], lv[Bl::kBytesAll];
+  constexpr int kKT = Bl::kBN / 16, kS = kDP / 32, kDT = kDP / 16, kRows = 64 * kNT, kBuf = 2 * Bl::kBytesAll;
+  __shared__ __attribute__((aligned(16))) char lds[2 * kBuf];
   const int lane = threadIdx.x & 63, wave = rfl(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
   const int item = xcd_item(blockIdx.x, gridDim.x);
   // long causal rows first
@@ -221,18 +332,6 @@ __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a, int row_blocks) {
   const int b = bh / a.hk, hk = bh - b * a.hk;
   const Seq s = seq_of(a, b);
   const int r0 = rb * kRows;
-  const T* kb = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
-  const T* vb = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
-  const int last = (r0 + kRows < a.rows ? r0 + kRows : a.rows) - 1;
-  // the last row in use of this block sees most
-  int kend = s.klen;
-  if (query_of(r0, a.group) >= s.qlen) {
-    kend = 0;
-  } else if (a.causal) {
-    int i = query_of(last, a.group);
-    i = i < s.qlen ? i : s.qlen - 1;
-    kend = i + s.off + 1;
-  }
   V8 qf[kNT][kS];
   int lim[kNT];
   float m[kNT], l[kNT];
@@ -250,20 +349,11 @@ __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a, int row_blocks) {
     for (int t = 0; t < kDT; ++t) acc[j][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const float sl2 = a.scale * kLog2e;
-  Stage<Tr, kDP> sk, sv;
-  if (kend > 0) {
-    sk.load_keys(kb, a.ks[1], 0, s.klen, a.d);
-    sv.load_keys(vb, a.vs[1], 0, s.klen, a.d);
-  }
-  for (int k0 = 0; k0 < kend; k0 += Bl::kBN) {
-    __syncthreads();
-    sk.store(lk);
-    sv.store(lv);
-    __syncthreads();
-    if (k0 + Bl::kBN < kend) {
-      sk.load_keys(kb, a.ks[1], k0 + Bl::kBN, s.klen, a.d);
-      sv.load_keys(vb, a.vs[1], k0 + Bl::kBN, s.klen, a.d);
-    }
+  Feed<Tr, kDP, kAsync> fk, fv;
+  fk.init(a.k, a.ks, b, hk, 1, a.d, 0);
+  fv.init(a.v, a.vs, b, hk, 1, a.d, 0);
+  for_blocks<Tr, kDP, kAsync>(fk, fv, 0, key_end(a, s, r0, kRows), s.klen, lds, kBuf, [](char*, int) {}, [&](const char* lk, int k0) {
+    const char* lv = lk + Bl::kBytesAll;
     f32x4 st[kNT][kKT];
 #pragma unroll
     for (int t = 0; t < kKT; ++t) {
@@ -279,10 +369,10 @@ __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a, int row_blocks) {
     V8 pf[kNT][kKT / 2];
 #pragma unroll
     for (int j = 0; j < kNT; ++j) {
-      const bool mask = __any(lim[j] < k0 + Bl::kBN);
-      const float alpha = softmax_step<kKT>(st[j], k0, lim[j], mask, sl2, m[j], l[j]);
+      softmax_step<kKT>(st[j], k0, lim[j], __any(lim[j] < k0 + Bl::kBN), sl2, m[j], l[j], [&](float f) {
 #pragma unroll
-      for (int t = 0; t < kDT; ++t) acc[j][t] *= alpha;
+        for (int t = 0; t < kDT; ++t) acc[j][t] *= f;
+      });
 #pragma unroll
       for (int u = 0; u < kKT / 2; ++u) pf[j][u] = pack8<Tr>(st[j][2 * u], st[j][2 * u + 1]);
     }
@@ -294,21 +384,19 @@ __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a, int row_blocks) {
 #pragma unroll
         for (int j = 0; j < kNT; ++j) acc[j][t] = mma<Tr>(vf, pf[j][u], acc[j][t]);
       }
-  }
+  });
 #pragma unroll
   for (int j = 0; j < kNT; ++j) {
     const int r = r0 + (wave * kNT + j) * 16 + l16;
-    l[j] += __shfl_xor(l[j], 16, 64);
-    l[j] += __shfl_xor(l[j], 32, 64);
+    const float sum = column_sum(l[j]);
     if (r >= a.rows) continue;
-    const float inv = l[j] == 0.f ? 0.f : 1.f / l[j];
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T* o = row_ptr((T*)a.out, a.os, b, hk, a.group, r);
 #pragma unroll
     for (int t = 0; t < kDT; ++t) store_out<Tr>(o, t * 16 + g * 4, a.d, acc[j][t] * inv);
     if (a.lse && g == 0) {
       const int i = query_of(r, a.group);
-      a.lse[((int64_t)(b * a.hk + hk) * a.group + (r - i * a.group)) * a.nq + i] =
-          l[j] == 0.f ? -INFINITY : fmaf(m[j], kLn2, logf(l[j]));
+      a.lse[((int64_t)(b * a.hk + hk) * a.group + (r - i * a.group)) * a.nq + i] = sum == 0.f ? -INFINITY : fmaf(m[j], kLn2, logf(sum));
     }
   }
 }
@@ -369,13 +457,14 @@ __global__ __launch_bounds__(256) void attn_split_kernel(AttnArgs a, int row_blo
       for (int c = 0; c < kS; ++c) st[t] = mma<Tr>(kf[t][c], qf[c], st[t]);
     }
     const int lim2 = lim < k_end ? lim : k_end;
-    const float alpha = softmax_step<kKT>(st, k0, lim2, __any(lim2 < k0 + Bl::kBN), sl2, m, l);
+    softmax_step<kKT>(st, k0, lim2, __any(lim2 < k0 + Bl::kBN), sl2, m, l, [&](float f) {
 #pragma unroll
-    for (int t = 0; t < kDT; ++t) acc[t] *= alpha;
+      for (int t = 0; t < kDT; ++t) acc[t] *= f;
+    });
 #pragma unroll
     for (int i = 0; i < kVN; ++i) {
       const int j = i * 64 + lane, row = j / Bl::kRowChunks, c = j % Bl::kRowChunks;
-      *(u32x4*)(lv + row * Bl::kPitch + c * 16) = vr[i];
+      *(u32x4*)(lv + row * Bl::kRow + Bl::place(row, c) * 16) = vr[i];
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -388,8 +477,7 @@ __global__ __launch_bounds__(256) void attn_split_kernel(AttnArgs a, int row_blo
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
+  l = column_sum(l);
   if (g == 0) {
     stat[wave][0][l16] = m;
     stat[wave][1][l16] = l;
@@ -490,22 +578,20 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs a) {
   a.part[all + id] = s;
 }
 
-// dk and dv: 4 waves of 16 kNT keys, blocks of packed rows (q, do) through LDS.
-template <class Tr, int kDP, int kNT>
+// dk and dv: 4 waves of 16 kNT keys, blocks of packed rows (q, do and their statistics) through LDS.
+template <class Tr, int kDP, int kNT, bool kAsync>
 __global__ __launch_bounds__(256) void attn_dkv_kernel(AttnArgs a, int key_blocks) {
   using T = typename Tr::T;
   using V8 = typename Tr::V8;
   using Bl = Block<Tr, kDP>;
-  constexpr int kRT = Bl::kBN / 16, kS = kDP / 32, kDT = kDP / 16, kKeys = 64 * kNT;
-  __shared__ __attribute__((aligned(16))) char lq[Bl::kBytesAll], lo[Bl::kBytesAll];
-  __shared__ __attribute__((aligned(16))) float stat[2][Bl::kBN];
+  constexpr int kRT = Bl::kBN / 16, kS = kDP / 32, kDT = kDP / 16, kKeys = 64 * kNT, kBuf = 2 * Bl::kBytesAll + 8 * Bl::kBN;
+  __shared__ __attribute__((aligned(16))) char lds[2 * kBuf];
   const int lane = threadIdx.x & 63, wave = rfl(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
   const int item = xcd_item(blockIdx.x, gridDim.x);
   const int bh = item / key_blocks, key0 = (item - bh * key_blocks) * kKeys;
   const int b = bh / a.hk, hk = bh - b * a.hk;
   const Seq s = seq_of(a, b);
   const int64_t all = (int64_t)a.b * a.hk * a.rows;
-  const float* lse2 = a.part + (int64_t)bh * a.rows;
   V8 kf[kNT][kS], vf[kNT][kS];
   f32x4 dk[kNT][kDT], dv[kNT][kDT];
 #pragma unroll
@@ -526,31 +612,31 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(AttnArgs a, int key_block
   if (a.causal && key0 > s.off) r_begin = (int)((int64_t)(key0 - s.off) * a.group < r_end ? (int64_t)(key0 - s.off) * a.group : r_end);
   r_begin = r_begin / Bl::kBN * Bl::kBN;
   const float sl2 = a.scale * kLog2e;
-  Stage<Tr, kDP> sq, so;
-  float st_lse = 0.f, st_delta = 0.f;
-  auto fetch = [&](int r0) {
-    sq.load_rows((const T*)a.q, a.qs, b, hk, a.group, r0, r_end, a.d);
-    so.load_rows((const T*)a.go, a.gos, b, hk, a.group, r0, r_end, a.d);
-    if (threadIdx.x < Bl::kBN) {
-      const int r = r0 + threadIdx.x;
-      st_lse = r < r_end ? lse2[r] : INFINITY;
-      st_delta = r < r_end ? lse2[all + r] : 0.f;
+  Feed<Tr, kDP, kAsync> fq, fo;
+  fq.init(a.q, a.qs, b, hk * a.group, a.group, a.d, r_begin);
+  fo.init(a.go, a.gos, b, hk * a.group, a.group, a.d, r_begin);
+  // lse and delta of a block: waves 0 and 1, a lane a row.  Rows at and past the end read as zero,
+  // which with their q = do = 0 leaves nothing.
+  auto stats = [&](char* to, int r0) {
+    const int i = threadIdx.x & 63;
+    if (wave >= 2 || i >= Bl::kBN) return;
+    const float* p = a.part + (wave ? all : 0) + (int64_t)bh * a.rows + r0;
+    char* at = to + wave * 4 * Bl::kBN;
+    if constexpr (kAsync) {
+      const size_t ub = (size_t)p;
+      const size_t us = ((size_t)(unsigned)rfl((int)(ub >> 32)) << 32) | (unsigned)rfl((int)ub);
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)us, (short)0, 0x7ffffff0, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)at, 4,
+                                               r0 + i < r_end ? i * 4u : 0x80000000u, 0, 0, 0);
+    } else {
+      *(float*)(at + i * 4) = r0 + i < r_end ? p[i] : 0.f;
     }
   };
-  if (r_begin < r_end) fetch(r_begin);
-  for (int r0 = r_begin; r0 < r_end; r0 += Bl::kBN) {
-    __syncthreads();
-    sq.store(lq);
-    so.store(lo);
-    if (threadIdx.x < Bl::kBN) {
-      stat[0][threadIdx.x] = st_lse;
-      stat[1][threadIdx.x] = st_delta;
-    }
-    __syncthreads();
-    if (r0 + Bl::kBN < r_end) fetch(r0 + Bl::kBN);
+  for_blocks<Tr, kDP, kAsync>(fq, fo, r_begin, r_end, r_end, lds, kBuf, stats, [&](const char* lq, int r0) {
+    const char* lo = lq + Bl::kBytesAll;
+    const float* stat = (const float*)(lo + Bl::kBytesAll);
     // the block's first query sees least
-    const int sees = query_of(r0, a.group) + s.off;
-    const bool mask = a.causal && key0 + kKeys - 1 > sees;
+    const bool mask = a.causal && key0 + kKeys - 1 > query_of(r0, a.group) + s.off;
 #pragma unroll
     for (int u = 0; u < kRT / 2; ++u) {
       f32x4 p[kNT][2], ds[kNT][2];
@@ -568,17 +654,19 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(AttnArgs a, int key_block
             ds[j][h] = mma<Tr>(of, vf[j][c], ds[j][h]);
           }
         }
-        const f32x4 ls = *(const f32x4*)&stat[0][t * 16 + g * 4], dl = *(const f32x4*)&stat[1][t * 16 + g * 4];
+        const f32x4 ls = *(const f32x4*)(stat + t * 16 + g * 4), dl = *(const f32x4*)(stat + Bl::kBN + t * 16 + g * 4);
 #pragma unroll
         for (int j = 0; j < kNT; ++j) {
-          const int key = key0 + (wave * kNT + j) * 16 + l16;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float e = __builtin_amdgcn_exp2f(fmaf(p[j][h][i], sl2, -ls[i]));
-            if (mask && key > query_of(r0 + t * 16 + g * 4 + i, a.group) + s.off) e = 0.f;
-            p[j][h][i] = e;
-            ds[j][h][i] = e * (ds[j][h][i] - dl[i]);
+          for (int i = 0; i < 4; ++i) p[j][h][i] = exp2_f(fmaf(p[j][h][i], sl2, -ls[i]));
+          if (mask) {
+            const int key = key0 + (wave * kNT + j) * 16 + l16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (key > query_of(r0 + t * 16 + g * 4 + i, a.group) + s.off) p[j][h][i] = 0.f;
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ds[j][h][i] = p[j][h][i] * (ds[j][h][i] - dl[i]);
         }
       }
       V8 pf[kNT], df[kNT];
@@ -597,7 +685,7 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(AttnArgs a, int key_block
         }
       }
     }
-  }
+  });
 #pragma unroll
   for (int j = 0; j < kNT; ++j) {
     const int key = key0 + (wave * kNT + j) * 16 + l16;
@@ -615,30 +703,19 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(AttnArgs a, int key_block
 }
 
 // dq: 4 waves of 16 kNT rows, key blocks (k, v) through LDS.
-template <class Tr, int kDP, int kNT>
+template <class Tr, int kDP, int kNT, bool kAsync>
 __global__ __launch_bounds__(256) void attn_dq_kernel(AttnArgs a, int row_blocks) {
   using T = typename Tr::T;
   using V8 = typename Tr::V8;
   using Bl = Block<Tr, kDP>;
-  constexpr int kKT = Bl::kBN / 16, kS = kDP / 32, kDT = kDP / 16, kRows = 64 * kNT;
-  __shared__ __attribute__((aligned(16))) char lk[Bl::kBytesAll], lv[Bl::kBytesAll];
+  constexpr int kKT = Bl::kBN / 16, kS = kDP / 32, kDT = kDP / 16, kRows = 64 * kNT, kBuf = 2 * Bl::kBytesAll;
+  __shared__ __attribute__((aligned(16))) char lds[2 * kBuf];
   const int lane = threadIdx.x & 63, wave = rfl(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
   const int item = xcd_item(blockIdx.x, gridDim.x);
   const int bh = item / row_blocks, rb = a.causal ? row_blocks - 1 - (item - bh * row_blocks) : item - bh * row_blocks;
   const int b = bh / a.hk, hk = bh - b * a.hk;
   const Seq s = seq_of(a, b);
   const int r0 = rb * kRows;
-  const T* kb = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
-  const T* vb = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
-  const int last = (r0 + kRows < a.rows ? r0 + kRows : a.rows) - 1;
-  int kend = s.klen;
-  if (query_of(r0, a.group) >= s.qlen) {
-    kend = 0;
-  } else if (a.causal) {
-    int i = query_of(last, a.group);
-    i = i < s.qlen ? i : s.qlen - 1;
-    kend = i + s.off + 1;
-  }
   const int64_t all = (int64_t)a.b * a.hk * a.rows;
   const float* lse2 = a.part + (int64_t)bh * a.rows;
   V8 qf[kNT][kS], of[kNT][kS];
@@ -660,20 +737,11 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(AttnArgs a, int row_blocks
     for (int t = 0; t < kDT; ++t) dq[j][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const float sl2 = a.scale * kLog2e;
-  Stage<Tr, kDP> sk, sv;
-  if (kend > 0) {
-    sk.load_keys(kb, a.ks[1], 0, s.klen, a.d);
-    sv.load_keys(vb, a.vs[1], 0, s.klen, a.d);
-  }
-  for (int k0 = 0; k0 < kend; k0 += Bl::kBN) {
-    __syncthreads();
-    sk.store(lk);
-    sv.store(lv);
-    __syncthreads();
-    if (k0 + Bl::kBN < kend) {
-      sk.load_keys(kb, a.ks[1], k0 + Bl::kBN, s.klen, a.d);
-      sv.load_keys(vb, a.vs[1], k0 + Bl::kBN, s.klen, a.d);
-    }
+  Feed<Tr, kDP, kAsync> fk, fv;
+  fk.init(a.k, a.ks, b, hk, 1, a.d, 0);
+  fv.init(a.v, a.vs, b, hk, 1, a.d, 0);
+  for_blocks<Tr, kDP, kAsync>(fk, fv, 0, key_end(a, s, r0, kRows), s.klen, lds, kBuf, [](char*, int) {}, [&](const char* lk, int k0) {
+    const char* lv = lk + Bl::kBytesAll;
 #pragma unroll
     for (int u = 0; u < kKT / 2; ++u) {
       f32x4 p[kNT][2], ds[kNT][2];
@@ -693,13 +761,15 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(AttnArgs a, int row_blocks
         }
 #pragma unroll
         for (int j = 0; j < kNT; ++j) {
-          const bool mask = __any(lim[j] < k0 + Bl::kBN);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float e = __builtin_amdgcn_exp2f(fmaf(p[j][h][i], sl2, -ls[j]));
-            if (mask && k0 + t * 16 + g * 4 + i >= lim[j]) e = 0.f;
-            ds[j][h][i] = e * (ds[j][h][i] - dl[j]);
+          for (int i = 0; i < 4; ++i) p[j][h][i] = exp2_f(fmaf(p[j][h][i], sl2, -ls[j]));
+          if (__any(lim[j] < k0 + Bl::kBN)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (k0 + t * 16 + g * 4 + i >= lim[j]) p[j][h][i] = 0.f;
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ds[j][h][i] = p[j][h][i] * (ds[j][h][i] - dl[j]);
         }
       }
       V8 df[kNT];
@@ -712,7 +782,7 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(AttnArgs a, int row_blocks
         for (int j = 0; j < kNT; ++j) dq[j][t] = mma<Tr>(kf, df[j], dq[j][t]);
       }
     }
-  }
+  });
 #pragma unroll
   for (int j = 0; j < kNT; ++j) {
     const int r = r0 + (wave * kNT + j) * 16 + l16;
@@ -732,11 +802,9 @@ inline int pad_d(int d) { return (d + 31) / 32 * 32; }
 // lane masks than there are scalar registers
 inline int split_pad(int d) { return pad_d(d) == 96 ? 128 : pad_d(d); }
 
-// Row tiles per wave of the forward and dq kernels (a fragment read from LDS serves all of them):
-// two for 16-bit heads while the workgroups still fill the chip
-inline int row_tiles(int bytes, int64_t bh, int64_t rows) {
-  return bytes == 2 && bh * cdiv(rows, 128) >= kCUs ? 2 : 1;
-}
+// Two 16-wide tiles per wave (a fragment read from LDS serves both): 16-bit types, while the
+// workgroups still fill the chip
+inline bool two_tiles(int bytes, int64_t bh, int64_t n) { return bytes == 2 && bh * cdiv(n, 128) >= kCUs; }
 // Key ranges of the few-rows kernel; 0: the block kernel takes the call
 inline int split_count(int bytes, int64_t bh, int64_t rows, int64_t nk) {
   const int64_t wgs = bh * cdiv(rows, 64), items = bh * cdiv(rows, 16);
@@ -756,27 +824,62 @@ void run_split(const AttnArgs& a, hipStream_t st) {
     hipLaunchKernelGGL(attn_join_kernel<Tr>, dim3((unsigned)(bh * a.rows)), dim3(64), 0, st, a, rb, kDP);
 }
 
+// What Feed's kAsync needs of one operand: chunks whole and on 16-byte boundaries, a block's offsets
+// below 2^30.
+inline bool feed_async(const char* p, const int64_t* st, int d, int group, int bytes) {
+  const int64_t bn = 128 / bytes;
+  for (int i = 0; i < 3; ++i)
+    if (st[i] * bytes % 16) return false;
+  return (uintptr_t)p % 16 == 0 && d * bytes % 16 == 0 && bn % group == 0 && st[1] >= 0 && st[2] >= 0 &&
+         (bn / group * st[1] + group * st[2]) * bytes < (int64_t(1) << 30);
+}
+
+template <class Tr, int kDP, int kNT>
+void launch_fwd(const AttnArgs& a, bool async, hipStream_t st) {
+  const int rb = (int)cdiv(a.rows, 64 * kNT);
+  const dim3 grid((unsigned)((int64_t)a.b * a.hk * rb));
+  if (async) hipLaunchKernelGGL((attn_kernel<Tr, kDP, kNT, true>), grid, dim3(256), 0, st, a, rb);
+  else hipLaunchKernelGGL((attn_kernel<Tr, kDP, kNT, false>), grid, dim3(256), 0, st, a, rb);
+}
+template <class Tr, int kDP, int kNT>
+void launch_dkv(const AttnArgs& a, bool async, hipStream_t st) {
+  const int kb = (int)cdiv(a.nk, 64 * kNT);
+  const dim3 grid((unsigned)((int64_t)a.b * a.hk * kb));
+  if (async) hipLaunchKernelGGL((attn_dkv_kernel<Tr, kDP, kNT, true>), grid, dim3(256), 0, st, a, kb);
+  else hipLaunchKernelGGL((attn_dkv_kernel<Tr, kDP, kNT, false>), grid, dim3(256), 0, st, a, kb);
+}
+template <class Tr, int kDP, int kNT>
+void launch_dq(const AttnArgs& a, bool async, hipStream_t st) {
+  const int rb = (int)cdiv(a.rows, 64 * kNT);
+  const dim3 grid((unsigned)((int64_t)a.b * a.hk * rb));
+  if (async) hipLaunchKernelGGL((attn_dq_kernel<Tr, kDP, kNT, true>), grid, dim3(256), 0, st, a, rb);
+  else hipLaunchKernelGGL((attn_dq_kernel<Tr, kDP, kNT, false>), grid, dim3(256), 0, st, a, rb);
+}
+
 template <class Tr, int kDP>
 void run_fwd(const AttnArgs& a, hipStream_t st) {
-  const int64_t bh = (int64_t)a.b * a.hk;
-  if (row_tiles(Tr::kBytes, bh, a.rows) == 2) {
-    if constexpr (Tr::kBytes == 2) {
-      const int rb = (int)cdiv(a.rows, 128);
-      hipLaunchKernelGGL((attn_kernel<Tr, kDP, 2>), dim3((unsigned)(bh * rb)), dim3(256), 0, st, a, rb);
-    }
-  } else {
-    const int rb = (int)cdiv(a.rows, 64);
-    hipLaunchKernelGGL((attn_kernel<Tr, kDP, 1>), dim3((unsigned)(bh * rb)), dim3(256), 0, st, a, rb);
+  const bool async = feed_async(a.k, a.ks, a.d, 1, Tr::kBytes) && feed_async(a.v, a.vs, a.d, 1, Tr::kBytes);
+  if constexpr (Tr::kBytes == 2) {
+    if (two_tiles(Tr::kBytes, (int64_t)a.b * a.hk, a.rows)) return launch_fwd<Tr, kDP, 2>(a, async, st);
   }
+  launch_fwd<Tr, kDP, 1>(a, async, st);
 }
 
 template <class Tr, int kDP>
 void run_bwd(const AttnArgs& a, hipStream_t st) {
   const int64_t bh = (int64_t)a.b * a.hk;
   hipLaunchKernelGGL(attn_delta_kernel<Tr>, dim3((unsigned)cdiv(bh * a.rows, 16)), dim3(256), 0, st, a);
-  const int rb = (int)cdiv(a.rows, 64), kb = (int)cdiv(a.nk, 64);
-  hipLaunchKernelGGL((attn_dkv_kernel<Tr, kDP, 1>), dim3((unsigned)(bh * kb)), dim3(256), 0, st, a, kb);
-  hipLaunchKernelGGL((attn_dq_kernel<Tr, kDP, 1>), dim3((unsigned)(bh * rb)), dim3(256), 0, st, a, rb);
+  const bool rows = feed_async(a.q, a.qs, a.d, a.group, Tr::kBytes) && feed_async(a.go, a.gos, a.d, a.group, Tr::kBytes);
+  const bool keys = feed_async(a.k, a.ks, a.d, 1, Tr::kBytes) && feed_async(a.v, a.vs, a.d, 1, Tr::kBytes);
+  if constexpr (Tr::kBytes == 2) {
+    if (kDP <= 64 && two_tiles(Tr::kBytes, bh, a.nk)) launch_dkv<Tr, kDP, kDP <= 64 ? 2 : 1>(a, rows, st);
+    else launch_dkv<Tr, kDP, 1>(a, rows, st);
+    if (two_tiles(Tr::kBytes, bh, a.rows)) launch_dq<Tr, kDP, 2>(a, keys, st);
+    else launch_dq<Tr, kDP, 1>(a, keys, st);
+  } else {
+    launch_dkv<Tr, kDP, 1>(a, rows, st);
+    launch_dq<Tr, kDP, 1>(a, keys, st);
+  }
 }
 
 template <class Tr>
