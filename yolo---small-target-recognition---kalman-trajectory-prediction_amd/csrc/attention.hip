@@ -26,7 +26,7 @@ struct AttnArgs {
   float* lse;         // [b][hq][nq]
   const int32_t *q_lengths, *lengths;
   int64_t qs[3], ks[3], vs[3], os[3], gos[3], dqs[3], dks[3], dvs[3];
-  float* part;        // split: [item][split][16][d_pad + 2]; backward: lse2, delta [b][hk][rows]
+  float* part;        // split: [item][split][16][d_pad + 4]; backward: lse2, delta [b][hk][rows]
   float scale;
   int b, hk, group, d, nq, nk, causal, rows, splits;  // rows = nq * group
 };
@@ -401,17 +401,21 @@ __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a, int row_blocks) {
   }
 }
 
-// Few rows, long keys: 16 rows per workgroup, whose waves walk different key blocks on their own
-// (fragments of k straight from memory, v through a wave's own LDS), and blockIdx.y a range of
-// keys.  The waves' sums meet in LDS; ranges go to scratch unless there is one.
-template <class Tr, int kDP>
-__global__ __launch_bounds__(256) void attn_split_kernel(AttnArgs a, int row_blocks) {
+// Few rows, long keys: 16 rows per workgroup and blockIdx.y a range of keys, which the waves walk 32
+// keys at a time on their own, each through two slabs of LDS of its own (no barrier; the next slab on
+// its way while one is worked on).  The waves' sums meet in LDS; ranges go to scratch unless there is
+// one.  Bound by the keys' and values' bytes: what counts is how many are on their way per CU
+// (64 KiB with two workgroups of four waves at d = 64).
+template <class Tr, int kDP, int kWaves, bool kAsync>
+__global__ __launch_bounds__(64 * kWaves) void attn_split_kernel(AttnArgs a, int row_blocks) {
   using T = typename Tr::T;
   using V8 = typename Tr::V8;
   using Bl = Block<Tr, kDP>;
-  constexpr int kKT = Bl::kBN / 16, kS = kDP / 32, kDT = kDP / 16, kVN = Bl::kN * 4;
-  __shared__ __attribute__((aligned(16))) char lds[4 * Bl::kBytesAll];
-  __shared__ float stat[4][2][16];
+  constexpr int kKeys = 32, kS = kDP / 32, kDT = kDP / 16, kHalf = kKeys * Bl::kRow, kN = kHalf / 1024;
+  constexpr unsigned kOut = 0x80000000u;
+  __shared__ __attribute__((aligned(16))) char lds[kWaves * 4 * kHalf];
+  __shared__ float stat[kWaves][2][16];
+  static_assert(kDT * 1024 <= 4 * kHalf, "a wave's sums fit its slabs");
   const int lane = threadIdx.x & 63, wave = rfl(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
   const int bh = blockIdx.x / row_blocks, rb = blockIdx.x - bh * row_blocks;
   const int b = bh / a.hk, hk = bh - b * a.hk;
@@ -420,10 +424,10 @@ __global__ __launch_bounds__(256) void attn_split_kernel(AttnArgs a, int row_blo
   const int lim = key_limit(a, s, r);
   const T* kb = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
   const T* vb = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
-  // the range of this workgroup: whole key blocks
-  const int blocks = (s.klen + Bl::kBN - 1) / Bl::kBN, per = (blocks + a.splits - 1) / a.splits;
-  const int k_begin = blockIdx.y * per * Bl::kBN;
-  int k_end = k_begin + per * Bl::kBN < s.klen ? k_begin + per * Bl::kBN : s.klen;
+  // the range of this workgroup: whole slabs for each of its waves
+  const int turns = (s.klen + kKeys * kWaves - 1) / (kKeys * kWaves), per = (turns + a.splits - 1) / a.splits;
+  const int64_t k_begin = (int64_t)blockIdx.y * per * kKeys * kWaves;
+  const int k_end = (int)(k_begin + per * kKeys * kWaves < s.klen ? k_begin + per * kKeys * kWaves : s.klen);
   V8 qf[kS];
 #pragma unroll
   for (int c = 0; c < kS; ++c)
@@ -433,82 +437,103 @@ __global__ __launch_bounds__(256) void attn_split_kernel(AttnArgs a, int row_blo
 #pragma unroll
   for (int t = 0; t < kDT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   const float sl2 = a.scale * kLog2e;
-  char* lv = lds + wave * Bl::kBytesAll;
-  for (int k0 = k_begin + wave * Bl::kBN; k0 < k_end; k0 += 4 * Bl::kBN) {
-    V8 kf[kKT][kS];
-    u32x4 vr[kVN];
+  char* mine = lds + wave * 4 * kHalf;
+
+  unsigned ko[kAsync ? kN : 1], vo[kAsync ? kN : 1];
+  if constexpr (kAsync) {
 #pragma unroll
-    for (int t = 0; t < kKT; ++t)
-#pragma unroll
-      for (int c = 0; c < kS; ++c) {
-        const int key = k0 + t * 16 + l16;
-        kf[t][c] = load8<Tr>(kb + (int64_t)key * a.ks[1], kb, c * 32 + g * 8, a.d, key < k_end);
-      }
-#pragma unroll
-    for (int i = 0; i < kVN; ++i) {
-      const int j = i * 64 + lane, row = j / Bl::kRowChunks, c = (j % Bl::kRowChunks) * Bl::kEpc;
-      vr[i] = load16_if<Tr>(vb + (int64_t)(k0 + row) * a.vs[1] + c, vb, a.d - c, k0 + row < k_end, a.d % Bl::kEpc == 0);
+    for (int i = 0; i < kN; ++i) {
+      const int j = i * 64 + lane, row = j / Bl::kRowChunks, c = Bl::place(row, j % Bl::kRowChunks) * Bl::kEpc;
+      ko[i] = c < a.d ? (unsigned)((row * (int)a.ks[1] + c) * Tr::kBytes) : kOut;
+      vo[i] = c < a.d ? (unsigned)((row * (int)a.vs[1] + c) * Tr::kBytes) : kOut;
     }
-    f32x4 st[kKT];
+  }
+  auto issue = [&](char* to, int k0) {
+    if constexpr (kAsync) {
+      const bool tail = k0 + kKeys > k_end;
+      auto one = [&](const T* p, const unsigned* off, char* at) {
+        const size_t u = (size_t)p;
+        const size_t us = ((size_t)(unsigned)rfl((int)(u >> 32)) << 32) | (unsigned)rfl((int)u);
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)us, (short)0, 0x7ffffff0, 0x00020000);
 #pragma unroll
-    for (int t = 0; t < kKT; ++t) {
+        for (int i = 0; i < kN; ++i) {
+          unsigned o = off[i];
+          if (tail && k0 + (i * 64 + lane) / Bl::kRowChunks >= k_end) o = kOut;
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(at + i * 1024), 16, o, 0, 0, 0);
+        }
+      };
+      one(kb + (int64_t)k0 * a.ks[1], ko, to);
+      one(vb + (int64_t)k0 * a.vs[1], vo, to + kHalf);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int j = i * 64 + lane, row = j / Bl::kRowChunks, c = j % Bl::kRowChunks, e = c * Bl::kEpc;
+        const bool whole = a.d % Bl::kEpc == 0, in = k0 + row < k_end;
+        *(u32x4*)(to + row * Bl::kRow + Bl::place(row, c) * 16) =
+            load16_if<Tr>(kb + (int64_t)(k0 + row) * a.ks[1] + e, kb, a.d - e, in, whole);
+        *(u32x4*)(to + kHalf + row * Bl::kRow + Bl::place(row, c) * 16) =
+            load16_if<Tr>(vb + (int64_t)(k0 + row) * a.vs[1] + e, vb, a.d - e, in, whole);
+      }
+    }
+  };
+  int cur = 0;
+  const int first = (int)k_begin + wave * kKeys;
+  if (k_begin < k_end && first < k_end) issue(mine, first);
+  for (int k0 = first; k_begin < k_end && k0 < k_end; k0 += kKeys * kWaves) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other slab's last reads are done
+    if (k0 + kKeys * kWaves < k_end) {
+      issue(mine + (cur ^ 1) * 2 * kHalf, k0 + kKeys * kWaves);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kAsync ? 2 * kN : 0) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    const char* lk = mine + cur * 2 * kHalf;
+    const char* lv = lk + kHalf;
+    f32x4 st[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
       st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < kS; ++c) st[t] = mma<Tr>(kf[t][c], qf[c], st[t]);
+      for (int c = 0; c < kS; ++c) st[t] = mma<Tr>(Bl::row_frag(lk, t, c, lane), qf[c], st[t]);
     }
     const int lim2 = lim < k_end ? lim : k_end;
-    softmax_step<kKT>(st, k0, lim2, __any(lim2 < k0 + Bl::kBN), sl2, m, l, [&](float f) {
+    softmax_step<2>(st, k0, lim2, __any(lim2 < k0 + kKeys), sl2, m, l, [&](float f) {
 #pragma unroll
       for (int t = 0; t < kDT; ++t) acc[t] *= f;
     });
+    const V8 pf = pack8<Tr>(st[0], st[1]);
 #pragma unroll
-    for (int i = 0; i < kVN; ++i) {
-      const int j = i * 64 + lane, row = j / Bl::kRowChunks, c = j % Bl::kRowChunks;
-      *(u32x4*)(lv + row * Bl::kRow + Bl::place(row, c) * 16) = vr[i];
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int u = 0; u < kKT / 2; ++u) {
-      const V8 pf = pack8<Tr>(st[2 * u], st[2 * u + 1]);
-#pragma unroll
-      for (int t = 0; t < kDT; ++t) acc[t] = mma<Tr>(Bl::col_frag(lv, t, u, lane), pf, acc[t]);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    for (int t = 0; t < kDT; ++t) acc[t] = mma<Tr>(Bl::col_frag(lv, t, 0, lane), pf, acc[t]);
+    cur ^= 1;
   }
   l = column_sum(l);
   if (g == 0) {
     stat[wave][0][l16] = m;
     stat[wave][1][l16] = l;
   }
-  __syncthreads();  // (also: every wave is done with its part of lds)
+  __syncthreads();
   float mm = stat[0][0][l16];
 #pragma unroll
-  for (int w = 1; w < 4; ++w) mm = fmaxf(mm, stat[w][0][l16]);
+  for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, stat[w][0][l16]);
   const float ref = mm == -INFINITY ? 0.f : mm;
-  const float f = __builtin_amdgcn_exp2f(m - ref);
+  const float f = exp2_f(m - ref);
   float ll = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) ll += stat[w][1][l16] * __builtin_amdgcn_exp2f(stat[w][0][l16] - ref);
-  float* sum = (float*)lds;  // [4 waves][kDT][64 lanes][4]
+  for (int w = 0; w < kWaves; ++w) ll += stat[w][1][l16] * exp2_f(stat[w][0][l16] - ref);
+  float* sum = (float*)mine;  // [kDT][64 lanes][4] of each wave
 #pragma unroll
-  for (int t = 0; t < kDT; ++t) *(f32x4*)(sum + ((wave * kDT + t) * 64 + lane) * 4) = acc[t] * f;
+  for (int t = 0; t < kDT; ++t) *(f32x4*)(sum + (t * 64 + lane) * 4) = acc[t] * f;
   __syncthreads();
   if (r >= a.rows) return;
   const bool one = a.splits == 1;
   const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  float* part = one ? nullptr : a.part + (((int64_t)blockIdx.x * a.splits + blockIdx.y) * 16 + l16) * (kDP + 2);
-  for (int t = wave; t < kDT; t += 4) {
+  float* part = one ? nullptr : a.part + (((int64_t)blockIdx.x * a.splits + blockIdx.y) * 16 + l16) * (kDP + 4);
+  for (int t = wave; t < kDT; t += kWaves) {
     f32x4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) v += *(const f32x4*)(sum + ((w * kDT + t) * 64 + lane) * 4);
-    if (one) {
-      store_out<Tr>(row_ptr((T*)a.out, a.os, b, hk, a.group, r), t * 16 + g * 4, a.d, v * inv);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) part[t * 16 + g * 4 + i] = v[i];
-    }
+    for (int w = 0; w < kWaves; ++w) v += *(const f32x4*)((float*)(lds + w * 4 * kHalf) + (t * 64 + lane) * 4);
+    if (one) store_out<Tr>(row_ptr((T*)a.out, a.os, b, hk, a.group, r), t * 16 + g * 4, a.d, v * inv);
+    else *(f32x4*)(part + t * 16 + g * 4) = v;
   }
   if (wave || g) return;
   if (!one) {
@@ -520,30 +545,53 @@ __global__ __launch_bounds__(256) void attn_split_kernel(AttnArgs a, int row_blo
   }
 }
 
-// The ranges of one row joined in order: a wave per row, two elements of it per lane.
+// The ranges of one row joined, in a fixed order: 4 waves take every fourth range each (8 at a time, so
+// that their loads overlap), two elements of the row per lane.
 template <class Tr>
-__global__ __launch_bounds__(64) void attn_join_kernel(AttnArgs a, int row_blocks, int dp) {
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int row_blocks, int dp) {
   using T = typename Tr::T;
-  const int lane = threadIdx.x, bh = blockIdx.x / a.rows, r = blockIdx.x - bh * a.rows;
+  __shared__ float sums[4][128], denom[4];
+  const int lane = threadIdx.x & 63, wave = rfl(threadIdx.x >> 6), bh = blockIdx.x / a.rows, r = blockIdx.x - bh * a.rows;
   const int b = bh / a.hk, hk = bh - b * a.hk;
-  const float* p = a.part + (((int64_t)(bh * row_blocks + r / 16) * a.splits) * 16 + r % 16) * (dp + 2);
-  const int64_t step = (int64_t)16 * (dp + 2);
+  const float* p = a.part + (((int64_t)(bh * row_blocks + r / 16) * a.splits) * 16 + r % 16) * (dp + 4);
+  const int64_t step = (int64_t)16 * (dp + 4);
   float mm = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, p[s * step + dp]);
+  for (int s = lane; s < a.splits; s += 64) mm = fmaxf(mm, p[s * step + dp]);
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) mm = fmaxf(mm, __shfl_xor(mm, x, 64));
   const float ref = mm == -INFINITY ? 0.f : mm;
+  const bool b0 = lane < a.d, b1 = lane + 64 < a.d;
   float ll = 0.f, v0 = 0.f, v1 = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float* q = p + s * step;
-    const float f = __builtin_amdgcn_exp2f(q[dp] - ref);
-    ll += q[dp + 1] * f;
-    if (lane < a.d) v0 += q[lane] * f;
-    if (lane + 64 < a.d) v1 += q[lane + 64] * f;
+  for (int s0 = wave; s0 < a.splits; s0 += 32) {
+    float e[8], n[8], x0[8], x1[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int s = s0 + 4 * i < a.splits ? s0 + 4 * i : s0;
+      const float* q = p + s * step;
+      e[i] = q[dp];
+      n[i] = q[dp + 1];
+      x0[i] = b0 ? q[lane] : 0.f;
+      x1[i] = b1 ? q[lane + 64] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = s0 + 4 * i < a.splits ? exp2_f(e[i] - ref) : 0.f;
+      ll += n[i] * f;
+      v0 += x0[i] * f;
+      v1 += x1[i] * f;
+    }
   }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  T* o = row_ptr((T*)a.out, a.os, b, hk, a.group, r);
-  if (lane < a.d) o[lane] = from_f32<Tr>(v0 * inv);
-  if (lane + 64 < a.d) o[lane + 64] = from_f32<Tr>(v1 * inv);
-  if (a.lse && lane == 0) {
+  sums[wave][lane] = v0;
+  sums[wave][lane + 64] = v1;
+  if (lane == 0) denom[wave] = ll;
+  __syncthreads();
+  ll = (denom[0] + denom[1]) + (denom[2] + denom[3]);
+  const int e = threadIdx.x;
+  if (e < a.d) {
+    const float v = (sums[0][e] + sums[1][e]) + (sums[2][e] + sums[3][e]);
+    row_ptr((T*)a.out, a.os, b, hk, a.group, r)[e] = from_f32<Tr>(ll == 0.f ? 0.f : v / ll);
+  }
+  if (a.lse && e == 0) {
     const int i = query_of(r, a.group);
     a.lse[((int64_t)(b * a.hk + hk) * a.group + (r - i * a.group)) * a.nq + i] = ll == 0.f ? -INFINITY : fmaf(mm, kLn2, logf(ll));
   }
@@ -798,30 +846,18 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(AttnArgs a, int row_blocks
 // ---- launch rules -----------------------------------------------------------------------------
 constexpr int kCUs = 256;
 inline int pad_d(int d) { return (d + 31) / 32 * 32; }
-// The few-rows kernel pads 96 to 128: it is bound by its loads, and rows of 12 chunks cost it more
-// lane masks than there are scalar registers
-inline int split_pad(int d) { return pad_d(d) == 96 ? 128 : pad_d(d); }
-
 // Two 16-wide tiles per wave (a fragment read from LDS serves both): 16-bit types, while the
 // workgroups still fill the chip
 inline bool two_tiles(int bytes, int64_t bh, int64_t n) { return bytes == 2 && bh * cdiv(n, 128) >= kCUs; }
-// Key ranges of the few-rows kernel; 0: the block kernel takes the call
-inline int split_count(int bytes, int64_t bh, int64_t rows, int64_t nk) {
+// Key ranges of the few-rows kernel; 0: the block kernel takes the call.  Two workgroups per CU, and
+// at least four slabs for each wave of one.
+inline int split_count(int64_t bh, int64_t rows, int64_t nk) {
   const int64_t wgs = bh * cdiv(rows, 64), items = bh * cdiv(rows, 16);
   if (rows > 32 && (wgs >= kCUs / 2 || nk < 512)) return 0;
-  int64_t s = cdiv(3 * kCUs, items);
-  const int64_t most = cdiv(nk, 4 * (128 / bytes));
+  int64_t s = cdiv(2 * kCUs, items);
+  const int64_t most = cdiv(nk, 512);
   if (s > most) s = most;
   return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
-}
-
-template <class Tr, int kDP>
-void run_split(const AttnArgs& a, hipStream_t st) {
-  const int64_t bh = (int64_t)a.b * a.hk;
-  const int rb = (int)cdiv(a.rows, 16);
-  hipLaunchKernelGGL((attn_split_kernel<Tr, kDP>), dim3((unsigned)(bh * rb), a.splits), dim3(256), 0, st, a, rb);
-  if (a.splits > 1)
-    hipLaunchKernelGGL(attn_join_kernel<Tr>, dim3((unsigned)(bh * a.rows)), dim3(64), 0, st, a, rb, kDP);
 }
 
 // What Feed's kAsync needs of one operand: chunks whole and on 16-byte boundaries, a block's offsets
@@ -832,6 +868,20 @@ inline bool feed_async(const char* p, const int64_t* st, int d, int group, int b
     if (st[i] * bytes % 16) return false;
   return (uintptr_t)p % 16 == 0 && d * bytes % 16 == 0 && bn % group == 0 && st[1] >= 0 && st[2] >= 0 &&
          (bn / group * st[1] + group * st[2]) * bytes < (int64_t(1) << 30);
+}
+
+template <class Tr, int kDP>
+void run_split(const AttnArgs& a, hipStream_t st) {
+  const int64_t bh = (int64_t)a.b * a.hk;
+  const int rb = (int)cdiv(a.rows, 16);
+  constexpr int kWaves = kDP * Tr::kBytes > 256 ? 2 : 4;  // (as many as have their slabs in 160 KB)
+  const dim3 grid((unsigned)(bh * rb), a.splits);
+  if (feed_async(a.k, a.ks, a.d, 1, Tr::kBytes) && feed_async(a.v, a.vs, a.d, 1, Tr::kBytes))
+    hipLaunchKernelGGL((attn_split_kernel<Tr, kDP, kWaves, true>), grid, dim3(64 * kWaves), 0, st, a, rb);
+  else
+    hipLaunchKernelGGL((attn_split_kernel<Tr, kDP, kWaves, false>), grid, dim3(64 * kWaves), 0, st, a, rb);
+  if (a.splits > 1)
+    hipLaunchKernelGGL(attn_join_kernel<Tr>, dim3((unsigned)(bh * a.rows)), dim3(256), 0, st, a, rb, kDP);
 }
 
 template <class Tr, int kDP, int kNT>
@@ -885,9 +935,10 @@ void run_bwd(const AttnArgs& a, hipStream_t st) {
 template <class Tr>
 void run_attn(const AttnArgs& a, bool bwd, hipStream_t st) {
   if (!bwd && a.splits) {
-    switch (split_pad(a.d)) {
+    switch (pad_d(a.d)) {
       case 32: run_split<Tr, 32>(a, st); break;
       case 64: run_split<Tr, 64>(a, st); break;
+      case 96: run_split<Tr, 96>(a, st); break;
       default: run_split<Tr, 128>(a, st); break;
     }
     return;
@@ -941,8 +992,8 @@ int yk_attention_workspace(const yk_attention_args* a, int64_t* bytes) {
   const int64_t bh = (int64_t)a->b * a->h_kv, rows = a->nq * (a->h_q / a->h_kv);
   *bytes = 0;
   if (bh == 0 || rows == 0) return YK_OK;
-  const int s = split_count(tok_bytes(a->dtype), bh, rows, a->nk);
-  if (s > 1) *bytes = bh * cdiv(rows, 16) * s * 16 * (split_pad(a->d) + 2) * 4;
+  const int s = split_count(bh, rows, a->nk);
+  if (s > 1) *bytes = bh * cdiv(rows, 16) * s * 16 * (pad_d(a->d) + 4) * 4;
   return YK_OK;
 }
 
@@ -959,7 +1010,7 @@ int yk_attention(yk_ctx* ctx, const yk_attention_args* a, void* stream) {
   AttnArgs k = common_args(a);
   k.out = (char*)a->o;
   k.lse = a->lse;
-  k.splits = split_count(tok_bytes(a->dtype), (int64_t)k.b * k.hk, k.rows, k.nk);
+  k.splits = split_count((int64_t)k.b * k.hk, k.rows, k.nk);
   if (k.splits > 1 && !a->ws) k.splits = 1;
   const hipStream_t st = (hipStream_t)stream;
   if (a->dtype == YK_ACT_F32) run_attn<F32>(k, false, st);
