@@ -178,13 +178,17 @@ struct Feed {
       const size_t b = (size_t)base;
       const size_t ub = ((size_t)(unsigned)rfl((int)(b >> 32)) << 32) | (unsigned)rfl((int)b);
       const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)ub, (short)0, 0x7ffffff0, 0x00020000);
-      const bool tail = first + Bl::kBN > limit;
-#pragma unroll
-      for (int i = 0; i < Bl::kN; ++i) {
-        unsigned o = off[i];
-        if (tail && first + (int)((i * 256 + threadIdx.x) / Bl::kRowChunks) >= limit) o = kOut;
+      auto one = [&](int i, unsigned o) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
             rsrc, (__attribute__((address_space(3))) void*)(lds + (i * 256 + rfl(threadIdx.x & ~63)) * 16), 16, o, 0, 0, 0);
+      };
+      if (first + Bl::kBN <= limit) {
+#pragma unroll
+        for (int i = 0; i < Bl::kN; ++i) one(i, off[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < Bl::kN; ++i)
+          one(i, first + (int)((i * 256 + threadIdx.x) / Bl::kRowChunks) < limit ? off[i] : kOut);
       }
     } else {
 #pragma unroll
@@ -264,42 +268,53 @@ __device__ __forceinline__ void store_out(typename Tr::T* p, int d0, int d, f32x
 }
 
 // One column's running softmax over a block of kT score tiles: raw scores in st, p comes back in
-// it, keys beyond `lim` left out (mask: some lane has any).  m is the reference of the column's
-// exponents, in score * scale * log2 e: not the running maximum itself but at most kLag below
-// it, so that most blocks need neither the other lanes' maxima nor a rescaling (p then reaches 2^kLag,
-// which costs no accuracy).  l: this lane's share of the denominator, from p as it is before any
-// rounding.  rescale(f): what else was accumulated so far times f.
-constexpr float kLag = 8.f;
+// it, keys beyond `lim` left out.  m is the reference of the column's exponents, in score * scale *
+// log2 e: a maximum seen so far, renewed only when a lane's p add up to more than 2^8 under it.
+// Most blocks then need no maximum at all, neither a lane's nor the other lanes', and no rescaling;
+// that p may exceed 1 costs no accuracy (fp16 holds 2^15).  l: this lane's share of the denominator,
+// from p as it is before any rounding.  rescale(f): what else was accumulated so far times f.
+constexpr float kRenew = 256.f;
 template <int kT, class R>
-__device__ __forceinline__ void softmax_step(f32x4* st, int key0, int lim, bool mask, float sl2, float& m, float& l, R&& rescale) {
-  const int g = (threadIdx.x & 63) >> 4;
-  if (mask) {
+__device__ __forceinline__ void softmax_step(f32x4* st, int key0, int lim, float sl2, float& m, float& l, R&& rescale) {
+  const int left = lim - key0 - ((threadIdx.x & 63) >> 4) * 4;  // this lane's keys t * 16 + i below it are seen
+  if (__any(lim < key0 + kT * 16)) {
 #pragma unroll
     for (int t = 0; t < kT; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) st[t][i] = key0 + t * 16 + g * 4 + i < lim ? st[t][i] : -INFINITY;
+      for (int i = 0; i < 4; ++i) st[t][i] = t * 16 + i < left ? st[t][i] : -INFINITY;
   }
-  float mx = -INFINITY;
+  f32x4 p[kT];
+  auto exps = [&](float ref) {
+    float sum = 0.f;
 #pragma unroll
-  for (int t = 0; t < kT; ++t) mx = fmaxf(fmaxf(fmaxf(mx, st[t][0]), fmaxf(st[t][1], st[t][2])), st[t][3]);
-  mx *= sl2;
-  if (__any(mx > m + kLag)) {
+    for (int t = 0; t < kT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[t][i] = exp2_f(fmaf(st[t][i], sl2, -ref));
+        sum += p[t][i];
+      }
+    return sum;
+  };
+  // (nothing seen yet: m is -infinity, and every p of a column that sees nothing here exp2(-inf) = 0)
+  float sum = exps(m == -INFINITY ? 0.f : m);
+  if (__any(sum > kRenew || (m == -INFINITY && lim > key0))) {
+    float mx = st[0][0];
+#pragma unroll
+    for (int t = 0; t < kT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, st[t][i]);
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float mn = fmaxf(m, mx);
-    const float f = exp2_f(m - (mn == -INFINITY ? 0.f : mn));
+    const float mn = fmaxf(m, mx * sl2), ref = mn == -INFINITY ? 0.f : mn;
+    const float f = exp2_f(m - ref);
     l *= f;
     rescale(f);
     m = mn;
+    sum = exps(ref);
   }
-  const float ref = m == -INFINITY ? 0.f : m;  // nothing seen yet: every p is exp2(-inf) = 0
+  l += sum;
 #pragma unroll
-  for (int t = 0; t < kT; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      st[t][i] = exp2_f(fmaf(st[t][i], sl2, -ref));
-      l += st[t][i];
-    }
+  for (int t = 0; t < kT; ++t) st[t] = p[t];
 }
 
 // A column's sum over the lanes that share it.
@@ -307,6 +322,12 @@ __device__ __forceinline__ float column_sum(float v) {
   v += __shfl_xor(v, 16, 64);
   return v + __shfl_xor(v, 32, 64);
 }
+
+// Two waves per SIMD for the 16-bit types: with 256 registers a wave the compiler keeps the MFMA's
+// results where the vector instructions read them, with more it moves them there and back (a third of
+// the forward kernel's instructions).
+template <class Tr>
+constexpr int kWavesPerSimd = Tr::kBytes == 2 ? 2 : 1;
 
 // Keys that a block of rows [r0, r0 + n) sees: its last row in use sees most.
 __device__ __forceinline__ int key_end(const AttnArgs& a, const Seq& s, int r0, int n) {
@@ -319,7 +340,7 @@ __device__ __forceinline__ int key_end(const AttnArgs& a, const Seq& s, int r0, 
 
 // Forward: 4 waves of 16 kNT rows.
 template <class Tr, int kDP, int kNT, bool kAsync>
-__global__ __launch_bounds__(256) void attn_kernel(AttnArgs a, int row_blocks) {
+__global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_kernel(AttnArgs a, int row_blocks) {
   using T = typename Tr::T;
   using V8 = typename Tr::V8;
   using Bl = Block<Tr, kDP>;
@@ -369,7 +390,7 @@ __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a, int row_blocks) {
     V8 pf[kNT][kKT / 2];
 #pragma unroll
     for (int j = 0; j < kNT; ++j) {
-      softmax_step<kKT>(st[j], k0, lim[j], __any(lim[j] < k0 + Bl::kBN), sl2, m[j], l[j], [&](float f) {
+      softmax_step<kKT>(st[j], k0, lim[j], sl2, m[j], l[j], [&](float f) {
 #pragma unroll
         for (int t = 0; t < kDT; ++t) acc[j][t] *= f;
       });
@@ -497,7 +518,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_split_kernel(AttnArgs a, int
       for (int c = 0; c < kS; ++c) st[t] = mma<Tr>(Bl::row_frag(lk, t, c, lane), qf[c], st[t]);
     }
     const int lim2 = lim < k_end ? lim : k_end;
-    softmax_step<2>(st, k0, lim2, __any(lim2 < k0 + kKeys), sl2, m, l, [&](float f) {
+    softmax_step<2>(st, k0, lim2, sl2, m, l, [&](float f) {
 #pragma unroll
       for (int t = 0; t < kDT; ++t) acc[t] *= f;
     });
@@ -628,7 +649,7 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs a) {
 
 // dk and dv: 4 waves of 16 kNT keys, blocks of packed rows (q, do and their statistics) through LDS.
 template <class Tr, int kDP, int kNT, bool kAsync>
-__global__ __launch_bounds__(256) void attn_dkv_kernel(AttnArgs a, int key_blocks) {
+__global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_dkv_kernel(AttnArgs a, int key_blocks) {
   using T = typename Tr::T;
   using V8 = typename Tr::V8;
   using Bl = Block<Tr, kDP>;
@@ -708,10 +729,16 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(AttnArgs a, int key_block
 #pragma unroll
           for (int i = 0; i < 4; ++i) p[j][h][i] = exp2_f(fmaf(p[j][h][i], sl2, -ls[i]));
           if (mask) {
-            const int key = key0 + (wave * kNT + j) * 16 + l16;
+            const int sees = key0 + (wave * kNT + j) * 16 + l16 - s.off;  // the first query that sees this key
+            if (a.group == 1) {
+              const int skip = sees - r0 - g * 4;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (key > query_of(r0 + t * 16 + g * 4 + i, a.group) + s.off) p[j][h][i] = 0.f;
+              for (int i = 0; i < 4; ++i) p[j][h][i] = t * 16 + i < skip ? 0.f : p[j][h][i];
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (query_of(r0 + t * 16 + g * 4 + i, a.group) < sees) p[j][h][i] = 0.f;
+            }
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) ds[j][h][i] = p[j][h][i] * (ds[j][h][i] - dl[i]);
@@ -752,7 +779,7 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(AttnArgs a, int key_block
 
 // dq: 4 waves of 16 kNT rows, key blocks (k, v) through LDS.
 template <class Tr, int kDP, int kNT, bool kAsync>
-__global__ __launch_bounds__(256) void attn_dq_kernel(AttnArgs a, int row_blocks) {
+__global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_dq_kernel(AttnArgs a, int row_blocks) {
   using T = typename Tr::T;
   using V8 = typename Tr::V8;
   using Bl = Block<Tr, kDP>;
@@ -812,9 +839,9 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(AttnArgs a, int row_blocks
 #pragma unroll
           for (int i = 0; i < 4; ++i) p[j][h][i] = exp2_f(fmaf(p[j][h][i], sl2, -ls[j]));
           if (__any(lim[j] < k0 + Bl::kBN)) {
+            const int left = lim[j] - k0 - g * 4;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (k0 + t * 16 + g * 4 + i >= lim[j]) p[j][h][i] = 0.f;
+            for (int i = 0; i < 4; ++i) p[j][h][i] = t * 16 + i < left ? p[j][h][i] : 0.f;
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) ds[j][h][i] = p[j][h][i] * (ds[j][h][i] - dl[j]);
@@ -846,9 +873,9 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(AttnArgs a, int row_blocks
 // ---- launch rules -----------------------------------------------------------------------------
 constexpr int kCUs = 256;
 inline int pad_d(int d) { return (d + 31) / 32 * 32; }
-// Two 16-wide tiles per wave (a fragment read from LDS serves both): 16-bit types, while the
-// workgroups still fill the chip
-inline bool two_tiles(int bytes, int64_t bh, int64_t n) { return bytes == 2 && bh * cdiv(n, 128) >= kCUs; }
+// Two 16-wide tiles per wave (a fragment read from LDS serves both) where they fit the registers:
+// 16-bit heads of up to 64, while the workgroups still fill the chip
+inline bool two_tiles(int64_t bh, int64_t n) { return bh * cdiv(n, 128) >= kCUs; }
 // Key ranges of the few-rows kernel; 0: the block kernel takes the call.  Two workgroups per CU, and
 // at least four slabs for each wave of one.
 inline int split_count(int64_t bh, int64_t rows, int64_t nk) {
@@ -884,35 +911,29 @@ void run_split(const AttnArgs& a, hipStream_t st) {
     hipLaunchKernelGGL(attn_join_kernel<Tr>, dim3((unsigned)(bh * a.rows)), dim3(256), 0, st, a, rb, kDP);
 }
 
-template <class Tr, int kDP, int kNT>
-void launch_fwd(const AttnArgs& a, bool async, hipStream_t st) {
+template <class Tr, int kDP, int kNT, bool kAsync = true>
+void launch_fwd(const AttnArgs& a, hipStream_t st) {
   const int rb = (int)cdiv(a.rows, 64 * kNT);
-  const dim3 grid((unsigned)((int64_t)a.b * a.hk * rb));
-  if (async) hipLaunchKernelGGL((attn_kernel<Tr, kDP, kNT, true>), grid, dim3(256), 0, st, a, rb);
-  else hipLaunchKernelGGL((attn_kernel<Tr, kDP, kNT, false>), grid, dim3(256), 0, st, a, rb);
+  hipLaunchKernelGGL((attn_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * rb)), dim3(256), 0, st, a, rb);
 }
-template <class Tr, int kDP, int kNT>
-void launch_dkv(const AttnArgs& a, bool async, hipStream_t st) {
+template <class Tr, int kDP, int kNT, bool kAsync = true>
+void launch_dkv(const AttnArgs& a, hipStream_t st) {
   const int kb = (int)cdiv(a.nk, 64 * kNT);
-  const dim3 grid((unsigned)((int64_t)a.b * a.hk * kb));
-  if (async) hipLaunchKernelGGL((attn_dkv_kernel<Tr, kDP, kNT, true>), grid, dim3(256), 0, st, a, kb);
-  else hipLaunchKernelGGL((attn_dkv_kernel<Tr, kDP, kNT, false>), grid, dim3(256), 0, st, a, kb);
+  hipLaunchKernelGGL((attn_dkv_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * kb)), dim3(256), 0, st, a, kb);
 }
-template <class Tr, int kDP, int kNT>
-void launch_dq(const AttnArgs& a, bool async, hipStream_t st) {
+template <class Tr, int kDP, int kNT, bool kAsync = true>
+void launch_dq(const AttnArgs& a, hipStream_t st) {
   const int rb = (int)cdiv(a.rows, 64 * kNT);
-  const dim3 grid((unsigned)((int64_t)a.b * a.hk * rb));
-  if (async) hipLaunchKernelGGL((attn_dq_kernel<Tr, kDP, kNT, true>), grid, dim3(256), 0, st, a, rb);
-  else hipLaunchKernelGGL((attn_dq_kernel<Tr, kDP, kNT, false>), grid, dim3(256), 0, st, a, rb);
+  hipLaunchKernelGGL((attn_dq_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * rb)), dim3(256), 0, st, a, rb);
 }
 
 template <class Tr, int kDP>
 void run_fwd(const AttnArgs& a, hipStream_t st) {
-  const bool async = feed_async(a.k, a.ks, a.d, 1, Tr::kBytes) && feed_async(a.v, a.vs, a.d, 1, Tr::kBytes);
-  if constexpr (Tr::kBytes == 2) {
-    if (two_tiles(Tr::kBytes, (int64_t)a.b * a.hk, a.rows)) return launch_fwd<Tr, kDP, 2>(a, async, st);
-  }
-  launch_fwd<Tr, kDP, 1>(a, async, st);
+  constexpr int kTwo = Tr::kBytes == 2 && kDP <= 64 ? 2 : 1;
+  const int64_t bh = (int64_t)a.b * a.hk;
+  if (!feed_async(a.k, a.ks, a.d, 1, Tr::kBytes) || !feed_async(a.v, a.vs, a.d, 1, Tr::kBytes)) launch_fwd<Tr, kDP, 1, false>(a, st);
+  else if (two_tiles(bh, a.rows)) launch_fwd<Tr, kDP, kTwo>(a, st);
+  else launch_fwd<Tr, kDP, 1>(a, st);
 }
 
 template <class Tr, int kDP>
@@ -921,15 +942,13 @@ void run_bwd(const AttnArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(attn_delta_kernel<Tr>, dim3((unsigned)cdiv(bh * a.rows, 16)), dim3(256), 0, st, a);
   const bool rows = feed_async(a.q, a.qs, a.d, a.group, Tr::kBytes) && feed_async(a.go, a.gos, a.d, a.group, Tr::kBytes);
   const bool keys = feed_async(a.k, a.ks, a.d, 1, Tr::kBytes) && feed_async(a.v, a.vs, a.d, 1, Tr::kBytes);
-  if constexpr (Tr::kBytes == 2) {
-    if (kDP <= 64 && two_tiles(Tr::kBytes, bh, a.nk)) launch_dkv<Tr, kDP, kDP <= 64 ? 2 : 1>(a, rows, st);
-    else launch_dkv<Tr, kDP, 1>(a, rows, st);
-    if (two_tiles(Tr::kBytes, bh, a.rows)) launch_dq<Tr, kDP, 2>(a, keys, st);
-    else launch_dq<Tr, kDP, 1>(a, keys, st);
-  } else {
-    launch_dkv<Tr, kDP, 1>(a, rows, st);
-    launch_dq<Tr, kDP, 1>(a, keys, st);
-  }
+  constexpr int kTwo = Tr::kBytes == 2 && kDP <= 64 ? 2 : 1;
+  if (!rows) launch_dkv<Tr, kDP, 1, false>(a, st);
+  else if (two_tiles(bh, a.nk)) launch_dkv<Tr, kDP, kTwo>(a, st);
+  else launch_dkv<Tr, kDP, 1>(a, st);
+  if (!keys) launch_dq<Tr, kDP, 1, false>(a, st);
+  else if (two_tiles(bh, a.rows)) launch_dq<Tr, kDP, kTwo>(a, st);
+  else launch_dq<Tr, kDP, 1>(a, st);
 }
 
 template <class Tr>
