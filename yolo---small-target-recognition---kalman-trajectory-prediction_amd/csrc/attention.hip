@@ -874,7 +874,9 @@ __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_dq_kernel(AttnArg
 constexpr int kCUs = 256;
 inline int pad_d(int d) { return (d + 31) / 32 * 32; }
 // Two 16-wide tiles per wave (a fragment read from LDS serves both) where they fit the registers:
-// 16-bit heads of up to 64, while the workgroups still fill the chip
+// 16-bit heads, while the workgroups still fill the chip.  dk and dv (two sets of sums): at d = 96
+// only, 775 against 1018 us for 4 x 4096 x 16 heads; up to 64 one tile is as fast, and faster where
+// rows are causal or few (8 x 1280 x 8 heads of 40: 72 against 80), at 128 two do not fit
 inline bool two_tiles(int64_t bh, int64_t n) { return bh * cdiv(n, 128) >= kCUs; }
 // Key ranges of the few-rows kernel; 0: the block kernel takes the call.  Two workgroups per CU, and
 // at least four slabs for each wave of one.
@@ -929,7 +931,7 @@ void launch_dq(const AttnArgs& a, hipStream_t st) {
 
 template <class Tr, int kDP>
 void run_fwd(const AttnArgs& a, hipStream_t st) {
-  constexpr int kTwo = Tr::kBytes == 2 && kDP <= 64 ? 2 : 1;
+  constexpr int kTwo = Tr::kBytes == 2 ? 2 : 1;
   const int64_t bh = (int64_t)a.b * a.hk;
   if (!feed_async(a.k, a.ks, a.d, 1, Tr::kBytes) || !feed_async(a.v, a.vs, a.d, 1, Tr::kBytes)) launch_fwd<Tr, kDP, 1, false>(a, st);
   else if (two_tiles(bh, a.rows)) launch_fwd<Tr, kDP, kTwo>(a, st);
@@ -942,9 +944,9 @@ void run_bwd(const AttnArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(attn_delta_kernel<Tr>, dim3((unsigned)cdiv(bh * a.rows, 16)), dim3(256), 0, st, a);
   const bool rows = feed_async(a.q, a.qs, a.d, a.group, Tr::kBytes) && feed_async(a.go, a.gos, a.d, a.group, Tr::kBytes);
   const bool keys = feed_async(a.k, a.ks, a.d, 1, Tr::kBytes) && feed_async(a.v, a.vs, a.d, 1, Tr::kBytes);
-  constexpr int kTwo = Tr::kBytes == 2 && kDP <= 64 ? 2 : 1;
+  constexpr int kTwo = Tr::kBytes == 2 ? 2 : 1, kTwoKeys = kDP == 96 ? kTwo : 1;
   if (!rows) launch_dkv<Tr, kDP, 1, false>(a, st);
-  else if (two_tiles(bh, a.nk)) launch_dkv<Tr, kDP, kTwo>(a, st);
+  else if (two_tiles(bh, a.nk)) launch_dkv<Tr, kDP, kTwoKeys>(a, st);
   else launch_dkv<Tr, kDP, 1>(a, st);
   if (!keys) launch_dq<Tr, kDP, 1, false>(a, st);
   else if (two_tiles(bh, a.rows)) launch_dq<Tr, kDP, kTwo>(a, st);

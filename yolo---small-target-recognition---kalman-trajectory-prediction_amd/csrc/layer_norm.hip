@@ -39,16 +39,30 @@ struct NormGradArgs {
   int c, param_f32, dtype;
 };
 
-// Sum over the NT lanes of a row, in every one of them.  256: through one LDS word per wave.
+// v of the lane n places round the row of 16 lanes
+template <int kN>
+__device__ __forceinline__ float rotate16(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + kN, 0xf, 0xf, true));
+}
+// Sum over the NT lanes of a row, in every one of them: rotations within 16 lanes (vector speed),
+// then across them, for more than a wave through one LDS word per wave.
 template <int NT>
 __device__ __forceinline__ float row_sum(float v, float* red) {
-#pragma unroll
-  for (int s = 1; s < (NT < 64 ? NT : 64); s <<= 1) v += __shfl_xor(v, s, 64);
-  if constexpr (NT == 256) {
+  v += rotate16<8>(v);
+  v += rotate16<4>(v);
+  v += rotate16<2>(v);
+  v += rotate16<1>(v);
+  if constexpr (NT >= 64) {
+    v += __shfl_xor(v, 16, 64);
+    v += __shfl_xor(v, 32, 64);
+  }
+  if constexpr (NT > 64) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = (red[0] + red[1]) + (red[2] + red[3]);
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) v += red[i];
   }
   return v;
 }
@@ -193,9 +207,9 @@ __global__ __launch_bounds__(256) void norm_wide_kernel(NormArgs a) {
 }
 
 template <class Tr, int NT, int NV>
-__global__ __launch_bounds__(256) void norm_grad_kernel(NormGradArgs a) {
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_grad_kernel(NormGradArgs a) {
   using T = typename Tr::T;
-  constexpr int kEpc = 16 / Tr::kBytes, kRows = 256 / NT;
+  constexpr int kEpc = 16 / Tr::kBytes, kRows = NT < 256 ? 256 / NT : 1;
   extern __shared__ float lds[];  // [kRows][c] while the column sums meet; row_sum's words
   const int lane = threadIdx.x % NT, sub = threadIdx.x / NT;
   u32x4 w[NV];  // dtype, or unused with float32 parameters next to 16-bit rows
@@ -210,20 +224,28 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormGradArgs a) {
   }
   const float inv = 1.f / (float)a.c;
   const int64_t step = (int64_t)gridDim.x * kRows;
-  for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.m; row0 += step) {
-    const int64_t row = row0 + sub;
+  u32x4 xn[NV], gn[NV];  // the next row, on its way while one is worked on
+  float mean_n = 0.f, rstd_n = 0.f;
+  auto fetch = [&](int64_t row) {
     const bool live = row < a.m;
     const int64_t r = live ? row : a.m - 1;
     const T* x = (const T*)a.x + r * a.x_stride;
     const T* dy = (const T*)a.dy + r * a.dy_stride;
-    u32x4 xr[NV], gr[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c0 = (i * NT + lane) * kEpc;
-      xr[i] = load16<Tr>(x + c0, a.c - c0);
-      gr[i] = load16<Tr>(dy + c0, live ? a.c - c0 : 0);
+      xn[i] = load16<Tr>(x + c0, a.c - c0);
+      gn[i] = load16<Tr>(dy + c0, live ? a.c - c0 : 0);
     }
-    const float mean = a.mean[r], rstd = a.rstd[r];
+    mean_n = a.mean[r];
+    rstd_n = a.rstd[r];
+  };
+  fetch((int64_t)blockIdx.x * kRows + sub);
+  for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.m; row0 += step) {
+    const int64_t row = row0 + sub;
+    const bool live = row < a.m;
+    const float rstd = rstd_n, shift = -mean_n * rstd;
+    float h[NV * kEpc], g[NV * kEpc];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -231,14 +253,17 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormGradArgs a) {
       if (!own_w) params<Tr>(a.w, (i * NT + lane) * kEpc, a.c, a.param_f32, a.dtype, 1.f, wf);
 #pragma unroll
       for (int e = 0; e < kEpc; ++e) {
-        const float d = elem<Tr>(gr[i], e), h = (elem<Tr>(xr[i], e) - mean) * rstd;
-        const float g = d * (own_w ? elem<Tr>(w[i], e) : wf[e]);
-        s1 += g;
-        s2 += g * h;
-        aw[i * kEpc + e] += d * h;
-        ab[i * kEpc + e] += d;
+        const int k = i * kEpc + e;
+        const float d = elem<Tr>(gn[i], e);
+        h[k] = fmaf(elem<Tr>(xn[i], e), rstd, shift);
+        g[k] = d * (own_w ? elem<Tr>(w[i], e) : wf[e]);
+        s1 += g[k];
+        s2 = fmaf(g[k], h[k], s2);
+        aw[k] = fmaf(d, h[k], aw[k]);
+        ab[k] += d;
       }
     }
+    if (row0 + step < a.m) fetch(row + step);
     if (a.dx) {
       s1 = row_sum<NT>(s1, lds) * inv;
       s2 = row_sum<NT>(s2, lds) * inv;
@@ -248,14 +273,9 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormGradArgs a) {
         for (int i = 0; i < NV; ++i) {
           const int c0 = (i * NT + lane) * kEpc;
           if (c0 >= a.c) break;
-          float wf[kEpc], v[kEpc];
-          if (!own_w) params<Tr>(a.w, c0, a.c, a.param_f32, a.dtype, 1.f, wf);
+          float v[kEpc];
 #pragma unroll
-          for (int e = 0; e < kEpc; ++e) {
-            const float h = (elem<Tr>(xr[i], e) - mean) * rstd;
-            const float g = elem<Tr>(gr[i], e) * (own_w ? elem<Tr>(w[i], e) : wf[e]);
-            v[e] = rstd * (g - s1 - h * s2);
-          }
+          for (int e = 0; e < kEpc; ++e) v[e] = rstd * fmaf(-h[i * kEpc + e], s2, g[i * kEpc + e] - s1);
           store16<Tr>(dx + c0, v, a.c - c0);
         }
       }
@@ -268,9 +288,10 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormGradArgs a) {
     const float* acc = which ? ab : aw;
     if constexpr (kRows == 1) {
 #pragma unroll
-      for (int i = 0; i < NV * kEpc; ++i) {
-        const int c = (i / kEpc * NT + lane) * kEpc + i % kEpc;
-        if (c < a.c) out[c] = acc[i];
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * NT + lane) * kEpc;
+#pragma unroll
+        for (int e = 0; e < kEpc; e += 4) store16<F32>(out + c + e, acc + i * kEpc + e, a.c - c - e);
       }
     } else {
       __syncthreads();
@@ -360,32 +381,52 @@ __global__ __launch_bounds__(256) void norm_cols_kernel(NormGradArgs a) {
   }
 }
 
-// dw / db from the workgroups' rows: 64 columns x 16 row groups, each group's rows in order.
+// dw / db from the workgroups' rows: 32 columns x 32 ranges of rows, 8 loads in flight each, all
+// added in a fixed order.
 __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* part, int n_part, int c, void* dw, void* db,
                                                            int param_f32, int dtype) {
-  __shared__ float lds[16][64];
-  const int lane = threadIdx.x & 63, g = threadIdx.x >> 6, col = blockIdx.x * 64 + lane, which = blockIdx.y;
+  __shared__ float lds[32][33];
+  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, col = blockIdx.x * 32 + lane, which = blockIdx.y;
   void* out = which ? db : dw;
   if (!out) return;
   float s = 0.f;
-  if (col < c)
-    for (int r = g; r < n_part; r += 16) s += part[((int64_t)r * 2 + which) * c + col];
+  if (col < c) {
+    const float* p = part + (int64_t)which * c + col;
+    for (int r0 = g; r0 < n_part; r0 += 256) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = r0 + 32 * i < n_part ? p[(int64_t)(r0 + 32 * i) * 2 * c] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[i];
+    }
+  }
   lds[g][lane] = s;
   __syncthreads();
   if (g == 0 && col < c) {
     float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v += lds[i][lane];
+    for (int i = 0; i < 32; ++i) v += lds[i][lane];
     store_param(out, col, v, param_f32, dtype);
   }
 }
 
 constexpr int kMaxChunks = 4 * 256;       // a row in the registers of a workgroup
-constexpr int kGradGroups = 512;          // workgroups (and rows of partial sums) of the backward pass
+constexpr int kGradGroups = 1024;         // workgroups (and rows of partial sums) of the backward pass
+
+constexpr int kNarrowRows = 8192;
 
 template <class Tr, int NT>
 void launch_norm(const NormArgs& a, int nv, hipStream_t st) {
   const dim3 grid((unsigned)cdiv(a.m, 256 / NT));
+  if constexpr (NT == 16) {
+    switch (nv) {
+      case 5: hipLaunchKernelGGL((norm_kernel<Tr, NT, 5>), grid, dim3(256), 0, st, a); return;
+      case 6: hipLaunchKernelGGL((norm_kernel<Tr, NT, 6>), grid, dim3(256), 0, st, a); return;
+      case 7: hipLaunchKernelGGL((norm_kernel<Tr, NT, 7>), grid, dim3(256), 0, st, a); return;
+      case 8: hipLaunchKernelGGL((norm_kernel<Tr, NT, 8>), grid, dim3(256), 0, st, a); return;
+      default: break;
+    }
+  }
   switch (nv) {
     case 1: hipLaunchKernelGGL((norm_kernel<Tr, NT, 1>), grid, dim3(256), 0, st, a); break;
     case 2: hipLaunchKernelGGL((norm_kernel<Tr, NT, 2>), grid, dim3(256), 0, st, a); break;
@@ -396,7 +437,8 @@ void launch_norm(const NormArgs& a, int nv, hipStream_t st) {
 template <class Tr>
 void run_norm(const NormArgs& a, hipStream_t st) {
   const int chunks = (int)cdiv(a.c, 16 / Tr::kBytes);
-  if (chunks <= 4 * 16) launch_norm<Tr, 16>(a, (int)cdiv(chunks, 16), st);
+  // 16 lanes a row while that fills the chip (wider rows then use every lane); else a wave, a workgroup
+  if (chunks <= 16 || (chunks <= 8 * 16 && a.m >= kNarrowRows)) launch_norm<Tr, 16>(a, (int)cdiv(chunks, 16), st);
   else if (chunks <= 4 * 64) launch_norm<Tr, 64>(a, (int)cdiv(chunks, 64), st);
   else if (chunks <= kMaxChunks) launch_norm<Tr, 256>(a, (int)cdiv(chunks, 256), st);
   else hipLaunchKernelGGL(norm_wide_kernel<Tr>, dim3((unsigned)a.m), dim3(256), 0, st, a);
@@ -404,20 +446,20 @@ void run_norm(const NormArgs& a, hipStream_t st) {
 
 template <class Tr, int NT>
 void launch_norm_grad(const NormGradArgs& a, int nv, int groups, hipStream_t st) {
-  const size_t lds = NT == 256 ? 16 : (size_t)(256 / NT) * a.c * 4;
-  switch (nv) {
-    case 1: hipLaunchKernelGGL((norm_grad_kernel<Tr, NT, 1>), dim3(groups), dim3(256), lds, st, a); break;
-    case 2: hipLaunchKernelGGL((norm_grad_kernel<Tr, NT, 2>), dim3(groups), dim3(256), lds, st, a); break;
-    case 3: hipLaunchKernelGGL((norm_grad_kernel<Tr, NT, 3>), dim3(groups), dim3(256), lds, st, a); break;
-    default: hipLaunchKernelGGL((norm_grad_kernel<Tr, NT, 4>), dim3(groups), dim3(256), lds, st, a); break;
-  }
+  const size_t lds = NT >= 256 ? NT / 64 * 4 : (size_t)(256 / NT) * a.c * 4;
+  const dim3 block(NT < 256 ? 256 : NT);
+  if (nv == 1) hipLaunchKernelGGL((norm_grad_kernel<Tr, NT, 1>), dim3(groups), block, lds, st, a);
+  else hipLaunchKernelGGL((norm_grad_kernel<Tr, NT, 2>), dim3(groups), block, lds, st, a);
 }
-// lanes per row of the backward pass: 16 chunks x 1 while a row has so few, a wave, a workgroup
-inline int grad_lanes(int chunks) { return chunks <= 16 ? 16 : chunks <= 256 ? 64 : 256; }
+// Lanes per row of the backward pass: at most two chunks each, whose sums, row and next row are some
+// 150 registers (four took 270, one wave per SIMD: 10000 x 8192 bf16 187 us)
+inline int grad_lanes(int chunks) { return chunks <= 16 ? 16 : chunks <= 128 ? 64 : chunks <= 512 ? 256 : 512; }
+// Workgroups: enough for the chip, several rows each so that their sums are not most of the traffic
 inline int grad_groups(int64_t m, int c, int bytes) {
   const int nt = grad_lanes((int)cdiv(c, 16 / bytes));
-  const int64_t rows = cdiv(m, 256 / nt);
-  return (int)(rows < kGradGroups ? rows : kGradGroups);
+  const int64_t turns = cdiv(m, nt < 256 ? 256 / nt : 1);
+  const int64_t g = turns / 4 < 128 ? 128 : turns / 4;
+  return (int)(turns < g ? turns : g > kGradGroups ? kGradGroups : g);
 }
 template <class Tr>
 void run_norm_grad(const NormGradArgs& a, hipStream_t st) {
@@ -432,7 +474,8 @@ void run_norm_grad(const NormGradArgs& a, hipStream_t st) {
   switch (grad_lanes(chunks)) {
     case 16: launch_norm_grad<Tr, 16>(a, 1, groups, st); break;
     case 64: launch_norm_grad<Tr, 64>(a, (int)cdiv(chunks, 64), groups, st); break;
-    default: launch_norm_grad<Tr, 256>(a, (int)cdiv(chunks, 256), groups, st); break;
+    case 256: launch_norm_grad<Tr, 256>(a, (int)cdiv(chunks, 256), groups, st); break;
+    default: launch_norm_grad<Tr, 512>(a, (int)cdiv(chunks, 512), groups, st); break;
   }
 }
 
@@ -497,7 +540,7 @@ int yk_layer_norm_backward(yk_ctx* ctx, const yk_layer_norm_grad_args* a, void* 
     else run_norm_grad<H16>(k, st);
   }
   if (cols)
-    hipLaunchKernelGGL(norm_reduce_kernel, dim3((unsigned)cdiv(a->c, 64), 2), dim3(1024), 0, st, (const float*)a->ws,
+    hipLaunchKernelGGL(norm_reduce_kernel, dim3((unsigned)cdiv(a->c, 32), 2), dim3(1024), 0, st, (const float*)a->ws,
                        grad_groups(a->m, (int)a->c, tok_bytes(a->dtype)), (int)a->c, a->dw, a->db, f32, a->dtype);
   return launched("yk_layer_norm_backward");
 }

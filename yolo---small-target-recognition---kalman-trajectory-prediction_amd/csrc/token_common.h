@@ -132,15 +132,17 @@ __device__ __forceinline__ void add8(const typename Tr::T* p, float* v) {
 template <class Tr>
 __device__ __forceinline__ u32x4 load16(const typename Tr::T* p, int n) {
   constexpr int kEpc = 16 / Tr::kBytes;
-  if (n >= kEpc) return *(const u32x4_any*)p;
-  typename Tr::T t[kEpc];
+  u32x4 u{0, 0, 0, 0};
+  if (n >= kEpc) {
+    u = *(const u32x4_any*)p;
+  } else if (n > 0) {
+    typename Tr::T t[kEpc];
 #pragma unroll
-  for (int e = 0; e < kEpc; ++e) t[e] = e < n ? p[e] : (typename Tr::T)0;
-  u32x4 u;
-  __builtin_memcpy(&u, t, 16);
+    for (int e = 0; e < kEpc; ++e) t[e] = e < n ? p[e] : (typename Tr::T)0;
+    __builtin_memcpy(&u, t, 16);
+  }
   return u;
 }
-
 // The same of a row that may not be there (`ok`), without branches: what is not to be read is
 // loaded from `safe` (an element, or with `whole` 16 bytes, that exist) and replaced by zero.
 // whole: n is a multiple of the chunk, so a chunk is there or not.
