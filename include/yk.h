@@ -411,7 +411,14 @@ enum yk_op_kind {
   YK_K_CONV_INPUT = 0, /* first conv, reads uint8 BGR frames (fused letterbox/RGB//255)    */
   YK_K_CONV = 1,       /* implicit-GEMM conv (+bias, SiLU, residual, concat/upsample read)   */
   YK_K_SPPF_POOL = 2,  /* SPPF's three chained 5x5 max-pools, written as concat slices     */
-  YK_K_DETECT = 3      /* Detect level: box/cls 1x1 + DFL + dist2bbox + sigmoid + threshold  */
+  YK_K_DETECT = 3,     /* Detect level: box/cls 1x1 + DFL + dist2bbox + sigmoid + threshold  */
+  /* a transformer layer over the pixels of one map (bf16, f32 and f16 programs): */
+  YK_K_LINEAR = 4,     /* yk_linear on every pixel's channels: w_off [cout][src_ch] in the activation
+                        * type, b_off f32 [cout], act = yk_token_act; has_res 1: res is added,
+                        * 2: a table [out_h * out_w][cout] in the activation type at t_off         */
+  YK_K_LAYER_NORM = 5, /* yk_layer_norm, eps 1e-5: w_off / b_off f32 [cout]                        */
+  YK_K_ATTENTION = 6   /* yk_attention of an image's pixels: src is [q | k | v] of cout channels
+                        * each, ksize heads, scale (cout / ksize)^-0.5                             */
 };
 
 typedef struct {
@@ -424,7 +431,7 @@ typedef struct {
 
 typedef struct {
   int32_t kind;
-  int32_t ksize, stride, act; /* act: 0 none, 1 SiLU                                   */
+  int32_t ksize, stride, act; /* act: 0 none, 1 SiLU (YK_K_LINEAR: yk_token_act)        */
   int32_t n_src;
   yk_view src[2];
   int32_t src_ch[2];          /* physical channels of each source (multiples of 8; FP8 16) */

@@ -8,7 +8,8 @@ SPPF block.py:216-238, Detect head.py:26-209 with legacy=True for v8 models).
 The topology table below encodes ultralytics/cfg/models/v8/yolov8-small.yaml (the
 reference's custom 4-scale model with the extra P2 output).  A user YAML with the same
 module vocabulary (Conv, C2f, SPPF, nn.Upsample, Concat, Detect) is parsed the same way,
-so the standard 3-scale yolov8.yaml works too.
+so the standard 3-scale yolov8.yaml works too.  ``AIFI`` ([hidden, heads]) is a post-norm transformer
+layer over the cells of its input map, with 2-D sine-cosine positions on the queries and keys.
 """
 from __future__ import annotations
 
@@ -94,7 +95,7 @@ def load_model_dict(path: str) -> dict:
 class Layer:
     i: int
     f: object          # int or list[int]
-    kind: str          # Conv | C2f | SPPF | Upsample | Concat | Detect
+    kind: str          # Conv | C2f | SPPF | AIFI | Upsample | Concat | Detect
     c1: object         # input channels (int, or list for Concat/Detect)
     c2: int            # output channels (Detect: 4*REG_MAX + nc)
     args: dict = field(default_factory=dict)
@@ -136,6 +137,13 @@ def parse_arch(d: dict, ch: int = 3) -> Arch:
                 L = Layer(i, f, m, c1, c2, {"n": n, "shortcut": bool(args[1]) if len(args) > 1 else False})
             else:
                 L = Layer(i, f, m, c1, c2, {"k": args[1] if len(args) > 1 else 5})
+        elif m == "AIFI":
+            c, heads = chs[f], args[1] if len(args) > 1 else 8
+            if n != 1:
+                raise ValueError("AIFI: one layer per row (repeats must be 1)")
+            if c % 8 or c % heads or c // heads > 128:
+                raise ValueError(f"AIFI: {c} channels must be a multiple of 8 and of the {heads} heads, at most 128 each")
+            L = Layer(i, f, m, c, c, {"hidden": args[0] if args else 2048, "heads": heads})
         elif m == "Upsample":
             L = Layer(i, f, m, chs[f], chs[f], {"scale": args[1]})
         elif m == "Concat":
@@ -187,6 +195,19 @@ def conv_specs(arch: Arch):
     return out
 
 
+def encoder_specs(arch: Arch):
+    """Every parameter of the AIFI layers in state-dict naming: (name, shape)."""
+    out = []
+    for L in arch.layers:
+        if L.kind == "AIFI":
+            p, c, h = f"model.{L.i}", L.c2, L.args["hidden"]
+            out += [(f"{p}.ma.in_proj_weight", (3 * c, c)), (f"{p}.ma.in_proj_bias", (3 * c,)),
+                    (f"{p}.ma.out_proj.weight", (c, c)), (f"{p}.ma.out_proj.bias", (c,)),
+                    (f"{p}.fc1.weight", (h, c)), (f"{p}.fc1.bias", (h,)), (f"{p}.fc2.weight", (c, h)), (f"{p}.fc2.bias", (c,))]
+            out += [(f"{p}.norm{j}.{n}", (c,)) for j in (1, 2) for n in ("weight", "bias")]
+    return out
+
+
 def detect_strides(arch: Arch) -> list:
     """Per-level strides of the Detect inputs (what DetectionModel's stride probe measures,
     tasks.py:409-418): products of conv strides / upsample factors along the graph."""
@@ -198,7 +219,7 @@ def detect_strides(arch: Arch) -> list:
             return st[x]
         if L.kind == "Conv":
             s = src(L.f) * L.args["s"]
-        elif L.kind in ("C2f", "SPPF"):
+        elif L.kind in ("C2f", "SPPF", "AIFI"):
             s = src(L.f)
         elif L.kind == "Upsample":
             s = src(L.f) // L.args["scale"]

@@ -4034,6 +4034,46 @@ void launch_wide_n(const WideArgs& a, int upt, size_t lds, hipStream_t st) {
   else launch_wide_t<Tr, NNT, 16, NW>(a, lds, st);
 }
 
+// The token operators on images [b0, b0 + B): an image's pixels are rows of c_stride elements, and
+// the images of a buffer follow each other, so a batch is one matrix.
+int launch_token_op(yk_model* m, const yk_op& op, int B, hipStream_t st, int b0) {
+  const int esz = act_bytes(m), dtype = m->desc.act_dtype;
+  const int64_t T = (int64_t)op.out_h * op.out_w;
+  auto at = [&](const yk_view& v) { return (char*)img_ptr(m, v.buf, v.h, v.w, v.c_stride, b0) + (size_t)v.c_off * esz; };
+  char* x = at(op.src[0]);
+  char* y = at(op.dst);
+  if (op.kind == YK_K_LINEAR) {
+    yk_linear_args a{};
+    a.dtype = dtype, a.act = op.act, a.bias_f32 = 1;
+    a.m = B * T, a.n = op.cout, a.k = op.src_ch[0];
+    a.x = x, a.x_stride = op.src[0].c_stride;
+    a.w = m->blob + op.w_off, a.w_stride = op.src_ch[0];
+    a.bias = m->blob + op.b_off;
+    a.y = y, a.y_stride = op.dst.c_stride;
+    if (op.has_res == 1) a.res = at(op.res), a.res_stride = op.res.c_stride, a.res_rows = a.m;
+    else if (op.has_res == 2) a.res = m->blob + op.t_off, a.res_stride = op.cout, a.res_rows = T;
+    return yk_linear(m->ctx, &a, st);
+  }
+  if (op.kind == YK_K_LAYER_NORM) {
+    yk_layer_norm_args a{};
+    a.dtype = dtype, a.param_f32 = 1;
+    a.m = B * T, a.c = op.cout, a.eps = 1e-5f;
+    a.x = x, a.x_stride = op.src[0].c_stride;
+    a.w = m->blob + op.w_off, a.b = m->blob + op.b_off;
+    a.y = y, a.y_stride = op.dst.c_stride;
+    return yk_layer_norm(m->ctx, &a, st);
+  }
+  const int d = op.cout / op.ksize;
+  yk_attention_args a{};
+  a.dtype = dtype;
+  a.b = B, a.h_q = a.h_kv = op.ksize, a.d = d, a.nq = a.nk = T;
+  a.scale = 1.f / sqrtf((float)d);
+  a.q = x, a.k = x + (size_t)op.cout * esz, a.v = x + (size_t)2 * op.cout * esz, a.o = y;
+  for (int64_t* s : {a.q_stride, a.k_stride, a.v_stride}) s[0] = T * op.src[0].c_stride, s[1] = op.src[0].c_stride, s[2] = d;
+  a.o_stride[0] = T * op.dst.c_stride, a.o_stride[1] = op.dst.c_stride, a.o_stride[2] = d;
+  return yk_attention(m->ctx, &a, st);
+}
+
 template <class Tr>
 int launch_op(yk_model* m, const yk_op& op, const uint8_t* frames, int B, float conf, hipStream_t st, int b0 = 0) {
   // images [b0, b0 + B) of the batch
@@ -4343,6 +4383,9 @@ int launch_op(yk_model* m, const yk_op& op, const uint8_t* frames, int B, float 
         hipLaunchKernelGGL(detect_kernel<Tr>, dim3((a.M + 63) / 64), dim3(256), 0, st, a);
         break;
       }
+      case YK_K_LINEAR:
+      case YK_K_LAYER_NORM:
+      case YK_K_ATTENTION: return launch_token_op(m, op, B, st, b0);
       default:
         yk::set_error("yk_detect: unknown op kind");
         return YK_ERR_ARG;
@@ -4390,6 +4433,10 @@ const char* op_kernel_name(const yk_model* m, const yk_op& op) {
         snprintf(buf, sizeof buf, "sppf_pool_kernel<yk::det::%s>", tn);
       return buf;
     case YK_K_DETECT: snprintf(buf, sizeof buf, "detect_kernel<yk::det::%s>", tn); return buf;
+    // (the token operators pick their instantiation by shape: the kernel's own name)
+    case YK_K_LINEAR: return (int64_t)op.out_h * op.out_w * m->desc.max_batch <= 64 ? "rows_kernel" : "gemm_kernel";
+    case YK_K_LAYER_NORM: return "norm_kernel";
+    case YK_K_ATTENTION: return "attn_kernel";
     default: break;
   }
   const ConvPlan cp = conv_plan(m, op, m->plan_batch);
@@ -4449,7 +4496,7 @@ void op_access(const yk_model* m, const yk_op& op, std::vector<int>& rd, std::ve
       break;
     default:
       for (int i = 0; i < op.n_src; ++i) rd.push_back(op.src[i].buf);
-      if (op.has_res) rd.push_back(op.res.buf);
+      if (op.has_res && !(op.kind == YK_K_LINEAR && op.has_res == 2)) rd.push_back(op.res.buf);
       wr.push_back(op.dst.buf);
       break;
   }

@@ -53,7 +53,7 @@ int validate_model_desc(const yk_model_desc* desc, int64_t blob_bytes) {
   for (int i = 0; i < desc->n_ops; ++i) {
     const yk_op& op = desc->ops[i];
     const std::string at = " (op " + std::to_string(i) + ", kind " + std::to_string(op.kind) + ")";
-    YK_CHECK_ARG(op.kind >= YK_K_CONV_INPUT && op.kind <= YK_K_DETECT, std::string("yk_model_create: bad op kind") + at);
+    YK_CHECK_ARG(op.kind >= YK_K_CONV_INPUT && op.kind <= YK_K_ATTENTION, std::string("yk_model_create: bad op kind") + at);
     YK_CHECK_ARG(op.dst.buf >= 0 && op.dst.buf < desc->n_bufs, std::string("yk_model_create: dst buffer index out of range") + at);
     YK_CHECK_ARG(op.n_src >= (op.kind == YK_K_CONV_INPUT ? 0 : 1) && op.n_src <= 2, std::string("yk_model_create: n_src") + at);
     for (int s = 0; s < op.n_src; ++s)
@@ -84,6 +84,38 @@ int validate_model_desc(const yk_model_desc* desc, int64_t blob_bytes) {
                          in_blob(op.b_off, (int64_t)(fp8 ? op.n_tiles * 16 + op.cout : op.cout) * 4, blob_bytes) &&
                          in_blob(op.t_off, 0, blob_bytes),
                      std::string("yk_model_create: conv weights outside the blob") + at);
+        break;
+      }
+      case YK_K_LINEAR:
+      case YK_K_LAYER_NORM:
+      case YK_K_ATTENTION: {
+        const int64_t esz = desc->act_dtype == YK_ACT_F32 ? 4 : 2, c = op.cout, k = op.src_ch[0];
+        YK_CHECK_ARG(!fp8, std::string("yk_model_create: token ops take bf16, f32 and f16 programs") + at);
+        YK_CHECK_ARG(op.n_src == 1 && c >= 1 && c <= 65536 && k >= 1 && k <= 65536 && op.src[0].up == 0 && op.dst.up == 0 &&
+                         op.src[0].buf != op.dst.buf,
+                     std::string("yk_model_create: token op geometry") + at);
+        YK_CHECK_ARG(view_ok(desc, op.src[0], k) && view_ok(desc, op.dst, c) && op.src[0].h == op.out_h &&
+                         op.src[0].w == op.out_w && op.dst.h == op.out_h && op.dst.w == op.out_w &&
+                         (int64_t)op.out_h * op.out_w * desc->max_batch < (1 << 30),
+                     std::string("yk_model_create: token op view outside its buffer") + at);
+        if (op.kind == YK_K_LINEAR) {
+          YK_CHECK_ARG(op.act >= YK_TOK_NONE && op.act <= YK_TOK_RELU && op.has_res >= 0 && op.has_res <= 2,
+                       std::string("yk_model_create: linear activation or residual kind") + at);
+          YK_CHECK_ARG(op.has_res != 1 || (view_ok(desc, op.res, c) && op.res.h == op.out_h && op.res.w == op.out_w &&
+                                           op.res.up == 0 && op.res.buf != op.dst.buf),
+                       std::string("yk_model_create: residual view outside its buffer") + at);
+          YK_CHECK_ARG(in_blob(op.w_off, c * k * esz, blob_bytes) && in_blob(op.b_off, c * 4, blob_bytes) &&
+                           (op.has_res != 2 || in_blob(op.t_off, (int64_t)op.out_h * op.out_w * c * esz, blob_bytes)) &&
+                           op.w_off % 4 == 0 && op.b_off % 4 == 0 && (op.has_res != 2 || op.t_off % 4 == 0),
+                       std::string("yk_model_create: linear weights outside the blob") + at);
+        } else if (op.kind == YK_K_LAYER_NORM) {
+          YK_CHECK_ARG(k == c && in_blob(op.w_off, c * 4, blob_bytes) && in_blob(op.b_off, c * 4, blob_bytes) &&
+                           op.w_off % 4 == 0 && op.b_off % 4 == 0,
+                       std::string("yk_model_create: layer norm weights outside the blob") + at);
+        } else {
+          YK_CHECK_ARG(k == 3 * c && op.ksize >= 1 && c % op.ksize == 0 && c / op.ksize <= 128,
+                       std::string("yk_model_create: attention heads must divide the channels, at most 128 each") + at);
+        }
         break;
       }
       case YK_K_CONV_INPUT:

@@ -9,6 +9,9 @@ resident in HBM:
   * Concat and C2f's chunk/cat become channel slices: producers write straight into
     the consumer's buffer, a consumer reads up to two views (K-space concatenation);
   * nn.Upsample(2, nearest) is folded into the consumer's gather (view.up = 1);
+  * an AIFI row is seven ops over the map's cells as tokens (the matrix product with its fused
+    epilogue, attention, layer norm: ops.py's kernels); the positions' part of the queries and keys
+    is a constant table, added by the first product's epilogue;
   * Detect's two first 3x3 convs share their input and are fused into one conv with
     N = 64 + c3; its final 1x1 convs are fused into the decode kernel.
 
@@ -30,7 +33,8 @@ from . import arch as A
 from . import letterbox as LB
 from . import weights as Wt
 
-YK_K_CONV_INPUT, YK_K_CONV, YK_K_SPPF_POOL, YK_K_DETECT = range(4)
+YK_K_CONV_INPUT, YK_K_CONV, YK_K_SPPF_POOL, YK_K_DETECT, YK_K_LINEAR, YK_K_LAYER_NORM, YK_K_ATTENTION = range(7)
+TOK_ACT = {"none": 0, "silu": 1, "gelu": 2, "relu": 3}
 ACT = {"bf16": 0, "fp32": 1, "fp8": 2, "fp16": 3}
 ESZ = {"bf16": 2, "fp32": 4, "fp8": 1, "fp16": 2}
 
@@ -110,6 +114,17 @@ def _fp8_bits(a: np.ndarray) -> np.ndarray:
 def fp8_round(t: torch.Tensor) -> torch.Tensor:
     """Values as stored in an FP8 activation buffer (saturated e4m3, round-to-nearest-even)."""
     return t.float().clamp(-448.0, 448.0).to(torch.float8_e4m3fn).float()
+
+
+def sincos_positions(h: int, w: int, c: int, temperature: float = 10000.0) -> np.ndarray:
+    """2-D sine-cosine position table [h * w, c] of an AIFI layer: sines and cosines of the column
+    number, then of the row number, at c / 4 frequencies.  Token t is cell (t // w, t % w) of the map,
+    but the table counts its columns first -- row t holds column t // h, row t % h, as trained weights
+    of this layer expect it -- so the two agree on square maps only."""
+    t = np.arange(h * w)
+    omega = 1.0 / temperature ** (np.arange(c // 4) / (c // 4))
+    a, b = (t // h)[:, None] * omega, (t % h)[:, None] * omega
+    return np.concatenate([np.sin(a), np.cos(a), np.sin(b), np.cos(b)], 1).astype(np.float32)
 
 
 class Program:
@@ -295,6 +310,8 @@ class Program:
                 out = self._c2f(Ly, inp(Ly.f))
             elif Ly.kind == "SPPF":
                 out = self._sppf(Ly, inp(Ly.f))
+            elif Ly.kind == "AIFI":
+                out = self._aifi(Ly, inp(Ly.f))
             elif Ly.kind == "Upsample":
                 assert Ly.args["scale"] == 2
                 out = [replace(s_, up=s_.up + 1) for s_ in inp(Ly.f)]
@@ -354,6 +371,68 @@ class Program:
         dst = Seg(ob, 0, c2p, c2p, Ly.c2, hh, ww)
         self.conv_op(f"{p}.cv2", zs, dst, list(range(Ly.c2)), c2p)
         return [dst]
+
+    def act_blob(self, a: np.ndarray) -> int:
+        """A float32 array stored in the activation type."""
+        a = np.ascontiguousarray(a, dtype=np.float32)
+        return self.add_blob(_bf16_bits(a) if self.dtype == "bf16" else _f16_bits(a) if self.dtype == "fp16" else a)
+
+    def token_op(self, kind, src: Seg, k: int, dst: Seg, n: int, macs: int) -> Op:
+        """A token op from k channels of src to n of dst, without its weights."""
+        op = Op()
+        op.kind, op.n_src = kind, 1
+        op.src[0] = View(src.buf, src.c_off, src.c_stride, src.h, src.w, 0)
+        op.src_ch[0] = k
+        op.dst = View(dst.buf, dst.c_off, dst.c_stride, dst.h, dst.w, 0)
+        op.cout = n
+        op.out_h, op.out_w = dst.h, dst.w
+        self.ops.append(op)
+        self.op_meta.append(macs)
+        return op
+
+    def _aifi(self, Ly, src):
+        if self.dtype == "fp8":
+            raise ValueError("AIFI runs in fp32, bf16 and fp16 programs")
+        if len(src) != 1 or src[0].up or src[0].cp != src[0].cl:
+            raise ValueError("AIFI must follow a layer with one output map (not Concat or nn.Upsample)")
+        x, c, hid, heads = src[0], Ly.c2, Ly.args["hidden"], Ly.args["heads"]
+        hh, ww = x.h, x.w
+        p, T = f"model.{Ly.i}", x.h * x.w
+        W = {k: self.sd[f"{p}.{k}"].float().numpy() for k in
+             ("ma.in_proj_weight", "ma.in_proj_bias", "ma.out_proj.weight", "ma.out_proj.bias", "fc1.weight", "fc1.bias",
+              "fc2.weight", "fc2.bias", "norm1.weight", "norm1.bias", "norm2.weight", "norm2.bias")}
+
+        def seg(n):
+            return Seg(self.new_buf(hh, ww, self.phys(n)), 0, self.phys(n), self.phys(n), n, hh, ww)
+
+        def linear(a: Seg, b: Seg, w, bias, act="none", res: Seg | None = None, table=None):
+            n, k = w.shape
+            op = self.token_op(YK_K_LINEAR, a, k, b, n, T * n * k)
+            op.act = TOK_ACT[act]
+            op.w_off, op.b_off = self.act_blob(w), self.add_blob(bias.astype(np.float32))
+            if res is not None:
+                op.has_res = 1
+                op.res = View(res.buf, res.c_off, res.c_stride, res.h, res.w, 0)
+            if table is not None:
+                op.has_res, op.t_off = 2, self.act_blob(table)
+
+        def norm(a: Seg, b: Seg, which):
+            op = self.token_op(YK_K_LAYER_NORM, a, c, b, c, 0)
+            op.w_off, op.b_off = (self.add_blob(W[f"norm{which}.{n}"].astype(np.float32)) for n in ("weight", "bias"))
+
+        qkv, o, h1, n1, a, h2, out = seg(3 * c), seg(c), seg(c), seg(c), seg(hid), seg(c), seg(c)
+        # queries and keys see the map plus the positions, values the map alone
+        wi = W["ma.in_proj_weight"]
+        table = np.zeros((T, 3 * c), np.float32)
+        table[:, :2 * c] = (sincos_positions(hh, ww, c).astype(np.float64) @ wi[:2 * c].T.astype(np.float64)).astype(np.float32)
+        linear(x, qkv, wi, W["ma.in_proj_bias"], table=table)
+        self.token_op(YK_K_ATTENTION, qkv, 3 * c, o, c, 2 * T * T * c).ksize = heads
+        linear(o, h1, W["ma.out_proj.weight"], W["ma.out_proj.bias"], res=x)
+        norm(h1, n1, 1)
+        linear(n1, a, W["fc1.weight"], W["fc1.bias"], act="gelu")
+        linear(a, h2, W["fc2.weight"], W["fc2.bias"], res=n1)
+        norm(h2, out, 2)
+        return [out]
 
     def _detect(self, Ly, level_in):
         c2b, c3, nc = Ly.args["c2"], Ly.args["c3"], Ly.args["nc"]

@@ -48,6 +48,11 @@ def synthetic_state_dict(ar: A.Arch, seed: int = 0, planted: bool = True, box_bi
                 sd[f"{p}.bias"] = torch.ones(c2)
             else:
                 sd[f"{p}.bias"] = torch.full((c2,), math.log(5 / ar.nc / (640 / strides[lvl]) ** 2))
+    for name, shape in A.encoder_specs(ar):
+        if ".norm" in name:
+            sd[name] = ru(0.8, 1.2, *shape) if name.endswith("weight") else rn(*shape, std=0.05)
+        else:
+            sd[name] = rn(*shape, std=1.0 / math.sqrt(shape[-1])) if len(shape) == 2 else rn(*shape, std=0.02)
     det = ar.layers[-1]
     sd[f"model.{det.i}.dfl.conv.weight"] = torch.arange(A.REG_MAX, dtype=torch.float32).view(1, A.REG_MAX, 1, 1)
     if planted and _is_p2_topology(ar):
