@@ -454,3 +454,51 @@ def test_calls_on_two_streams(ops):
     for o in outs:
         for a, b in zip(o, want):
             assert torch.equal(a, b)
+
+
+def test_linear_fp32_of_infinite_and_huge_values(ops):
+    """float32 products run as sums of bf16 parts, which cannot hold infinity nor what rounds to it:
+    sums they break are taken again, so infinities, NaN and values next to the largest come out as
+    the plain product's, in every direction and split."""
+    big = 3.4e38
+    for m, k, n in ((70, 96, 80), (300, 1500, 40)):
+        x, w, dy = rn(m, k), rn(n, k, std=k ** -0.5), rn(m, n, seed=1)
+        x[1, 2], x[2, 3], x[3, 4], x[5, 0], w[6, 7] = math.inf, -math.inf, math.nan, big, math.inf
+        w[8, 0], w[9, 9] = 2.0 ** -20, 0.0
+        x[10, 9] = math.inf  # times zero
+        want = x.double() @ w.double().t()
+        y = ops.linear(x, w)
+        fits = torch.where(want.abs() > torch.finfo(torch.float32).max, want.sign() * math.inf, want)
+        R.check(y, fits, (k + 8) * R.F * (x.double().abs() @ w.double().abs().t()).nan_to_num(posinf=0) * 2 + R.TINY, "y")
+        dx, dw, _, _ = ops.linear_backward(dy, x, w)
+        for got, a, b in ((dx, dy, w), (dw, dy.t(), x)):
+            g = a.double() @ b.double()
+            mag = (a.double().abs() @ b.double().abs()).nan_to_num(posinf=0)
+            R.check(got, torch.where(g.abs() > torch.finfo(torch.float32).max, g.sign() * math.inf, g), (m + n + 8) * R.F * mag * 2 + R.TINY,
+                    "gradient")
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_few_keys_many_rows(ops, dt, causal):
+    """Few key blocks against many rows: the rows are split and their sums of dk and dv joined."""
+    run_attention(ops, dt, 2, 700, 30, 6, 2, 40, causal)
+    run_attention(ops, dt, 3, 333, 333, 6, 2, 24, causal, lengths=[333, 0, 170], q_lengths=[333, 0, 170])
+    run_attention(ops, dt, 1, 600, 100, 3, 3, 96, causal, lengths=[70])
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("m,k,n", [(100, 9000, 24), (16000, 100, 100), (70, 4000, 1000)])
+def test_linear_split_products(ops, dt, m, k, n):
+    """Products whose K is split: the join's lanes and orders, forward and backward."""
+    x, w, b, dy = rn(m, k, dt=dt), rn(n, k, dt=dt, std=k ** -0.5), rn(n, dt=dt), rn(m, n, dt=dt, seed=1)
+    y, z = ops.linear(x, w, b, act="silu", return_preact=True)
+    want, ey, wz, ez = R.linear(x, w, b, "silu", None)
+    R.check(y, want, ey, "y")
+    R.check(z, wz, ez, "z")
+    assert torch.equal(y, ops.linear(x, w, b, act="silu"))
+    got = ops.linear_backward(dy, x, w, b, act="silu", preact=z)
+    again = ops.linear_backward(dy, x, w, b, act="silu", preact=z)
+    for (want, e), g, a in zip(R.linear_grads(dy, x, w, "silu", z), got, again):
+        R.check(g, want, R._final(want, e, g.dtype) if g.dim() == 1 else e, "grads")
+        assert torch.equal(g, a)

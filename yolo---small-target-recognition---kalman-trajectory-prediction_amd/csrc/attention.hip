@@ -27,6 +27,7 @@ struct AttnArgs {
   const int32_t *q_lengths, *lengths;
   int64_t qs[3], ks[3], vs[3], os[3], gos[3], dqs[3], dks[3], dvs[3];
   float* part;        // split: [item][split][16][d_pad + 4]; backward: lse2, delta [b][hk][rows]
+  float* kv_part;     // backward, rows split: [split][b * hk * nk][dk, dv: 2 d_pad]
   float scale;
   int b, hk, group, d, nq, nk, causal, rows, splits;  // rows = nq * group
 };
@@ -647,7 +648,8 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs a) {
   a.part[all + id] = s;
 }
 
-// dk and dv: 4 waves of 16 kNT keys, blocks of packed rows (q, do and their statistics) through LDS.
+// dk and dv: 4 waves of 16 kNT keys, blocks of packed rows (q, do and their statistics) through LDS;
+// with few keys, blockIdx.y a range of the rows, whose float32 sums attn_dkv_sum_kernel adds.
 template <class Tr, int kDP, int kNT, bool kAsync>
 __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_dkv_kernel(AttnArgs a, int key_blocks) {
   using T = typename Tr::T;
@@ -680,6 +682,12 @@ __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_dkv_kernel(AttnAr
   int r_begin = 0;
   if (a.causal && key0 > s.off) r_begin = (int)((int64_t)(key0 - s.off) * a.group < r_end ? (int64_t)(key0 - s.off) * a.group : r_end);
   r_begin = r_begin / Bl::kBN * Bl::kBN;
+  int r_stop = r_end;
+  if (gridDim.y > 1 && r_begin < r_end) {
+    const int per = ((r_end - r_begin + Bl::kBN - 1) / Bl::kBN + gridDim.y - 1) / gridDim.y * Bl::kBN;
+    r_begin = blockIdx.y * per < r_end - r_begin ? r_begin + blockIdx.y * per : r_end;
+    r_stop = r_end - r_begin < per ? r_end : r_begin + per;
+  }
   const float sl2 = a.scale * kLog2e;
   Feed<Tr, kDP, kAsync> fq, fo;
   fq.init(a.q, a.qs, b, hk * a.group, a.group, a.d, r_begin);
@@ -701,7 +709,7 @@ __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_dkv_kernel(AttnAr
       *(float*)(at + i * 4) = r0 + i < r_end ? p[i] : 0.f;
     }
   };
-  for_blocks<Tr, kDP, kAsync>(fq, fo, r_begin, r_end, r_end, lds, kBuf, stats, [&](const char* lq, int r0) {
+  for_blocks<Tr, kDP, kAsync>(fq, fo, r_begin, r_stop, r_end, lds, kBuf, stats, [&](const char* lq, int r0) {
     const char* lo = lq + Bl::kBytesAll;
     const float* stat = (const float*)(lo + Bl::kBytesAll);
     // the block's first query sees least
@@ -766,6 +774,15 @@ __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_dkv_kernel(AttnAr
     const int key = key0 + (wave * kNT + j) * 16 + l16;
     if (key >= a.nk) continue;
     const bool live = key < s.klen;  // a column behind the length holds P of zeros, not a gradient
+    if (gridDim.y > 1) {
+      float* to = a.kv_part + (((int64_t)blockIdx.y * a.b * a.hk + bh) * a.nk + key) * (2 * kDP) + g * 4;
+#pragma unroll
+      for (int t = 0; t < kDT; ++t) {
+        *(f32x4*)(to + t * 16) = dk[j][t];
+        *(f32x4*)(to + kDP + t * 16) = dv[j][t];
+      }
+      continue;
+    }
     T* pk = (T*)a.dk + b * a.dks[0] + (int64_t)key * a.dks[1] + hk * a.dks[2];
     T* pv = (T*)a.dv + b * a.dvs[0] + (int64_t)key * a.dvs[1] + hk * a.dvs[2];
 #pragma unroll
@@ -775,6 +792,25 @@ __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_dkv_kernel(AttnAr
       store_out<Tr>(pv, t * 16 + g * 4, a.d, live ? dv[j][t] : z);
     }
   }
+}
+
+// The row ranges' sums of dk and dv added in order: 4 elements of a key's row per thread.
+template <class Tr>
+__global__ __launch_bounds__(256) void attn_dkv_sum_kernel(AttnArgs a, int dp, int splits) {
+  using T = typename Tr::T;
+  const int per = dp / 2, c = threadIdx.x % per;  // (dp / 4 quads of dk, then of dv)
+  const int64_t keys = (int64_t)a.b * a.hk * a.nk, id = (int64_t)blockIdx.x * (256 / per) + threadIdx.x / per;
+  if (threadIdx.x >= 256 / per * per || id >= keys) return;
+  const int bh = (int)(id / a.nk), key = (int)(id - (int64_t)bh * a.nk), b = bh / a.hk, hk = bh - b * a.hk;
+  f32x4 v{0.f, 0.f, 0.f, 0.f};
+  if (key < clamp_len(a.lengths, b, a.nk)) {
+    const float* p = a.kv_part + id * (2 * dp) + c * 4;
+    for (int s = 0; s < splits; ++s) v += *(const f32x4*)(p + s * keys * (2 * dp));
+  }
+  const bool k = c < per / 2;
+  T* to = k ? (T*)a.dk + b * a.dks[0] + (int64_t)key * a.dks[1] + hk * a.dks[2]
+            : (T*)a.dv + b * a.dvs[0] + (int64_t)key * a.dvs[1] + hk * a.dvs[2];
+  store_out<Tr>(to, (k ? c : c - per / 2) * 4, a.d, k ? v * a.scale : v);
 }
 
 // dq: 4 waves of 16 kNT rows, key blocks (k, v) through LDS.
@@ -899,6 +935,17 @@ inline bool feed_async(const char* p, const int64_t* st, int d, int group, int b
          (bn / group * st[1] + group * st[2]) * bytes < (int64_t(1) << 30);
 }
 
+// Row ranges of the dk / dv kernel: one where its key blocks fill the chip, else as many as fill it
+// twice, of two blocks of rows at least (5 x 333 tokens, 3 heads on a key head, float32: 61 us whole,
+// 17 in eight).
+inline int row_splits(int bytes, int64_t bh, int64_t rows, int64_t nk) {
+  const int64_t wgs = bh * cdiv(nk, 64), blocks = cdiv(rows, 128 / bytes);
+  int64_t s = wgs < kCUs ? cdiv(2 * kCUs, wgs) : 1;
+  if (s > blocks / 2) s = blocks / 2;
+  return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
+}
+inline int64_t stat_words(int64_t bh, int64_t rows) { return cdiv(2 * bh * rows, 4) * 4; }
+
 template <class Tr, int kDP>
 void run_split(const AttnArgs& a, hipStream_t st) {
   const int64_t bh = (int64_t)a.b * a.hk;
@@ -920,8 +967,11 @@ void launch_fwd(const AttnArgs& a, hipStream_t st) {
 }
 template <class Tr, int kDP, int kNT, bool kAsync = true>
 void launch_dkv(const AttnArgs& a, hipStream_t st) {
-  const int kb = (int)cdiv(a.nk, 64 * kNT);
-  hipLaunchKernelGGL((attn_dkv_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * kb)), dim3(256), 0, st, a, kb);
+  const int kb = (int)cdiv(a.nk, 64 * kNT), s = a.splits;
+  hipLaunchKernelGGL((attn_dkv_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * kb), s), dim3(256), 0, st, a, kb);
+  if (s > 1)
+    hipLaunchKernelGGL(attn_dkv_sum_kernel<Tr>, dim3((unsigned)cdiv((int64_t)a.b * a.hk * a.nk, 256 / (kDP / 2))), dim3(256), 0, st,
+                       a, kDP, s);
 }
 template <class Tr, int kDP, int kNT, bool kAsync = true>
 void launch_dq(const AttnArgs& a, hipStream_t st) {
@@ -1043,7 +1093,11 @@ int yk_attention(yk_ctx* ctx, const yk_attention_args* a, void* stream) {
 int yk_attention_backward_workspace(const yk_attention_grad_args* a, int64_t* bytes) {
   YK_CHECK_ARG(a && bytes, "yk_attention_backward_workspace: NULL argument");
   if (const int rc = check_attn("yk_attention_backward_workspace", a)) return rc;
-  *bytes = 2 * (int64_t)a->b * a->h_q * a->nq * 4;
+  const int64_t bh = (int64_t)a->b * a->h_kv, rows = a->nq * (a->h_q / a->h_kv);
+  *bytes = stat_words(bh, rows) * 4;
+  if (bh == 0 || rows == 0 || a->nk == 0) return YK_OK;
+  const int s = row_splits(tok_bytes(a->dtype), bh, rows, a->nk);
+  if (s > 1) *bytes += (int64_t)s * bh * a->nk * 2 * pad_d(a->d) * 4;
   return YK_OK;
 }
 
@@ -1063,6 +1117,8 @@ int yk_attention_backward(yk_ctx* ctx, const yk_attention_grad_args* a, void* st
   k.o = (const char*)a->o, k.go = (const char*)a->go;
   k.dq = (char*)a->dq, k.dk = (char*)a->dk, k.dv = (char*)a->dv;
   k.lse = (float*)a->lse;
+  k.splits = row_splits(tok_bytes(a->dtype), (int64_t)k.b * k.hk, k.rows, k.nk);
+  k.kv_part = k.part + stat_words((int64_t)k.b * k.hk, k.rows);
   for (int i = 0; i < 3; ++i) k.gos[i] = a->go_stride[i], k.dqs[i] = a->dq_stride[i], k.dks[i] = a->dk_stride[i], k.dvs[i] = a->dv_stride[i];
   const hipStream_t st = (hipStream_t)stream;
   if (a->dtype == YK_ACT_F32) run_attn<F32>(k, true, st);

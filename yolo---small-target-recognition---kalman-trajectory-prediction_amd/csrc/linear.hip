@@ -193,11 +193,14 @@ struct Loader {
             rsrc, (__attribute__((address_space(3))) void*)(lds + (i * kThreads + rfl(tid & ~63)) * 16), 16, o, 0, 0, 0);
       }
     } else {
+      const bool inside = rows >= (kTrans ? Tl::kK : kRows) && cols >= (kTrans ? kRows : Tl::kK);
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
         int row, col;
         Tl::locate(i * kThreads + tid, row, col);
-        reg[i] = row < rows ? load16<Tr>(base + row * stride + col, cols - col) : u32x4{0, 0, 0, 0};
+        const T* p = base + row * stride + col;
+        if (inside) reg[i] = *(const u32x4_any*)p;
+        else reg[i] = row < rows ? load16<Tr>(p, cols - col) : u32x4{0, 0, 0, 0};
       }
     }
   }
@@ -208,6 +211,54 @@ struct Loader {
     }
   }
 };
+
+// A wave's accumulators (rows m0 .., columns n0 ..) to memory: through the epilogue, or as a split's
+// sums.  mend(buf, pitch, first row): may change the 32 rows in transit.
+template <class Tr, int kFM, int kFN, int kWaves, int kLds, class F>
+__device__ __forceinline__ void finish_tile(const GemmArgs& a, const f32x4 (&acc)[kFN][kFM], char* lds, int m0, int n0, F&& mend) {
+  // The accumulators pass through LDS 32 rows at a time (each wave in a part of its own), so that
+  // a lane finishes 8 neighbouring n and a row's stores and residual reads are whole lines.
+  constexpr int kPass = 2, kPitch = kFN * 16 + 4, kCh = kFN * 2, kStepRows = 64 / kCh;
+  static_assert(kFM % kPass == 0 && kWaves * kPass * 16 * kPitch * 4 <= kLds, "the rows in transit fit the tiles' LDS");
+  float* buf = (float*)lds + rfl(threadIdx.x >> 6) * kPass * 16 * kPitch;
+  const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4, c = lane % kCh, n = n0 + c * 8;
+  float b[8];
+  bias8(a, n, b);
+#pragma unroll
+  for (int j0 = 0; j0 < kFM; j0 += kPass) {
+#pragma unroll
+    for (int j = 0; j < kPass; ++j)
+#pragma unroll
+      for (int i = 0; i < kFN; ++i) *(f32x4*)(buf + (j * 16 + l) * kPitch + i * 16 + g * 4) = acc[i][j0 + j];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    mend(buf, kPitch, m0 + j0 * 16);
+#pragma unroll
+    for (int h = 0; h < kPass * 16 / kStepRows; ++h) {
+      const int row = h * kStepRows + lane / kCh;
+      const int64_t m = (int64_t)m0 + j0 * 16 + row;
+      const f32x4 lo = *(const f32x4*)(buf + row * kPitch + c * 8), hi = *(const f32x4*)(buf + row * kPitch + c * 8 + 4);
+      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      if (m >= a.m || n >= a.n) continue;
+      if (a.part) {
+        float* p = a.part + ((int64_t)blockIdx.y * a.m + m) * a.n + n;
+        if (a.n - n >= 8) {
+          store8<F32>(p, v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e < a.n) p[e] = v[e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += b[e];
+        epilogue<Tr>(a, m, n, v);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
 
 // Until this wave's loads but the last kLeft have landed, and its LDS reads are done; then until all
 // waves are there.
@@ -306,69 +357,236 @@ __global__ __launch_bounds__(64 * kWM * kWN) void gemm_kernel(GemmArgs a) {
     }
   }
 
-  // The accumulators pass through LDS 32 rows at a time (each wave in a part of its own), so that
-  // a lane finishes 8 neighbouring n and a row's stores and residual reads are whole lines.
-  constexpr int kPass = 2, kPitch = kFN * 16 + 4, kCh = kFN * 2, kStepRows = 64 / kCh;
-  static_assert(kFM % kPass == 0 && kWM * kWN * kPass * 16 * kPitch * 4 <= kStages * kBuf, "the rows in transit fit the tiles' LDS");
-  float* buf = (float*)&lds[0][0] + wave * kPass * 16 * kPitch;
-  const int l = lane & 15, g = lane >> 4, c = lane % kCh, n = tn * kTN + wn * 16 + c * 8;
+  finish_tile<Tr, kFM, kFN, kWM * kWN, kStages * kBuf>(a, acc, &lds[0][0], tm * kTM + wm * 16, tn * kTN + wn * 16,
+                                                       [](float*, int, int) {});
+}
+
+// float32 on the bf16 matrix cores.  x = x0 + x1 + x2 exactly, three bf16 of 8 significant bits each
+// (rounded to nearest, so |x1| <= 2^-9 |x| and |x2| <= 2^-18 |x|), and six of the nine products are
+// summed: w0x0, w0x1, w1x0, w1x1, w0x2, w2x0.  bf16 products are exact in float32 and what is left out
+// is below 2^-25 |w x|, less than one float32 rounding; six 16-cycle MFMAs per 32 of K replace eight
+// 32-cycle float32 ones.  4096 x 1024 x 4096: 188 us, 267 on v_mfma_f32_16x16x4_f32.
+//
+// The parts are made once per tile, between the global loads' registers and LDS (three planes a
+// side), not by every wave that reads them.  A tile is 32 of K:
+//   plain       plane [row][4 chunks of 8 k], chunk c of row r at c ^ (r >> 2 & 3)
+//   transposed  plane [k][kRows], segments of 16 rows twisted as in Tile
+template <bool kTrans, int kRows>
+struct SplitTile {
+  using Tw = Tile<B16, kTrans, kRows>;
+  static constexpr int kK = 32, kUnits = kRows * 4, kPerRow = kTrans ? kRows / 8 : 4, kPlane = kRows * 64;
+  // stored row, first element and place of unit j (8 elements)
+  static __device__ __forceinline__ void locate(int j, int& row, int& col, int& at) {
+    row = j / kPerRow;
+    const int c = j % kPerRow;
+    col = c * 8;
+    if constexpr (kTrans) at = row * (kRows * 2) + (((c >> 1) ^ Tw::twist(row)) << 5) + (c & 1) * 16;
+    else at = row * 64 + ((c ^ ((row >> 2) & 3)) << 4);
+  }
+  static __device__ __forceinline__ s16x8 frag(const char* plane, int t, int lane) {
+    const int l = lane & 15, g = lane >> 4;
+    if constexpr (kTrans) return Tw::frag(plane, t, 0, lane);
+    else return *(const s16x8*)(plane + (t * 16 + l) * 64 + ((g ^ (l >> 2)) << 4));
+  }
+};
+
+// x rounded to bf16 (two at a time, v_cvt_pk_bf16_f32) and what that leaves
+__device__ __forceinline__ unsigned split_pair(float& a, float& b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const unsigned u = __builtin_bit_cast(unsigned, bf16x2{(__bf16)a, (__bf16)b});
+  a -= __uint_as_float(u << 16);
+  b -= __uint_as_float(u & 0xffff0000u);
+  return u;
+}
+
+template <bool kTrans, int kRows>
+struct SplitLoader {
+  using Tl = SplitTile<kTrans, kRows>;
+  static constexpr int kN = Tl::kUnits / 256;
+  const float* base;
+  int64_t stride;
+  int rows, cols;
+  u32x4 reg[kN][2];
+  __device__ __forceinline__ void init(const char* p, int64_t s, int r0, int m, int k0, int k1) {
+    stride = s;
+    base = (const float*)p + (kTrans ? (int64_t)k0 * s + r0 : (int64_t)r0 * s + k0);
+    rows = kTrans ? k1 - k0 : m - r0;
+    cols = kTrans ? m - r0 : k1 - k0;
+  }
+  __device__ __forceinline__ void advance() {
+    base += kTrans ? Tl::kK * stride : Tl::kK;
+    (kTrans ? rows : cols) -= Tl::kK;
+  }
+  __device__ __forceinline__ void issue() {
+    const bool inside = rows >= (kTrans ? Tl::kK : kRows) && cols >= (kTrans ? kRows : Tl::kK);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      int row, col, at;
+      Tl::locate(i * 256 + threadIdx.x, row, col, at);
+      const float* p = base + row * stride + col;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (inside) reg[i][h] = *(const u32x4_any*)(p + 4 * h);
+        else reg[i][h] = row < rows ? load16<F32>(p + 4 * h, cols - col - 4 * h) : u32x4{0, 0, 0, 0};
+      }
+    }
+  }
+  __device__ __forceinline__ void commit(char* lds) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      int row, col, at;
+      Tl::locate(i * 256 + threadIdx.x, row, col, at);
+      u32x4 part[3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float a = __uint_as_float(reg[i][e >> 1][(e & 1) * 2]), b = __uint_as_float(reg[i][e >> 1][(e & 1) * 2 + 1]);
+        part[0][e] = split_pair(a, b);
+        part[1][e] = split_pair(a, b);
+        part[2][e] = split_pair(a, b);
+      }
+#pragma unroll
+      for (int q = 0; q < 3; ++q) *(u32x4*)(lds + q * Tl::kPlane + at) = part[q];
+    }
+  }
+};
+
+template <bool kXT, bool kWT, int kTile>
+__global__ __launch_bounds__(256, 2) void gemm_f32_kernel(GemmArgs a) {
+  using XTile = SplitTile<kXT, kTile>;
+  using WTile = SplitTile<kWT, kTile>;
+  constexpr int kF = kTile / 32, kHalf = 3 * XTile::kPlane;
+  __shared__ __attribute__((aligned(16))) char lds[2 * kHalf];
+  const int lane = threadIdx.x & 63, wave = rfl(threadIdx.x >> 6);
+  const int item = xcd_item(blockIdx.x, a.tiles_m * a.tiles_n);
+  const int per = 8 * a.tiles_n, grp = item / per, in = item - grp * per;
+  const int gm = a.tiles_m - grp * 8 < 8 ? a.tiles_m - grp * 8 : 8;
+  const int tn = in / gm, tm = grp * 8 + in - tn * gm;
+  const int k0 = blockIdx.y * a.k_split, k1 = a.k - k0 < a.k_split ? a.k : k0 + a.k_split;
+  SplitLoader<kXT, kTile> lx;
+  SplitLoader<kWT, kTile> lw;
+  lx.init(a.x, a.x_stride, tm * kTile, a.m, k0, k1);
+  lw.init(a.w, a.w_stride, tn * kTile, a.n, k0, k1);
+  const int wm = (wave & 1) * kF, wn = (wave >> 1) * kF;
+  f32x4 acc[kF][kF];
+#pragma unroll
+  for (int i = 0; i < kF; ++i)
+#pragma unroll
+    for (int j = 0; j < kF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int nk = (k1 - k0 + 31) / 32;
+  lx.issue();
+  lw.issue();
+  for (int kt = 0; kt < nk; ++kt) {
+    __syncthreads();
+    lx.commit(lds);
+    lw.commit(lds + kHalf);
+    __syncthreads();
+    if (kt + 1 < nk) {
+      lx.advance();
+      lw.advance();
+      lx.issue();
+      lw.issue();
+    }
+    s16x8 wf[kF][3];
+#pragma unroll
+    for (int i = 0; i < kF; ++i)
+#pragma unroll
+      for (int q = 0; q < 3; ++q) wf[i][q] = WTile::frag(lds + kHalf + q * WTile::kPlane, wn + i, lane);
+#pragma unroll
+    for (int j = 0; j < kF; ++j) {
+      s16x8 xf[3];
+#pragma unroll
+      for (int q = 0; q < 3; ++q) xf[q] = XTile::frag(lds + q * XTile::kPlane, wm + j, lane);
+      // (a pass over the wave's tiles per product: neighbouring MFMAs do not wait for each other)
+      constexpr int kPair[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
+#pragma unroll
+      for (int q = 0; q < 6; ++q)
+#pragma unroll
+        for (int i = 0; i < kF; ++i) acc[i][j] = mma<B16>(wf[i][kPair[q][0]], xf[kPair[q][1]], acc[i][j]);
+    }
+  }
+  __syncthreads();
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < kF; ++i)
+#pragma unroll
+    for (int j = 0; j < kF; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bad = bad || acc[i][j][e] != acc[i][j][e];
+  // An infinite operand, or one that bf16's range rounds to infinity, makes NaN of its parts: such
+  // sums are taken again, plainly.  (Once a sum is NaN it stays one.)
+  const bool any = __any(bad);
+  auto mend = [&](float* buf, int pitch, int m0) {
+    if (!any) return;
+#pragma unroll 1
+    for (int i = lane; i < 32 * kF * 16; i += 64) {
+      const int row = i / (kF * 16), col = i % (kF * 16), m = m0 + row, n = tn * kTile + wn * 16 + col;
+      if (buf[row * pitch + col] == buf[row * pitch + col] || m >= a.m || n >= a.n) continue;
+      float s = 0.f;
+#pragma unroll 1
+      for (int64_t k = k0; k < k1 && s == s; ++k)
+        s = fmaf(((const float*)a.x)[kXT ? k * a.x_stride + m : m * a.x_stride + k],
+                 ((const float*)a.w)[kWT ? k * a.w_stride + n : n * a.w_stride + k], s);
+      buf[row * pitch + col] = s;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  finish_tile<F32, kF, kF, 4, 2 * kHalf>(a, acc, lds, tm * kTile + wm * 16, tn * kTile + wn * 16, mend);
+}
+
+// Sum of the split products, then the epilogue: 8 consecutive n per kLanes threads, of which each adds
+// every kLanes-th split, 4 loads in flight; their sums are joined in a fixed order.
+template <class Tr, int kLanes>
+__global__ __launch_bounds__(256) void split_sum_kernel(GemmArgs a, int splits) {
+  __shared__ float lds[kLanes > 1 ? kLanes : 1][256 / kLanes][9];
+  const int n8 = (a.n + 7) / 8, sub = threadIdx.x / (256 / kLanes), id = threadIdx.x % (256 / kLanes);
+  const int64_t i = (int64_t)blockIdx.x * (256 / kLanes) + id;
+  const int64_t m = i / n8;
+  const int n = (int)(i - m * n8) * 8, left = a.n - n;
+  float v[8] = {};
+  if (m < a.m) {
+    const int64_t step = (int64_t)a.m * a.n;
+    const float* p = a.part + m * a.n + n;
+    if (left >= 8) {
+      for (int s0 = sub; s0 < splits; s0 += 4 * kLanes) {
+        f32x4 t[4][2];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int s = s0 + q * kLanes;
+          const float* r = p + (s < splits ? s : s0) * step;
+          t[q][0] = load4<F32>(r);
+          t[q][1] = load4<F32>(r + 4);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (s0 + q * kLanes >= splits) break;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += t[q][e >> 2][e & 3];
+        }
+      }
+    } else {
+      for (int s = sub; s < splits; s += kLanes) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < left) v[e] += p[s * step + e];
+      }
+    }
+  }
+  if constexpr (kLanes > 1) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) lds[sub][id][e] = v[e];
+    __syncthreads();
+    if (sub) return;
+#pragma unroll
+    for (int s = 1; s < kLanes; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += lds[s][id][e];
+  }
+  if (m >= a.m) return;
   float b[8];
   bias8(a, n, b);
 #pragma unroll
-  for (int j0 = 0; j0 < kFM; j0 += kPass) {
-#pragma unroll
-    for (int j = 0; j < kPass; ++j)
-#pragma unroll
-      for (int i = 0; i < kFN; ++i) *(f32x4*)(buf + (j * 16 + l) * kPitch + i * 16 + g * 4) = acc[i][j0 + j];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int h = 0; h < kPass * 16 / kStepRows; ++h) {
-      const int row = h * kStepRows + lane / kCh;
-      const int64_t m = (int64_t)tm * kTM + (wm + j0) * 16 + row;
-      const f32x4 lo = *(const f32x4*)(buf + row * kPitch + c * 8), hi = *(const f32x4*)(buf + row * kPitch + c * 8 + 4);
-      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      if (m >= a.m || n >= a.n) continue;
-      if (a.part) {
-        float* p = a.part + ((int64_t)blockIdx.y * a.m + m) * a.n + n;
-        if (a.n - n >= 8) {
-          store8<F32>(p, v);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (n + e < a.n) p[e] = v[e];
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += b[e];
-        epilogue<Tr>(a, m, n, v);
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  }
-}
-
-// Sum of the split products in order, then the epilogue: 8 consecutive n per thread.
-template <class Tr>
-__global__ __launch_bounds__(256) void split_sum_kernel(GemmArgs a, int splits) {
-  const int n8 = (a.n + 7) / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t m = i / n8;
-  if (m >= a.m) return;
-  const int n = (int)(i - m * n8) * 8, left = a.n - n;
-  float v[8];
-  bias8(a, n, v);
-  for (int s = 0; s < splits; ++s) {
-    const float* p = a.part + ((int64_t)s * a.m + m) * a.n + n;
-    if (left >= 8) {
-      add8<F32>(p, v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < left) v[e] += p[e];
-    }
-  }
+  for (int e = 0; e < 8; ++e) v[e] += b[e];
   epilogue<Tr>(a, m, n, v);
 }
 
@@ -519,7 +737,7 @@ constexpr int kCUs = 256;
 // Time of a product by tile size, from sweeps of tile and split on this card (microseconds; a step
 // is 64 of K for the 16-bit types, 32 for float32): `alone` per step for the only workgroup of
 // its CU (its loads' latency), `shared` per step and workgroup where `per_cu` of them share it
-// (the CU's load rate; the MFMAs for float32), `ends` / `ends_shared` for the first loads and the
+// (the CU's load rate; the MFMAs and the splitting for float32), `ends` / `ends_shared` for the first loads and the
 // epilogue.  16-bit, 4096 x 1024 x 4096: 128-tiles 49 us, 64-tiles 50, 256-tiles 95 (64 of them on
 // 256 CUs); 40960 x 4096 x 1024: 360 / 394 (256 / 128); 1000^3: 8.8 / 13.7 (64 / 128); float32
 // 10240 x 2048 x 512: 186 / 203 (64 / 128).
@@ -528,11 +746,11 @@ struct TileTime {
   double alone, shared, ends, ends_shared;
 };
 constexpr TileTime kTimes16[] = {{256, 1, 1.5, 1.5, 12, 12}, {128, 2, 0.7, 0.44, 4.5, 2.6}, {64, 4, 0.35, 0.19, 2.5, 0.8}};
-constexpr TileTime kTimes32[] = {{128, 2, 2.15, 2.05, 5, 3.5}, {64, 4, 0.72, 0.52, 2.5, 1}};
+constexpr TileTime kTimes32[] = {{128, 2, 1.75, 1.34, 5, 3.5}, {64, 4, 0.85, 0.455, 3, 1.2}};
 
 // The tile and the split of K that the table says are fastest.  trans: operands that lie transposed
-// (their fragments take twice the LDS reads, which shows where a workgroup is alone: 2048 x 512 x
-// 10240, both transposed, 256 64-tiles: 103 us, split in 4: 45).  A split costs a launch and its
+// (their fragments take twice the LDS reads, which shows where a 16-bit workgroup is alone: 2048 x 512
+// x 10240, both transposed, 256 64-tiles: 103 us, split in 4: 45).  A split costs a launch and its
 // float32 sums once written and once read.
 inline Plan plan_gemm(int64_t m, int64_t n, int64_t k, int bytes, int trans, bool async) {
   const int64_t kk = 128 / bytes, steps = cdiv(k, kk);
@@ -545,7 +763,7 @@ inline Plan plan_gemm(int64_t m, int64_t n, int64_t k, int bytes, int trans, boo
     for (int64_t s = 1; s == 1 || (s <= 64 && steps >= 4 * s && tiles * s <= kCUs * t.per_cu); s += s < 4 ? 1 : s / 2) {
       const int64_t per = cdiv(steps, s), wgs = cdiv(tiles * cdiv(steps, per), kCUs);
       auto turn = [&](int64_t r) {  // r workgroups at once on a CU
-        return r == 0 ? 0.0 : per * fmax(t.alone * (1 + 0.4 * trans), r * t.shared) + fmax(t.ends, r * t.ends_shared);
+        return r == 0 ? 0.0 : per * fmax(t.alone * (bytes == 2 ? 1 + 0.4 * trans : 1), r * t.shared) + fmax(t.ends, r * t.ends_shared);
       };
       double us = (wgs / t.per_cu) * turn(t.per_cu) + turn(wgs % t.per_cu);
       if (s > 1) us += 4 + (double)m * n * s * 8 / 8e6;
@@ -571,7 +789,12 @@ constexpr int kFewRows = 64;
 template <class Tr, bool kXT, bool kWT, bool kAsync>
 void launch_tiles(const GemmArgs& a, int tile, int splits, hipStream_t st) {
   const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), (unsigned)splits);
-  if constexpr (Tr::kBytes == 2 && kAsync) {
+  if constexpr (Tr::kBytes == 4) {
+    if (tile == 128) hipLaunchKernelGGL((gemm_f32_kernel<kXT, kWT, 128>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((gemm_f32_kernel<kXT, kWT, 64>), grid, dim3(256), 0, st, a);
+    return;
+  } else {
+  if constexpr (kAsync) {
     if (tile == 256) {
       hipLaunchKernelGGL((gemm_kernel<Tr, kXT, kWT, 256, 256, 2, 4, 2, true>), grid, dim3(512), 0, st, a);
       return;
@@ -579,6 +802,7 @@ void launch_tiles(const GemmArgs& a, int tile, int splits, hipStream_t st) {
   }
   if (tile == 128) hipLaunchKernelGGL((gemm_kernel<Tr, kXT, kWT, 128, 128, 2, 2, 2, kAsync>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((gemm_kernel<Tr, kXT, kWT, 64, 64, 2, 2, 2, kAsync>), grid, dim3(256), 0, st, a);
+  }
 }
 
 // rows of 16-byte chunks whose offsets inside a tile stay below 2^31 (256 rows of less than 2^23 bytes)
@@ -604,11 +828,13 @@ void launch_gemm(GemmArgs a, void* part, int64_t room, hipStream_t st) {
   a.k_split = p.k_split;
   a.tiles_m = (int)cdiv(a.m, p.tile);
   a.tiles_n = (int)cdiv(a.n, p.tile);
-  if (async) launch_tiles<Tr, kXT, kWT, true>(a, p.tile, p.splits, st);
+  if (async && Tr::kBytes == 2) launch_tiles<Tr, kXT, kWT, true>(a, p.tile, p.splits, st);
   else launch_tiles<Tr, kXT, kWT, false>(a, p.tile, p.splits, st);
-  if (p.splits > 1)
-    hipLaunchKernelGGL(split_sum_kernel<Tr>, dim3((unsigned)cdiv((int64_t)a.m * cdiv(a.n, 8), 256)), dim3(256), 0, st, a,
-                       p.splits);
+  if (p.splits > 1) {
+    const int64_t items = (int64_t)a.m * cdiv(a.n, 8);
+    if (p.splits >= 8) hipLaunchKernelGGL((split_sum_kernel<Tr, 8>), dim3((unsigned)cdiv(items, 32)), dim3(256), 0, st, a, p.splits);
+    else hipLaunchKernelGGL((split_sum_kernel<Tr, 1>), dim3((unsigned)cdiv(items, 256)), dim3(256), 0, st, a, p.splits);
+  }
 }
 
 template <class Tr>
