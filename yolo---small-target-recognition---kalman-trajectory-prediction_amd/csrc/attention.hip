@@ -93,8 +93,9 @@ __device__ __forceinline__ typename Tr::V8 pack8(f32x4 lo, f32x4 hi) {
 }
 
 // kBN x kDP block of rows in LDS (kDP = d padded to 32, zero filled) in 16-byte chunks.  Chunk c of a
-// row lies at c ^ (row >> kShift) within its group of kGroup chunks, so that the 16 rows of a
-// fragment, whichever way it is read, fall on different banks.
+// row lies at c ^ twist(row) within its group of kGroup chunks.  The 16-bit twist serves both reads without
+// bank conflicts (SQ_LDS_BANK_CONFLICT 0): 16 rows of one chunk (16 lanes a cycle, which are rows 0-3 and 12-15 of one lane
+// group with rows 4-11 of the next), and 8 rows of 32 bytes (the transposing read's 32 lanes).
 template <class Tr, int kDP>
 struct Block {
   using T = typename Tr::T;
@@ -105,10 +106,13 @@ struct Block {
   static constexpr int kN = kDP / 32;           // chunks per thread of 256
   static constexpr int kBytesAll = kBN * kRow;
   static constexpr int kGroup = kRow % 256 == 0 ? 16 : kRow % 128 == 0 ? 8 : 4;
-  static constexpr int kShift = kGroup == 16 ? 0 : kGroup == 8 ? 1 : 2;
 
   static __device__ __forceinline__ int place(int row, int c) {  // (its own inverse in c)
-    return (c & ~(kGroup - 1)) | ((c ^ (row >> kShift)) & (kGroup - 1));
+    const int twist = Tr::kBytes == 4 ? (kGroup == 16 ? row & 15 : (row >> 1) & 7)
+                      : kGroup == 16  ? (row & 7) << 1
+                      : kGroup == 8   ? row & 7
+                                      : (row >> 1) & 2;
+    return c ^ twist;
   }
   // A operand: row 16 t + l, elements 32 s + 8 g ..
   static __device__ __forceinline__ typename Tr::V8 row_frag(const char* lds, int t, int s, int lane) {

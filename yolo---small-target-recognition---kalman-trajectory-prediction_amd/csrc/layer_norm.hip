@@ -411,7 +411,7 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* part, in
 }
 
 constexpr int kMaxChunks = 4 * 256;       // a row in the registers of a workgroup
-constexpr int kGradGroups = 1024;         // workgroups (and rows of partial sums) of the backward pass
+constexpr int kGradGroups = 768;          // workgroups (and rows of partial sums) of the backward pass
 
 constexpr int kNarrowRows = 8192;
 

@@ -34,6 +34,9 @@ _NORM_GRAD = struct.Struct("2i 2q 8Q 3q")
 _ATTENTION = struct.Struct("6i 2q f i 7Q 12q")
 _ATTENTION_GRAD = struct.Struct("6i 2q f i 11Q 24q")
 _WS = struct.Struct("Q q")
+_NO_WS = _WS.pack(0, 0)
+_raw_stream = torch._C._cuda_getCurrentRawStream  # (torch.cuda.current_stream builds an object around it)
+_entry: dict = {}    # entry point -> its ctypes function
 _scratch: dict = {}  # (entry point, sizes) -> bytes of scratch
 
 
@@ -104,12 +107,14 @@ def _vector(t, name, n, dev, dtype):
 def _call(fn, packed, dev, sizes=None):
     """Enqueue an entry point on the device's current stream, with the scratch that `sizes` (all its
     size depends on) needs."""
-    lib = L.lib()
+    call = _entry.get(fn)
+    if call is None:
+        call = _entry[fn] = getattr(L.lib(), fn)
     if sizes is not None:
         need = _scratch.get((fn, sizes))
         if need is None:
             n = C.c_int64()
-            L.check(getattr(lib, fn + "_workspace")(packed + _WS.pack(0, 0), C.byref(n)), fn)
+            L.check(getattr(L.lib(), fn + "_workspace")(packed + _NO_WS, C.byref(n)), fn)
             if len(_scratch) >= 4096:
                 _scratch.clear()
             need = _scratch[(fn, sizes)] = n.value
@@ -117,8 +122,8 @@ def _call(fn, packed, dev, sizes=None):
             ws = _empty(need, dtype=torch.uint8, device=torch.device("cuda", dev))
             packed += _WS.pack(ws.data_ptr(), need)
         else:
-            packed += _WS.pack(0, 0)
-    rc = getattr(lib, fn)(L.context(dev), packed, torch._C._cuda_getCurrentRawStream(dev))
+            packed += _NO_WS
+    rc = call(L.context(dev), packed, _raw_stream(dev))
     if rc:
         L.check(rc, fn)
 
