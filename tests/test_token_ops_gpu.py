@@ -502,3 +502,12 @@ def test_linear_split_products(ops, dt, m, k, n):
     for (want, e), g, a in zip(R.linear_grads(dy, x, w, "silu", z), got, again):
         R.check(g, want, R._final(want, e, g.dtype) if g.dim() == 1 else e, "grads")
         assert torch.equal(g, a)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_few_rows_many_keys_backward(ops, dt, causal):
+    """A token or a few against many keys, trained: the keys are split and their sums of dq joined."""
+    run_attention(ops, dt, 2, 1, 1500, 4, 2, 80, causal)
+    run_attention(ops, dt, 3, 5, 700, 2, 1, 24, causal, lengths=[700, 0, 129], q_lengths=[5, 2, 0])
+    run_attention(ops, dt, 1, 40, 900, 2, 2, 128, causal, lengths=[333])

@@ -28,8 +28,9 @@ struct AttnArgs {
   int64_t qs[3], ks[3], vs[3], os[3], gos[3], dqs[3], dks[3], dvs[3];
   float* part;        // split: [item][split][16][d_pad + 4]; backward: lse2, delta [b][hk][rows]
   float* kv_part;     // backward, rows split: [split][b * hk * nk][dk, dv: 2 d_pad]
+  float* q_part;      // backward, keys split: [split][b * hk * rows][d_pad]
   float scale;
-  int b, hk, group, d, nq, nk, causal, rows, splits;  // rows = nq * group
+  int b, hk, group, d, nq, nk, causal, rows, splits, key_splits;  // rows = nq * group
 };
 
 struct Seq {          // one batch element's lengths
@@ -817,7 +818,21 @@ __global__ __launch_bounds__(256) void attn_dkv_sum_kernel(AttnArgs a, int dp, i
   store_out<Tr>(to, (k ? c : c - per / 2) * 4, a.d, k ? v * a.scale : v);
 }
 
-// dq: 4 waves of 16 kNT rows, key blocks (k, v) through LDS.
+// The key ranges' sums of dq added in order: 4 elements of a packed row per thread.
+template <class Tr>
+__global__ __launch_bounds__(256) void attn_dq_sum_kernel(AttnArgs a, int dp, int splits) {
+  using T = typename Tr::T;
+  const int per = dp / 4, c = threadIdx.x % per;
+  const int64_t all = (int64_t)a.b * a.hk * a.rows, id = (int64_t)blockIdx.x * (256 / per) + threadIdx.x / per;
+  if (threadIdx.x >= 256 / per * per || id >= all) return;
+  const int bh = (int)(id / a.rows), r = (int)(id - (int64_t)bh * a.rows), b = bh / a.hk, hk = bh - b * a.hk;
+  f32x4 v{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; ++s) v += *(const f32x4*)(a.q_part + (s * all + id) * dp + c * 4);
+  store_out<Tr>(row_ptr((T*)a.dq, a.dqs, b, hk, a.group, r), c * 4, a.d, v * a.scale);
+}
+
+// dq: 4 waves of 16 kNT rows, key blocks (k, v) through LDS; with few rows, blockIdx.y a range of the keys,
+// whose float32 sums attn_dq_sum_kernel adds.
 template <class Tr, int kDP, int kNT, bool kAsync>
 __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_dq_kernel(AttnArgs a, int row_blocks) {
   using T = typename Tr::T;
@@ -853,9 +868,16 @@ __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_dq_kernel(AttnArg
   }
   const float sl2 = a.scale * kLog2e;
   Feed<Tr, kDP, kAsync> fk, fv;
-  fk.init(a.k, a.ks, b, hk, 1, a.d, 0);
-  fv.init(a.v, a.vs, b, hk, 1, a.d, 0);
-  for_blocks<Tr, kDP, kAsync>(fk, fv, 0, key_end(a, s, r0, kRows), s.klen, lds, kBuf, [](char*, int) {}, [&](const char* lk, int k0) {
+  const int k_end = key_end(a, s, r0, kRows);
+  int k_begin = 0, k_stop = k_end;
+  if (gridDim.y > 1) {
+    const int per = ((k_end + Bl::kBN - 1) / Bl::kBN + (int)gridDim.y - 1) / (int)gridDim.y * Bl::kBN;
+    k_begin = (int)blockIdx.y * per < k_end ? (int)blockIdx.y * per : k_end;
+    k_stop = k_end - k_begin < per ? k_end : k_begin + per;
+  }
+  fk.init(a.k, a.ks, b, hk, 1, a.d, k_begin);
+  fv.init(a.v, a.vs, b, hk, 1, a.d, k_begin);
+  for_blocks<Tr, kDP, kAsync>(fk, fv, k_begin, k_stop, s.klen, lds, kBuf, [](char*, int) {}, [&](const char* lk, int k0) {
     const char* lv = lk + Bl::kBytesAll;
 #pragma unroll
     for (int u = 0; u < kKT / 2; ++u) {
@@ -902,8 +924,14 @@ __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_dq_kernel(AttnArg
   for (int j = 0; j < kNT; ++j) {
     const int r = r0 + (wave * kNT + j) * 16 + l16;
     if (r >= a.rows) continue;
-    T* p = row_ptr((T*)a.dq, a.dqs, b, hk, a.group, r);
     const bool live = lim[j] > 0;
+    if (gridDim.y > 1) {
+      float* to = a.q_part + (((int64_t)blockIdx.y * a.b * a.hk + bh) * a.rows + r) * kDP + g * 4;
+#pragma unroll
+      for (int t = 0; t < kDT; ++t) *(f32x4*)(to + t * 16) = live ? dq[j][t] : f32x4{0.f, 0.f, 0.f, 0.f};
+      continue;
+    }
+    T* p = row_ptr((T*)a.dq, a.dqs, b, hk, a.group, r);
 #pragma unroll
     for (int t = 0; t < kDT; ++t)
       store_out<Tr>(p, t * 16 + g * 4, a.d, live ? dq[j][t] * a.scale : f32x4{0.f, 0.f, 0.f, 0.f});
@@ -939,11 +967,12 @@ inline bool feed_async(const char* p, const int64_t* st, int d, int group, int b
          (bn / group * st[1] + group * st[2]) * bytes < (int64_t(1) << 30);
 }
 
-// Row ranges of the dk / dv kernel: one where its key blocks fill the chip, else as many as fill it
-// twice, of two blocks of rows at least (5 x 333 tokens, 3 heads on a key head, float32: 61 us whole,
-// 17 in eight).
-inline int row_splits(int bytes, int64_t bh, int64_t rows, int64_t nk) {
-  const int64_t wgs = bh * cdiv(nk, 64), blocks = cdiv(rows, 128 / bytes);
+// Ranges of the backward kernels (rows for dk / dv, keys for dq: `n` of the side that stays, `over` of
+// the one that is walked): one where the workgroups fill the chip, else as many as fill it twice, of
+// two blocks at least (5 x 333 tokens, 3 heads on a key head, float32: dk / dv 61 us whole, 17 in eight;
+// one query against 12731 keys, 48 heads of 80, forward and backward: 528 us with dq whole, 261 split).
+inline int range_splits(int bytes, int64_t bh, int64_t n, int64_t over) {
+  const int64_t wgs = bh * cdiv(n, 64), blocks = cdiv(over, 128 / bytes);
   int64_t s = wgs < kCUs ? cdiv(2 * kCUs, wgs) : 1;
   if (s > blocks / 2) s = blocks / 2;
   return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
@@ -979,8 +1008,11 @@ void launch_dkv(const AttnArgs& a, hipStream_t st) {
 }
 template <class Tr, int kDP, int kNT, bool kAsync = true>
 void launch_dq(const AttnArgs& a, hipStream_t st) {
-  const int rb = (int)cdiv(a.rows, 64 * kNT);
-  hipLaunchKernelGGL((attn_dq_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * rb)), dim3(256), 0, st, a, rb);
+  const int rb = (int)cdiv(a.rows, 64 * kNT), s = a.key_splits;
+  hipLaunchKernelGGL((attn_dq_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * rb), s), dim3(256), 0, st, a, rb);
+  if (s > 1)
+    hipLaunchKernelGGL(attn_dq_sum_kernel<Tr>, dim3((unsigned)cdiv((int64_t)a.b * a.hk * a.rows, 256 / (kDP / 4))), dim3(256), 0, st,
+                       a, kDP, s);
 }
 
 template <class Tr, int kDP>
@@ -1100,8 +1132,9 @@ int yk_attention_backward_workspace(const yk_attention_grad_args* a, int64_t* by
   const int64_t bh = (int64_t)a->b * a->h_kv, rows = a->nq * (a->h_q / a->h_kv);
   *bytes = stat_words(bh, rows) * 4;
   if (bh == 0 || rows == 0 || a->nk == 0) return YK_OK;
-  const int s = row_splits(tok_bytes(a->dtype), bh, rows, a->nk);
+  const int s = range_splits(tok_bytes(a->dtype), bh, a->nk, rows), ks = range_splits(tok_bytes(a->dtype), bh, rows, a->nk);
   if (s > 1) *bytes += (int64_t)s * bh * a->nk * 2 * pad_d(a->d) * 4;
+  if (ks > 1) *bytes += (int64_t)ks * bh * rows * pad_d(a->d) * 4;
   return YK_OK;
 }
 
@@ -1121,8 +1154,11 @@ int yk_attention_backward(yk_ctx* ctx, const yk_attention_grad_args* a, void* st
   k.o = (const char*)a->o, k.go = (const char*)a->go;
   k.dq = (char*)a->dq, k.dk = (char*)a->dk, k.dv = (char*)a->dv;
   k.lse = (float*)a->lse;
-  k.splits = row_splits(tok_bytes(a->dtype), (int64_t)k.b * k.hk, k.rows, k.nk);
-  k.kv_part = k.part + stat_words((int64_t)k.b * k.hk, k.rows);
+  const int64_t bh = (int64_t)k.b * k.hk;
+  k.splits = range_splits(tok_bytes(a->dtype), bh, k.nk, k.rows);
+  k.key_splits = range_splits(tok_bytes(a->dtype), bh, k.rows, k.nk);
+  k.kv_part = k.part + stat_words(bh, k.rows);
+  k.q_part = k.kv_part + (k.splits > 1 ? (int64_t)k.splits * bh * k.nk * 2 * pad_d(k.d) : 0);
   for (int i = 0; i < 3; ++i) k.gos[i] = a->go_stride[i], k.dqs[i] = a->dq_stride[i], k.dks[i] = a->dk_stride[i], k.dvs[i] = a->dv_stride[i];
   const hipStream_t st = (hipStream_t)stream;
   if (a->dtype == YK_ACT_F32) run_attn<F32>(k, true, st);

@@ -452,11 +452,15 @@ void launch_norm_grad(const NormGradArgs& a, int nv, int groups, hipStream_t st)
   else hipLaunchKernelGGL((norm_grad_kernel<Tr, NT, 2>), dim3(groups), block, lds, st, a);
 }
 // Lanes per row of the backward pass: at most two chunks each, whose sums, row and next row are some
-// 150 registers (four took 270, one wave per SIMD: 10000 x 8192 bf16 187 us)
-inline int grad_lanes(int chunks) { return chunks <= 16 ? 16 : chunks <= 128 ? 64 : chunks <= 512 ? 256 : 512; }
+// 150 registers (four took 270, one wave per SIMD: 10000 x 8192 bf16 187 us).  Two of 16 lanes only with
+// rows enough to fill the chip.
+inline int grad_lanes(int64_t m, int chunks) {
+  if (chunks <= 16 || (chunks <= 32 && m >= kNarrowRows)) return 16;
+  return chunks <= 128 ? 64 : chunks <= 512 ? 256 : 512;
+}
 // Workgroups: enough for the chip, several rows each so that their sums are not most of the traffic
 inline int grad_groups(int64_t m, int c, int bytes) {
-  const int nt = grad_lanes((int)cdiv(c, 16 / bytes));
+  const int nt = grad_lanes(m, (int)cdiv(c, 16 / bytes));
   const int64_t turns = cdiv(m, nt < 256 ? 256 / nt : 1);
   const int64_t g = turns / 4 < 128 ? 128 : turns / 4;
   return (int)(turns < g ? turns : g > kGradGroups ? kGradGroups : g);
@@ -471,8 +475,8 @@ void run_norm_grad(const NormGradArgs& a, hipStream_t st) {
       hipLaunchKernelGGL(norm_cols_kernel<Tr>, dim3((unsigned)cdiv(chunks, 64), groups), dim3(256), 0, st, a);
     return;
   }
-  switch (grad_lanes(chunks)) {
-    case 16: launch_norm_grad<Tr, 16>(a, 1, groups, st); break;
+  switch (grad_lanes(a.m, chunks)) {
+    case 16: launch_norm_grad<Tr, 16>(a, (int)cdiv(chunks, 16), groups, st); break;
     case 64: launch_norm_grad<Tr, 64>(a, (int)cdiv(chunks, 64), groups, st); break;
     case 256: launch_norm_grad<Tr, 256>(a, (int)cdiv(chunks, 256), groups, st); break;
     default: launch_norm_grad<Tr, 512>(a, (int)cdiv(chunks, 512), groups, st); break;

@@ -71,6 +71,11 @@ def _like(t, name, dev, dtype, other=None):
     return t
 
 
+def _fresh(t):
+    """An uninitialised contiguous tensor like t (empty_like is the faster call where that is one)."""
+    return _empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _rows(t, name, cols=None):
     """(rows, columns, row stride) of a tensor as a matrix of its last dimension."""
     shape = t.shape
@@ -189,7 +194,7 @@ def linear_backward(dy, x, weight, bias=None, *, act="none", preact=None, residu
         if mz != m:
             raise ValueError("preact must have a row for every row of x")
         z = preact.data_ptr()
-    dx, dw = x.new_empty(x.shape), x.new_empty(weight.shape)
+    dx, dw = _fresh(x), _fresh(weight)
     db = dres = None
     pb = bf = pr = rows = 0
     if bias is not None:
@@ -234,7 +239,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, return_stats=False):
     w, b, pf = _norm_params(weight, bias, c, dev, x.dtype)
     if not eps >= 0:
         raise ValueError("eps must be >= 0")
-    y = x.new_empty(x.shape)
+    y = _fresh(x)
     mean = rstd = None
     if return_stats:
         mean = x.new_empty(x.shape[:-1], dtype=_F32)
@@ -259,7 +264,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd):
         raise ValueError("dy must have a row for every row of x")
     w, _, pf = _norm_params(weight, None, c, dev, x.dtype)
     dw = x.new_empty(c, dtype=_F32) if weight is None else weight.new_empty(c)
-    dx, db = x.new_empty(x.shape), _empty_like(dw)
+    dx, db = _fresh(x), _empty_like(dw)
     _call("yk_layer_norm_backward",
           _NORM_GRAD.pack(dt, int(dw.dtype is _F32), m, c, dy.data_ptr(), x.data_ptr(), w, mean.data_ptr(), rstd.data_ptr(),
                           dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ds, xs, c),
@@ -315,7 +320,7 @@ def attention(q, k, v, *, scale=None, causal=False, lengths=None, q_lengths=None
     no key gives 0.  Returns o like q, with return_lse also ln of the softmax's denominators,
     float32 [B, H, Nq] (-inf where no key is seen), for attention_backward."""
     dev, head, qkv, lens, strides = _attention_args(q, k, v, scale, causal, q_lengths, lengths)
-    o = q.new_empty(q.shape)
+    o = _fresh(q)
     lse = q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=_F32) if return_lse else None
     if o.numel():
         _call("yk_attention", _ATTENTION.pack(*head, *qkv, *lens, o.data_ptr(), lse.data_ptr() if return_lse else 0, *strides,
@@ -331,7 +336,7 @@ def attention_backward(do, q, k, v, o, lse, *, scale=None, causal=False, lengths
     os = _heads(_like(o, "o", dev, q.dtype), "o", q.shape)
     if _like(lse, "lse", dev, _F32).shape != (q.shape[0], q.shape[2], q.shape[1]) or not lse.is_contiguous():
         raise ValueError("lse must be attention's second result, contiguous [B, H, Nq]")
-    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    dq, dk, dv = _fresh(q), _fresh(k), _fresh(v)
     if not q.numel() or not k.numel():
         return dq.zero_(), dk.zero_(), dv.zero_()
     _call("yk_attention_backward",
