@@ -511,3 +511,21 @@ def test_attention_few_rows_many_keys_backward(ops, dt, causal):
     run_attention(ops, dt, 2, 1, 1500, 4, 2, 80, causal)
     run_attention(ops, dt, 3, 5, 700, 2, 1, 24, causal, lengths=[700, 0, 129], q_lengths=[5, 2, 0])
     run_attention(ops, dt, 1, 40, 900, 2, 2, 128, causal, lengths=[333])
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("act", ["none", "gelu", "silu", "relu"])
+@pytest.mark.parametrize("m,k,n", [(4136, 64, 4096), (2560, 72, 1032)])
+def test_linear_whole_and_partial_tiles(ops, dt, act, m, k, n):
+    """Products of many tiles, most of them whole: the epilogue with and without a residual of
+    fewer rows, and their gradients."""
+    x, w, b, res = rn(m, k, dt=dt), rn(n, k, dt=dt, std=k ** -0.5), rn(n, dt=dt), rn(77, n, dt=dt, seed=2)
+    for bias, r in ((b, res), (None, None)):
+        y, z = ops.linear(x, w, bias, act=act, residual=r, return_preact=True)
+        want, ey, wz, ez = R.linear(x, w, bias, act, r)
+        R.check(y, want, ey, f"y {act}")
+        R.check(z, wz, ez, f"z {act}")
+        assert torch.equal(y, ops.linear(x, w, bias, act=act, residual=r))
+    dy = rn(m, n, dt=dt, seed=3)
+    for (want, e), g, name in zip(R.linear_grads(dy, x, w, act, z), ops.linear_backward(dy, x, w, b, act=act, preact=z), ("dx", "dw", "db")):
+        R.check(g, want, R._final(want, e, b.dtype) if name == "db" else e, f"{name} {act}")

@@ -212,33 +212,105 @@ struct Loader {
   }
 };
 
+// A wave's accumulators pass through LDS 32 rows at a time (each wave in a part of its own), so that a lane
+// finishes 8 neighbouring n and a row's stores and residual reads are whole lines.
+template <int kFM, int kFN, int kWaves, int kLds>
+struct Transit {
+  static constexpr int kPass = 2, kPitch = kFN * 16 + 4, kCh = kFN * 2, kStepRows = 64 / kCh, kSteps = kPass * 16 / kStepRows;
+  static_assert(kFM % kPass == 0 && kWaves * kPass * 16 * kPitch * 4 <= kLds, "the rows in transit fit the tiles' LDS");
+  // body(j0): the rows 16 j0 .. + 31 are in buf
+  template <class B>
+  static __device__ __forceinline__ void run(const f32x4 (&acc)[kFN][kFM], float* buf, B&& body) {
+    const int l = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int j0 = 0; j0 < kFM; j0 += kPass) {
+#pragma unroll
+      for (int j = 0; j < kPass; ++j)
+#pragma unroll
+        for (int i = 0; i < kFN; ++i) *(f32x4*)(buf + (j * 16 + l) * kPitch + i * 16 + g * 4) = acc[i][j0 + j];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      body(j0);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  static __device__ __forceinline__ void fetch(const float* buf, int row, int c, float* v) {
+    const f32x4 lo = *(const f32x4*)(buf + row * kPitch + c * 8), hi = *(const f32x4*)(buf + row * kPitch + c * 8 + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+  }
+};
+
+// The epilogue of rows and columns that all exist, its activation known: addresses are a uniform base and a
+// lane's 32-bit offset.
+template <class Tr, int kAct, class X, int kFM, int kFN, class F>
+__device__ __forceinline__ void finish_whole(const GemmArgs& a, const f32x4 (&acc)[kFN][kFM], float* buf, int m0, int n0, F&& mend) {
+  using T = typename Tr::T;
+  const int lane = threadIdx.x & 63, c = lane % X::kCh, r = lane / X::kCh;
+  const unsigned yo = (unsigned)(r * (int)a.y_stride + c * 8), zo = (unsigned)(r * (int)a.z_stride + c * 8);
+  float b[8];
+  bias8(a, n0 + c * 8, b);
+  X::run(acc, buf, [&](int j0) {
+    // the residual's rows are on their way before the first store (which they might alias, for all the
+    // compiler knows)
+    u32x4 rv[X::kSteps][Tr::kBytes / 2];
+    if (a.res) {
+#pragma unroll
+      for (int h = 0; h < X::kSteps; ++h) {
+        const unsigned mr = (unsigned)(m0 + j0 * 16 + h * X::kStepRows + r);
+        const T* p = (const T*)a.res + (int64_t)(a.res_rows == a.m ? mr : mr % (unsigned)a.res_rows) * a.res_stride + n0 + c * 8;
+#pragma unroll
+        for (int i = 0; i < Tr::kBytes / 2; ++i) rv[h][i] = *(const u32x4_any*)((const char*)p + i * 16);
+      }
+    }
+    mend(buf, X::kPitch, m0 + j0 * 16);
+#pragma unroll
+    for (int h = 0; h < X::kSteps; ++h) {
+      const int64_t m = (int64_t)m0 + j0 * 16 + h * X::kStepRows;  // (the first of the rows of this step)
+      float v[8];
+      X::fetch(buf, h * X::kStepRows + r, c, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += b[e];
+      if (a.z) store8<Tr>((T*)a.z + m * a.z_stride + n0 + zo, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = act_f32(v[e], kAct);
+      if (a.res) {
+        T t[8];
+        __builtin_memcpy(t, rv[h], sizeof t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += to_f32<Tr>(t[e]);
+      }
+      store8<Tr>((T*)a.y + m * a.y_stride + n0 + yo, v);
+    }
+  });
+}
+
 // A wave's accumulators (rows m0 .., columns n0 ..) to memory: through the epilogue, or as a split's
 // sums.  mend(buf, pitch, first row): may change the 32 rows in transit.
 template <class Tr, int kFM, int kFN, int kWaves, int kLds, class F>
 __device__ __forceinline__ void finish_tile(const GemmArgs& a, const f32x4 (&acc)[kFN][kFM], char* lds, int m0, int n0, F&& mend) {
-  // The accumulators pass through LDS 32 rows at a time (each wave in a part of its own), so that
-  // a lane finishes 8 neighbouring n and a row's stores and residual reads are whole lines.
-  constexpr int kPass = 2, kPitch = kFN * 16 + 4, kCh = kFN * 2, kStepRows = 64 / kCh;
-  static_assert(kFM % kPass == 0 && kWaves * kPass * 16 * kPitch * 4 <= kLds, "the rows in transit fit the tiles' LDS");
-  float* buf = (float*)lds + rfl(threadIdx.x >> 6) * kPass * 16 * kPitch;
-  const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4, c = lane % kCh, n = n0 + c * 8;
+  using X = Transit<kFM, kFN, kWaves, kLds>;
+  float* buf = (float*)lds + rfl(threadIdx.x >> 6) * X::kPass * 16 * X::kPitch;
+  constexpr int64_t kMaxStride = 1 << 24;
+  if (!a.part && m0 + kFM * 16 <= a.m && n0 + kFN * 16 <= a.n && a.y_stride < kMaxStride && (!a.z || a.z_stride < kMaxStride)) {
+    if (a.act == YK_TOK_GELU) finish_whole<Tr, YK_TOK_GELU, X>(a, acc, buf, m0, n0, mend);
+    else if (a.act == YK_TOK_SILU) finish_whole<Tr, YK_TOK_SILU, X>(a, acc, buf, m0, n0, mend);
+    else if (a.act == YK_TOK_RELU) finish_whole<Tr, YK_TOK_RELU, X>(a, acc, buf, m0, n0, mend);
+    else finish_whole<Tr, YK_TOK_NONE, X>(a, acc, buf, m0, n0, mend);
+    return;
+  }
+  const int lane = threadIdx.x & 63, c = lane % X::kCh, n = n0 + c * 8;
   float b[8];
   bias8(a, n, b);
+  X::run(acc, buf, [&](int j0) {
+    mend(buf, X::kPitch, m0 + j0 * 16);
 #pragma unroll
-  for (int j0 = 0; j0 < kFM; j0 += kPass) {
-#pragma unroll
-    for (int j = 0; j < kPass; ++j)
-#pragma unroll
-      for (int i = 0; i < kFN; ++i) *(f32x4*)(buf + (j * 16 + l) * kPitch + i * 16 + g * 4) = acc[i][j0 + j];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    mend(buf, kPitch, m0 + j0 * 16);
-#pragma unroll
-    for (int h = 0; h < kPass * 16 / kStepRows; ++h) {
-      const int row = h * kStepRows + lane / kCh;
+    for (int h = 0; h < X::kSteps; ++h) {
+      const int row = h * X::kStepRows + lane / X::kCh;
       const int64_t m = (int64_t)m0 + j0 * 16 + row;
-      const f32x4 lo = *(const f32x4*)(buf + row * kPitch + c * 8), hi = *(const f32x4*)(buf + row * kPitch + c * 8 + 4);
-      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      float v[8];
+      X::fetch(buf, row, c, v);
       if (m >= a.m || n >= a.n) continue;
       if (a.part) {
         float* p = a.part + ((int64_t)blockIdx.y * a.m + m) * a.n + n;
@@ -255,9 +327,7 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& a, const f32x4 (&acc
         epilogue<Tr>(a, m, n, v);
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  }
+  });
 }
 
 // Until this wave's loads but the last kLeft have landed, and its LDS reads are done; then until all
@@ -651,7 +721,7 @@ struct ColArgs {
 
 // Sums over the rows m % r == residue, for each column; a workgroup holds 32 chunks of columns x 8
 // rows of one residue, blockIdx.y a group of them.
-template <class Tr>
+template <class Tr, int kAct>
 __global__ __launch_bounds__(256) void cols_kernel(ColArgs a) {
   using T = typename Tr::T;
   constexpr int kEpc = 16 / Tr::kBytes;
@@ -663,24 +733,28 @@ __global__ __launch_bounds__(256) void cols_kernel(ColArgs a) {
   float acc[kEpc];
 #pragma unroll
   for (int e = 0; e < kEpc; ++e) acc[e] = 0.f;
-  if (n > 0) {
-    for (int64_t row = res + ((int64_t)blockIdx.y * 8 + sub) * a.r; row < a.m; row += (int64_t)gridDim.y * 8 * a.r) {
-      const u32x4 u = load16<Tr>((const T*)a.dy + row * a.dy_stride + c0, n);
-      T d[kEpc];
+  const int64_t step = (int64_t)gridDim.y * 8 * a.r;
+  int64_t row = res + ((int64_t)blockIdx.y * 8 + sub) * a.r;
+  if (n > 0 && row < a.m) {
+    u32x4 u, uz;  // the row after the one worked on is on its way
+    auto load = [&](int64_t at) {
+      u = load16<Tr>((const T*)a.dy + at * a.dy_stride + c0, n);
+      if constexpr (kAct != YK_TOK_NONE) uz = load16<Tr>((const T*)a.z + at * a.z_stride + c0, n);
+    };
+    load(row);
+    for (; row < a.m; row += step) {
+      T d[kEpc], zv[kEpc];
       __builtin_memcpy(d, &u, 16);
-      if (a.act != YK_TOK_NONE) {
-        const u32x4 uz = load16<Tr>((const T*)a.z + row * a.z_stride + c0, n);
-        T zv[kEpc];
-        __builtin_memcpy(zv, &uz, 16);
-        float f[kEpc];
-#pragma unroll
-        for (int e = 0; e < kEpc; ++e) f[e] = to_f32<Tr>(d[e]) * act_slope(to_f32<Tr>(zv[e]), a.act);
+      if constexpr (kAct != YK_TOK_NONE) __builtin_memcpy(zv, &uz, 16);
+      if (row + step < a.m) load(row + step);
+      if constexpr (kAct != YK_TOK_NONE) {
+        // dz is rounded to the operands' type: it is an operand of two matrix products
 #pragma unroll
         for (int e = 0; e < kEpc; ++e) {
-          acc[e] += f[e];
-          d[e] = from_f32<Tr>(f[e]);
+          const float f = to_f32<Tr>(d[e]) * act_slope(to_f32<Tr>(zv[e]), kAct);
+          acc[e] += f;
+          d[e] = from_f32<Tr>(f);
         }
-        // dz is rounded to the operands' type: it is an operand of two matrix products
         T* o = (T*)a.dz + row * a.n + c0;
         if (n >= kEpc) {
           u32x4 v;
@@ -745,7 +819,7 @@ struct TileTime {
   int tile, per_cu;
   double alone, shared, ends, ends_shared;
 };
-constexpr TileTime kTimes16[] = {{256, 1, 1.5, 1.5, 12, 12}, {128, 2, 0.7, 0.44, 4.5, 2.6}, {64, 4, 0.35, 0.19, 2.5, 0.8}};
+constexpr TileTime kTimes16[] = {{256, 1, 1.5, 1.5, 9, 9}, {128, 2, 0.7, 0.44, 4.5, 2.6}, {64, 4, 0.35, 0.19, 2.5, 0.8}};
 constexpr TileTime kTimes32[] = {{128, 2, 1.75, 1.34, 5, 3.5}, {64, 4, 0.85, 0.455, 3, 1.2}};
 
 // The tile and the split of K that the table says are fastest.  trans: operands that lie transposed
@@ -861,7 +935,13 @@ void run_cols(ColArgs c, float* part, hipStream_t st) {
   c.groups = col_groups(c.m, c.n, c.r, Tr::kBytes);
   c.chunk_blocks = (int)cdiv(c.n, 32 * (16 / Tr::kBytes));
   c.part = c.out && c.groups > 1 ? part : nullptr;
-  hipLaunchKernelGGL(cols_kernel<Tr>, dim3((unsigned)(c.chunk_blocks * (int64_t)c.r), (unsigned)c.groups), dim3(256), 0, st, c);
+  const dim3 grid((unsigned)(c.chunk_blocks * (int64_t)c.r), (unsigned)c.groups);
+  switch (c.act) {
+    case YK_TOK_GELU: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_GELU>), grid, dim3(256), 0, st, c); break;
+    case YK_TOK_SILU: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_SILU>), grid, dim3(256), 0, st, c); break;
+    case YK_TOK_RELU: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_RELU>), grid, dim3(256), 0, st, c); break;
+    default: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_NONE>), grid, dim3(256), 0, st, c);
+  }
   if (c.part)
     hipLaunchKernelGGL(cols_sum_kernel, dim3((unsigned)cdiv((int64_t)c.r * c.n, 64)), dim3(1024), 0, st, c);
 }
