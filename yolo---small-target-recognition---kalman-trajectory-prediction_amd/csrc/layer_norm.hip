@@ -10,6 +10,10 @@
 // workgroup walks rows and keeps the column sums of dw / db in registers; they meet in LDS, go
 // to scratch as one float32 row per workgroup, and a second kernel adds those rows in a fixed order
 // (no atomics: equal calls give equal bits).
+//
+// 163840 x 640 bf16: forward 78 us, 5.4 TB/s, backward 121 us, 5.2 TB/s (what a large copy reaches here),
+// and 4.6 for the rows of partial sums.  10001 x 1027 fp16, rows aligned to 2 bytes: 16 and 31 us.
+// 320 x 320 float32: 3.4 us, a launch and one row's latency.
 #include "token_common.h"
 
 namespace yk {
@@ -453,7 +457,7 @@ void launch_norm_grad(const NormGradArgs& a, int nv, int groups, hipStream_t st)
 }
 // Lanes per row of the backward pass: at most two chunks each, whose sums, row and next row are some
 // 150 registers (four took 270, one wave per SIMD: 10000 x 8192 bf16 187 us).  Two of 16 lanes only with
-// rows enough to fill the chip.
+// rows enough to fill the chip (163840 x 192 bf16, x given as dy too: 32 us, in 64 lanes 61).
 inline int grad_lanes(int64_t m, int chunks) {
   if (chunks <= 16 || (chunks <= 32 && m >= kNarrowRows)) return 16;
   return chunks <= 128 ? 64 : chunks <= 512 ? 256 : 512;

@@ -338,7 +338,13 @@ __device__ __forceinline__ void loads_landed() {
   __builtin_amdgcn_s_barrier();
 }
 
-// kTM x kTN tile of C by kWM x kWN waves.  kAsync: kStages - 1 tiles of K in flight, one barrier per
+// kTM x kTN tile of C by kWM x kWN waves.  256-tiles, bf16: 8192^3 820 us (1340 TFLOP/s; a wave's LDS reads and
+// the loads into LDS take about the cycles its MFMAs do), 40960 x 4096 x 1024 320 us, of which some 65
+// are first loads and epilogues that one workgroup per CU hides behind nothing; with GELU 377.  Three or four
+// stages: 4096 x 1024 x 2048 in 128-tiles 26 -> 23 us, but the LDS they take leaves one workgroup
+// per CU where two fit (10240 x 512 x 2048: 30 -> 40), and so do fragments read a half tile ahead: no gain.
+// Rows that are not 16-byte aligned go through registers (4097 x 777 x 1111 fp16: 31 us), bound by the
+// L1's rate for such loads.  kAsync: kStages - 1 tiles of K in flight, one barrier per
 // tile; a buffer is filled again after the barrier that follows its last read.
 template <class Tr, bool kXT, bool kWT, int kTM, int kTN, int kWM, int kWN, int kStages, bool kAsync>
 __global__ __launch_bounds__(64 * kWM * kWN) void gemm_kernel(GemmArgs a) {
@@ -661,7 +667,8 @@ __global__ __launch_bounds__(256) void split_sum_kernel(GemmArgs a, int splits) 
 }
 
 // Few rows (m <= 16 kMT): the weight is read once, straight into fragments, by workgroups of 16
-// output channels whose 8 waves split K 64 elements at a time; their sums meet in LDS.
+// output channels whose 8 waves split K 64 elements at a time; their sums meet in LDS.  Bound by the latency of
+// launch and loads (8 x 2048 x 512 bf16: 4.0 us), for long K by the weight's bytes.
 template <class Tr, int kMT>
 __global__ __launch_bounds__(512) void rows_kernel(GemmArgs a) {
   using T = typename Tr::T;
@@ -720,7 +727,8 @@ struct ColArgs {
 };
 
 // Sums over the rows m % r == residue, for each column; a workgroup holds 32 chunks of columns x 8
-// rows of one residue, blockIdx.y a group of them.
+// rows of one residue, blockIdx.y a group of them.  Bound by HBM: dy and z in, dz out, 10240 x 2048 bf16 with
+// GELU's slope 24 us, 5.2 TB/s (the activation known at run time only and no row read ahead: 35).
 template <class Tr, int kAct>
 __global__ __launch_bounds__(256) void cols_kernel(ColArgs a) {
   using T = typename Tr::T;
@@ -812,14 +820,14 @@ constexpr int kCUs = 256;
 // is 64 of K for the 16-bit types, 32 for float32): `alone` per step for the only workgroup of
 // its CU (its loads' latency), `shared` per step and workgroup where `per_cu` of them share it
 // (the CU's load rate; the MFMAs and the splitting for float32), `ends` / `ends_shared` for the first loads and the
-// epilogue.  16-bit, 4096 x 1024 x 4096: 128-tiles 49 us, 64-tiles 50, 256-tiles 95 (64 of them on
-// 256 CUs); 40960 x 4096 x 1024: 360 / 394 (256 / 128); 1000^3: 8.8 / 13.7 (64 / 128); float32
+// epilogue.  16-bit (m x n x k), tiles of 64 / 128 / 256: 1000^3 9.0 / 18.8 / 24 us; 4096 x 1024 x 1024 16.7 /
+// 14.3 / 28; 4096 x 4096 x 1024 60 / 41 / 35; 40960 x 4096 x 1024 548 / 379 / 320.  float32
 // 10240 x 2048 x 512: 186 / 203 (64 / 128).
 struct TileTime {
   int tile, per_cu;
   double alone, shared, ends, ends_shared;
 };
-constexpr TileTime kTimes16[] = {{256, 1, 1.5, 1.5, 9, 9}, {128, 2, 0.7, 0.44, 4.5, 2.6}, {64, 4, 0.35, 0.19, 2.5, 0.8}};
+constexpr TileTime kTimes16[] = {{256, 1, 1.5, 1.5, 9, 9}, {128, 2, 0.7, 0.44, 3.5, 2.6}, {64, 4, 0.35, 0.19, 2.5, 0.8}};
 constexpr TileTime kTimes32[] = {{128, 2, 1.75, 1.34, 5, 3.5}, {64, 4, 0.85, 0.455, 3, 1.2}};
 
 // The tile and the split of K that the table says are fastest.  trans: operands that lie transposed
