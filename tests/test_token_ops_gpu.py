@@ -529,3 +529,12 @@ def test_linear_whole_and_partial_tiles(ops, dt, act, m, k, n):
     dy = rn(m, n, dt=dt, seed=3)
     for (want, e), g, name in zip(R.linear_grads(dy, x, w, act, z), ops.linear_backward(dy, x, w, b, act=act, preact=z), ("dx", "dw", "db")):
         R.check(g, want, R._final(want, e, b.dtype) if name == "db" else e, f"{name} {act}")
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("b,nq,nk,h,hk,dd", [(2, 100, 2300, 4, 2, 72), (1, 150, 2111, 2, 2, 33), (2, 300, 3100, 1, 1, 128)])
+def test_attention_row_blocks_with_split_keys(ops, dt, causal, b, nq, nk, h, hk, dd):
+    """Too few row blocks to fill the chip: their keys in ranges, joined."""
+    run_attention(ops, dt, b, nq, nk, h, hk, dd, causal)
+    run_attention(ops, dt, b, nq, nk, h, hk, dd, causal, lengths=[nk - 5, 70][:b], q_lengths=[nq - 1, nq][:b])

@@ -26,7 +26,7 @@ struct AttnArgs {
   float* lse;         // [b][hq][nq]
   const int32_t *q_lengths, *lengths;
   int64_t qs[3], ks[3], vs[3], os[3], gos[3], dqs[3], dks[3], dvs[3];
-  float* part;        // split: [item][split][16][d_pad + 4]; backward: lse2, delta [b][hk][rows]
+  float* part;        // keys split: [16 rows][split][16][d_pad + 4] (sums, exponents' reference, denominator); backward: lse2, delta [b][hk][rows]
   float* kv_part;     // backward, rows split: [split][b * hk * nk][dk, dv: 2 d_pad]
   float* q_part;      // backward, keys split: [split][b * hk * rows][d_pad]
   float scale;
@@ -344,7 +344,16 @@ __device__ __forceinline__ int key_end(const AttnArgs& a, const Seq& s, int r0, 
   return i + s.off + 1;
 }
 
-// Forward: 4 waves of 16 kNT rows.  Bound by issue: per block and lane 32 kNT exponentials, their sums and
+// Range blockIdx.y of the keys [0, k_stop), in whole blocks.
+template <int kBN>
+__device__ __forceinline__ void key_range(int& k_begin, int& k_stop) {
+  const int end = k_stop > 0 ? k_stop : 0, per = ((end + kBN - 1) / kBN + (int)gridDim.y - 1) / (int)gridDim.y * kBN;
+  k_begin = (int)blockIdx.y * per < end ? (int)blockIdx.y * per : end;
+  k_stop = end - k_begin < per ? end : k_begin + per;
+}
+
+// Forward: 4 waves of 16 kNT rows; with few row blocks, blockIdx.y a range of the keys, whose sums
+// attn_join_rows_kernel joins.  Bound by issue: per block and lane 32 kNT exponentials, their sums and
 // conversions next to the MFMAs, neither of which hides the other wholly with two waves per SIMD.
 // bf16, 4 x 5120 x 5120, 8 heads of 64: 260 us, 826 TFLOP/s; 8 x 1280 x 1280, 8 heads of 40 (computed as
 // 64): 39 us.
@@ -380,9 +389,11 @@ __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_kernel(AttnArgs a
   }
   const float sl2 = a.scale * kLog2e;
   Feed<Tr, kDP, kAsync> fk, fv;
-  fk.init(a.k, a.ks, b, hk, 1, a.d, 0);
-  fv.init(a.v, a.vs, b, hk, 1, a.d, 0);
-  for_blocks<Tr, kDP, kAsync>(fk, fv, 0, key_end(a, s, r0, kRows), s.klen, lds, kBuf, [](char*, int) {}, [&](const char* lk, int k0) {
+  int k_begin = 0, k_stop = key_end(a, s, r0, kRows);
+  if (gridDim.y > 1) key_range<Bl::kBN>(k_begin, k_stop);
+  fk.init(a.k, a.ks, b, hk, 1, a.d, k_begin);
+  fv.init(a.v, a.vs, b, hk, 1, a.d, k_begin);
+  for_blocks<Tr, kDP, kAsync>(fk, fv, k_begin, k_stop, s.klen, lds, kBuf, [](char*, int) {}, [&](const char* lk, int k0) {
     const char* lv = lk + Bl::kBytesAll;
     f32x4 st[kNT][kKT];
 #pragma unroll
@@ -420,6 +431,17 @@ __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_kernel(AttnArgs a
     const int r = r0 + (wave * kNT + j) * 16 + l16;
     const float sum = column_sum(l[j]);
     if (r >= a.rows) continue;
+    if (gridDim.y > 1) {
+      const int64_t at = ((int64_t)bh * ((a.rows + 15) / 16) + r / 16) * gridDim.y + blockIdx.y;
+      float* part = a.part + (at * 16 + r % 16) * (kDP + 4);
+#pragma unroll
+      for (int t = 0; t < kDT; ++t) *(f32x4*)(part + t * 16 + g * 4) = acc[j][t];
+      if (g == 0) {
+        part[kDP] = m[j];
+        part[kDP + 1] = sum;
+      }
+      continue;
+    }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T* o = row_ptr((T*)a.out, a.os, b, hk, a.group, r);
 #pragma unroll
@@ -625,6 +647,33 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int row_bloc
   if (a.lse && e == 0) {
     const int i = query_of(r, a.group);
     a.lse[((int64_t)(b * a.hk + hk) * a.group + (r - i * a.group)) * a.nq + i] = ll == 0.f ? -INFINITY : fmaf(mm, kLn2, logf(ll));
+  }
+}
+
+// The same for many rows in few ranges: 4 elements of a row per thread.
+template <class Tr>
+__global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnArgs a, int dp) {
+  using T = typename Tr::T;
+  const int per = dp / 4, c = threadIdx.x % per;
+  const int64_t all = (int64_t)a.b * a.hk * a.rows, id = (int64_t)blockIdx.x * (256 / per) + threadIdx.x / per;
+  if (threadIdx.x >= 256 / per * per || id >= all) return;
+  const int bh = (int)(id / a.rows), r = (int)(id - (int64_t)bh * a.rows), b = bh / a.hk, hk = bh - b * a.hk;
+  const int64_t step = (int64_t)16 * (dp + 4);
+  const float* p = a.part + ((int64_t)bh * ((a.rows + 15) / 16) + r / 16) * a.splits * step + (r % 16) * (dp + 4);
+  float mm = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, p[s * step + dp]);
+  const float ref = mm == -INFINITY ? 0.f : mm;
+  float ll = 0.f;
+  f32x4 v{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) {
+    const float f = exp2_f(p[s * step + dp] - ref);
+    ll += p[s * step + dp + 1] * f;
+    v += *(const f32x4*)(p + s * step + c * 4) * f;
+  }
+  store_out<Tr>(row_ptr((T*)a.out, a.os, b, hk, a.group, r), c * 4, a.d, v * (ll == 0.f ? 0.f : 1.f / ll));
+  if (a.lse && c == 0) {
+    const int i = query_of(r, a.group);
+    a.lse[((int64_t)bh * a.group + (r - i * a.group)) * a.nq + i] = ll == 0.f ? -INFINITY : fmaf(mm, kLn2, logf(ll));
   }
 }
 
@@ -874,13 +923,8 @@ __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_dq_kernel(AttnArg
   }
   const float sl2 = a.scale * kLog2e;
   Feed<Tr, kDP, kAsync> fk, fv;
-  const int k_end = key_end(a, s, r0, kRows);
-  int k_begin = 0, k_stop = k_end;
-  if (gridDim.y > 1) {
-    const int per = ((k_end + Bl::kBN - 1) / Bl::kBN + (int)gridDim.y - 1) / (int)gridDim.y * Bl::kBN;
-    k_begin = (int)blockIdx.y * per < k_end ? (int)blockIdx.y * per : k_end;
-    k_stop = k_end - k_begin < per ? k_end : k_begin + per;
-  }
+  int k_begin = 0, k_stop = key_end(a, s, r0, kRows);
+  if (gridDim.y > 1) key_range<Bl::kBN>(k_begin, k_stop);
   fk.init(a.k, a.ks, b, hk, 1, a.d, k_begin);
   fv.init(a.v, a.vs, b, hk, 1, a.d, k_begin);
   for_blocks<Tr, kDP, kAsync>(fk, fv, k_begin, k_stop, s.klen, lds, kBuf, [](char*, int) {}, [&](const char* lk, int k0) {
@@ -952,15 +996,22 @@ inline int pad_d(int d) { return (d + 31) / 32 * 32; }
 // only, 775 against 1018 us for 4 x 4096 x 16 heads; up to 64 one tile is as fast, and faster where
 // rows are causal or few (8 x 1280 x 8 heads of 40: 72 against 80), at 128 two do not fit
 inline bool two_tiles(int64_t bh, int64_t n) { return bh * cdiv(n, 128) >= kCUs; }
-// Key ranges of the few-rows kernel; 0: the block kernel takes the call.  Two workgroups per CU, and
-// at least four slabs for each wave of one.
-inline int split_count(int64_t bh, int64_t rows, int64_t nk) {
-  const int64_t wgs = bh * cdiv(rows, 64), items = bh * cdiv(rows, 16);
-  if (rows > 32 && (wgs >= kCUs / 2 || nk < 512)) return 0;
-  int64_t s = cdiv(2 * kCUs, items);
-  const int64_t most = cdiv(nk, 512);
-  if (s > most) s = most;
-  return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+// Rows of a key head that attn_split_kernel takes (128 rows against 16384 keys: 13.6 us, in row blocks 42; from there
+// on the row blocks, which share their keys' reads, are as many).
+constexpr int64_t kFewRows = 128;
+// Key ranges of the forward pass.  Few rows: two workgroups per CU, and at least four slabs for each wave of
+// one.  Else one where the workgroups fill the chip, or as many as fill it twice, of 16 blocks at least
+// (bf16, 8192 x 8192, one head of 64: 77 us whole, 37 in four; 1280 x 1280, 8 heads: 16 whole, 19 in two of 10).
+inline int split_count(int bytes, int64_t bh, int64_t rows, int64_t nk) {
+  int64_t s;
+  if (rows <= kFewRows) {
+    s = cdiv(2 * kCUs, bh * cdiv(rows, 16));
+    const int64_t most = cdiv(nk, 512);
+    return (int)(s > most ? most > 1 ? most : 1 : s > 256 ? 256 : s);
+  }
+  const int64_t wgs = bh * cdiv(rows, 64), most = cdiv(nk, 128 / bytes) / 16;
+  s = wgs < kCUs ? cdiv(2 * kCUs, wgs) : 1;
+  return (int)(s > most ? most > 1 ? most : 1 : s > 64 ? 64 : s);
 }
 
 // What Feed's kAsync needs of one operand: chunks whole and on 16-byte boundaries, a block's offsets
@@ -1002,7 +1053,10 @@ void run_split(const AttnArgs& a, hipStream_t st) {
 template <class Tr, int kDP, int kNT, bool kAsync = true>
 void launch_fwd(const AttnArgs& a, hipStream_t st) {
   const int rb = (int)cdiv(a.rows, 64 * kNT);
-  hipLaunchKernelGGL((attn_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * rb)), dim3(256), 0, st, a, rb);
+  hipLaunchKernelGGL((attn_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * rb), a.splits), dim3(256), 0, st, a, rb);
+  if (a.splits > 1)
+    hipLaunchKernelGGL(attn_join_rows_kernel<Tr>, dim3((unsigned)cdiv((int64_t)a.b * a.hk * a.rows, 256 / (kDP / 4))), dim3(256), 0, st,
+                       a, kDP);
 }
 template <class Tr, int kDP, int kNT, bool kAsync = true>
 void launch_dkv(const AttnArgs& a, hipStream_t st) {
@@ -1047,7 +1101,7 @@ void run_bwd(const AttnArgs& a, hipStream_t st) {
 
 template <class Tr>
 void run_attn(const AttnArgs& a, bool bwd, hipStream_t st) {
-  if (!bwd && a.splits) {
+  if (!bwd && a.rows <= kFewRows) {
     switch (pad_d(a.d)) {
       case 32: run_split<Tr, 32>(a, st); break;
       case 64: run_split<Tr, 64>(a, st); break;
@@ -1105,7 +1159,7 @@ int yk_attention_workspace(const yk_attention_args* a, int64_t* bytes) {
   const int64_t bh = (int64_t)a->b * a->h_kv, rows = a->nq * (a->h_q / a->h_kv);
   *bytes = 0;
   if (bh == 0 || rows == 0) return YK_OK;
-  const int s = split_count(bh, rows, a->nk);
+  const int s = split_count(tok_bytes(a->dtype), bh, rows, a->nk);
   if (s > 1) *bytes = bh * cdiv(rows, 16) * s * 16 * (pad_d(a->d) + 4) * 4;
   return YK_OK;
 }
@@ -1123,7 +1177,7 @@ int yk_attention(yk_ctx* ctx, const yk_attention_args* a, void* stream) {
   AttnArgs k = common_args(a);
   k.out = (char*)a->o;
   k.lse = a->lse;
-  k.splits = split_count((int64_t)k.b * k.hk, k.rows, k.nk);
+  k.splits = split_count(tok_bytes(a->dtype), (int64_t)k.b * k.hk, k.rows, k.nk);
   if (k.splits > 1 && !a->ws) k.splits = 1;
   const hipStream_t st = (hipStream_t)stream;
   if (a->dtype == YK_ACT_F32) run_attn<F32>(k, false, st);
