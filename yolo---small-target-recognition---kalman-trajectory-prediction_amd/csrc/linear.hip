@@ -441,7 +441,8 @@ __global__ __launch_bounds__(64 * kWM * kWN) void gemm_kernel(GemmArgs a) {
 // (rounded to nearest, so |x1| <= 2^-9 |x| and |x2| <= 2^-18 |x|), and six of the nine products are
 // summed: w0x0, w0x1, w1x0, w1x1, w0x2, w2x0.  bf16 products are exact in float32 and what is left out
 // is below 2^-25 |w x|, less than one float32 rounding; six 16-cycle MFMAs per 32 of K replace eight
-// 32-cycle float32 ones.  4096 x 1024 x 4096: 188 us, 267 on v_mfma_f32_16x16x4_f32.
+// 32-cycle float32 ones.  (A part below bf16's normal range, of an operand below some 2^-110, may be
+// flushed.)  4096 x 1024 x 4096: 188 us, 267 on v_mfma_f32_16x16x4_f32.
 //
 // The parts are made once per tile, between the global loads' registers and LDS (three planes a
 // side), not by every wave that reads them.  A tile is 32 of K:
