@@ -5129,8 +5129,7 @@ int yk_detect_graph(yk_model* m, const uint8_t* frames, int batch, float conf, f
     }
     // Capture stream: one per model, kept for the model's lifetime (round 4 created one per
     // capture and destroyed it after hipStreamEndCapture, and multi-lane graphs then crashed in
-    // hipGraphLaunch once several models were alive; tools/graph_fork_repro.hip did not reproduce
-    // that in either form).  Which stream a graph is captured on moves the launch rate through
+    // hipGraphLaunch once several models were alive).  Which stream a graph is captured on moves the launch rate through
     // the streams' hardware-queue mapping, not through the graph: capturing on the launch stream
     // (YK_CAP_STREAM=launch) or on a temporary stream (=destroy) measured 4-11 % slower on the
     // host-frame bench lines with one created stream per slot (gpurun_out/r6i: config 3

@@ -147,7 +147,7 @@ class StreamPipeline:
         if self.D > 1:
             # forwards in flight are the concurrency: one lane per graph (bench.py's default too).
             # Multi-lane (forked) graphs of several in-flight slots plus other live models were
-            # seen to crash the HIP runtime inside hipGraphLaunch (tools/graph_lanes_repro.py, round 4)
+            # seen to crash the HIP runtime inside hipGraphLaunch
             self.set_schedule(1, 1)
         self.gmd = None
         if motion_method is not None:
