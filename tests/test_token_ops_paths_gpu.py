@@ -1,0 +1,44 @@
+"""The token operators (ops.py) on the GPU where their other tests do not reach: gradients at the ends of
+fp16's range.  Element by element against float64 within the bounds of token_helpers.py."""
+import pytest
+import torch
+
+import token_helpers as R
+from conftest import pkg
+
+pytestmark = pytest.mark.gpu
+DT = R.DTYPES
+
+
+@pytest.fixture(scope="module")
+def ops():
+    return pkg().ops
+
+
+def rn(*shape, dt="fp32", std=1.0, seed=0):
+    g = torch.Generator().manual_seed(seed + sum((i + 1) * s for i, s in enumerate(shape)))
+    return (torch.randn(*shape, generator=g) * std).to(DT[dt]).cuda()
+
+
+# ---- attention's gradients in fp16 -------------------------------------------------------------
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("b,nq,nk,h,hk,dd,sq,sk,sv,sg,scale", [
+    (1, 40, 8192, 1, 1, 8, 0.01, 100, 1, 6e-5, 1.0),      # dS of 2e-8: what fp16 rounds to 0
+    (1, 8192, 4096, 1, 1, 8, 100, 0.01, 1, 6e-5, 1.0),    # the same for sums over rows
+    (1, 3, 81920, 2, 1, 8, 1, 1, 1, 10, None),            # P of 1e-5: dv of few rows
+    (2, 100, 40, 6, 3, 64, 0.01, 0.01, 60, 2000, None),   # dS past 65504, gradients that fit
+    (4, 515, 515, 16, 16, 96, 0.3, 0.3, 1, 1e-4, None),   # two tiles a wave
+])
+def test_attention_backward_keeps_fp16s_digits(ops, causal, b, nq, nk, h, hk, dd, sq, sk, sv, sg, scale):
+    """P and dS enter a 16-bit product each with half a step of its own value, small or large.  The
+    kernels take powers of two out of both: half of fp16's subnormal step is 2^-40 of P, and of dS at
+    most 2^-34 of its column's largest, which here is below 2^-6, and below 2^17 where dS is large."""
+    q, k, v, do = (rn(b, n, hh, dd, dt="fp16", std=s, seed=i)
+                   for i, (n, hh, s) in enumerate(((nq, h, sq), (nk, hk, sk), (nk, hk, sv), (nq, h, sg))))
+    ref = R.attention(q, k, v, scale, causal, do=do, grad_tiny=(2.0 ** -40, 2.0 ** -40 if sg < 100 else 2.0 ** -17))
+    o, lse = ops.attention(q, k, v, scale=scale, causal=causal, return_lse=True)
+    got = ops.attention_backward(do, q, k, v, o, lse, scale=scale, causal=causal)
+    again = ops.attention_backward(do, q, k, v, o, lse, scale=scale, causal=causal)
+    for name, g, a in zip(("dq", "dk", "dv"), got, again):
+        R.check(g, *ref[name], name)
+        assert torch.equal(g, a)

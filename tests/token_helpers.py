@@ -150,14 +150,14 @@ def layer_norm_grads(dy, x, w, eps):
 
 
 # ---- attention ---------------------------------------------------------------------------------
-def attention(q, k, v, scale=None, causal=False, lengths=None, q_lengths=None, do=None):
+def attention(q, k, v, scale=None, causal=False, lengths=None, q_lengths=None, do=None, grad_tiny=(TINY, TINY)):
     """{"o": (o, bound), "lse": .., "dq": .., "dk": .., "dv": ..} by batch element and head.
 
     A score is off by es = (D + 8) f scale sum|q k| + 4 f |s| (its product, the scaling into a
     power of two, the maximum subtracted); P relatively by es of its row's largest, twice (numerator
     and denominator), n f for the denominator's sum and 8 f per key block for the rescaling; for the
     16-bit types the P and dS that enter a product are rounded once more (u, TINY in fp16's subnormal
-    range).  delta inherits o's bound."""
+    range; the backward pass's own, of P and of dS: grad_tiny).  delta inherits o's bound."""
     dt, u = q.dtype, half_step(q.dtype)
     b, nq, h, dd = q.shape
     nk, hk = k.shape[1], k.shape[2]
@@ -205,10 +205,11 @@ def attention(q, k, v, scale=None, causal=False, lengths=None, q_lengths=None, d
             delta = (G * O).sum(1, keepdim=True)
             edelta = (G.abs() * fO).sum(1, keepdim=True) + (dd + 8) * F * (G.abs() * (O.abs() + fO)).sum(1, keepdim=True)
             relP = es + rel + torch.where(seen, 8 * F * (L.abs() + 1), torch.zeros_like(L))
-            eP = P * (relP + u) + tiny
+            tP, tS = ((~hid).double() * (t if u else 0) for t in grad_tiny)
+            eP = P * (relP + u) + tP
             dS = P * (dP - delta)
             edS = P * ((relP + 2 * F) * (dP - delta).abs() + edP + edelta)
-            edS = edS + u * (dS.abs() + edS) + tiny
+            edS = edS + u * (dS.abs() + edS) + tS
             dQ, dK, dV = scale * (dS @ K), scale * (dS.t() @ Q), P.t() @ G
             n = kl + ql + 16
             add = {"dq": (i, slice(0, ql), j), "dk": (i, slice(0, kl), j // rep), "dv": (i, slice(0, kl), j // rep)}
