@@ -1,7 +1,8 @@
 """The token operators (ops.py) on the GPU where their other tests do not reach: gradients at the ends of
-fp16's range.  Element by element against float64 within the bounds of token_helpers.py."""
+fp16's range, refusals.  Element by element against float64 within the bounds of token_helpers.py."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import token_helpers as R
 from conftest import pkg
@@ -42,3 +43,31 @@ def test_attention_backward_keeps_fp16s_digits(ops, causal, b, nq, nk, h, hk, dd
     for name, g, a in zip(("dq", "dk", "dv"), got, again):
         R.check(g, *ref[name], name)
         assert torch.equal(g, a)
+
+
+# ---- refusals ------------------------------------------------------------------------------------
+def test_forward_mode_tangents_are_refused(ops):
+    """A tangent would be lost without a word: every argument that carries one is refused."""
+    x, w, b = rn(4, 8), rn(8, 8), rn(8)
+    q, o = rn(1, 4, 2, 8), rn(1, 4, 2, 8)
+    lse, m = rn(1, 2, 4), rn(4)
+    calls = [(ops.linear, (x, w, b), {"residual": x}), (ops.linear_backward, (x, x, w, b), {"act": "gelu", "preact": x, "residual": x}),
+             (ops.layer_norm, (x, b, b), {}), (ops.layer_norm_backward, (x, x, b, m, m), {}),
+             (ops.attention, (q, q, q), {}), (ops.attention_backward, (q, q, q, q, o, lse), {})]
+    with forward_ad.dual_level():
+        for f, args, kw in calls:
+            f(*args, **kw)  # nothing carries one
+            for i, t in enumerate(args):
+                d = forward_ad.make_dual(t, torch.ones_like(t))
+                with pytest.raises(ValueError, match="tangent"):
+                    f(*args[:i], d, *args[i + 1:], **kw)
+            for n, t in kw.items():
+                if isinstance(t, torch.Tensor):
+                    with pytest.raises(ValueError, match="tangent"):
+                        f(*args, **{**kw, n: forward_ad.make_dual(t, torch.ones_like(t))})
+
+
+def test_tracing_is_refused(ops):
+    x, w = rn(4, 8), rn(6, 8)
+    with pytest.raises(pkg().YKError, match="jit.trace"):
+        torch.jit.trace(lambda t: ops.linear(t, w), (x,))

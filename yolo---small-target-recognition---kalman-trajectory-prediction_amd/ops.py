@@ -5,8 +5,9 @@ The kernels are those the detector program runs for an ``AIFI`` row of a model Y
 here they take torch tensors (float32, bfloat16 or float16, on one GPU).  Calls are enqueued on
 the tensors' device's current stream, allocate their outputs and scratch from torch and never
 synchronise, so they can be captured into a graph.  No autograd graph is built: a call whose
-inputs require gradients raises while gradients are enabled, and the ``*_backward`` functions return
-the gradients.  Sums are float32 and outputs are rounded once; equal calls give equal bits.
+inputs require gradients (while gradients are enabled) or carry a forward-mode tangent raises, and so
+does one under torch.jit.trace, which would record its empty outputs; the ``*_backward`` functions
+return the gradients.  Sums are float32 and outputs are rounded once; equal calls give equal bits.
 
 A tensor's last dimension must be contiguous; what precedes it must step evenly from row to row
 (any row stride, so a channel slice of a wider tensor is fine).  Anything else raises ValueError.
@@ -17,13 +18,14 @@ import ctypes as C
 import struct
 
 import torch
+from torch.autograd import forward_ad as _fwd
 
 from . import _lib as L
 
 ACTS = {"none": 0, "silu": 1, "gelu": 2, "relu": 3}
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 3}  # yk_act_dtype
 _F32 = torch.float32
-_empty, _empty_like, _grad_enabled = torch.empty, torch.empty_like, torch.is_grad_enabled
+_empty, _empty_like, _grad_enabled, _tracing = torch.empty, torch.empty_like, torch.is_grad_enabled, torch._C._is_tracing
 
 # The C argument structs as packed bytes (a ctypes struct costs three times as long to fill); the
 # last two fields, scratch and its size, are appended once the size is known.
@@ -44,18 +46,23 @@ def _input(t, name):
     """The operator's first tensor: sets the type and the GPU.  Returns (yk_act_dtype, device index)."""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor")
+    if _tracing():
+        raise L.YKError("torch.jit.trace records torch operations only: this call's result would be an empty tensor")
     code = _DTYPES.get(t.dtype)
     if code is None:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
     if not t.is_cuda:
         raise L.YKError(f"{name} is on {t.device}: the token operators run on an AMD GPU only (no CPU fallback)")
-    if t.requires_grad and _grad_enabled():
-        _needs_no_grad(name)
+    if t.requires_grad or _fwd._current_level >= 0:
+        _no_derivative(t, name)
     return code, t.get_device()
 
 
-def _needs_no_grad(name):
-    raise ValueError(f"{name} requires grad: no autograd graph is built here (detach it, or torch.no_grad())")
+def _no_derivative(t, name):
+    if t.requires_grad and _grad_enabled():
+        raise ValueError(f"{name} requires grad: no autograd graph is built here (detach it, or torch.no_grad())")
+    if _fwd.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} has a forward-mode tangent, which would be lost: pass unpack_dual({name}).primal")
 
 
 def _like(t, name, dev, dtype, other=None):
@@ -66,8 +73,8 @@ def _like(t, name, dev, dtype, other=None):
         raise ValueError(f"{name} is on {t.device}, expected cuda:{dev}")
     if t.dtype is not dtype and t.dtype is not other:
         raise ValueError(f"{name} has dtype {t.dtype}, expected {dtype}" + (f" or {other}" if other else ""))
-    if t.requires_grad and _grad_enabled():
-        _needs_no_grad(name)
+    if t.requires_grad or _fwd._current_level >= 0:
+        _no_derivative(t, name)
     return t
 
 
