@@ -1,5 +1,5 @@
 """The token operators (ops.py) on the GPU where their other tests do not reach: gradients at the ends of
-fp16's range, refusals.  Element by element against float64 within the bounds of token_helpers.py."""
+fp16's range, rows with exact means, refusals.  Element by element against float64 within the bounds of token_helpers.py."""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -43,6 +43,26 @@ def test_attention_backward_keeps_fp16s_digits(ops, causal, b, nq, nk, h, hk, dd
     for name, g, a in zip(("dq", "dk", "dv"), got, again):
         R.check(g, *ref[name], name)
         assert torch.equal(g, a)
+
+
+# ---- layer norm ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt,at", [("fp32", 1000.0), ("bf16", 144.0), ("fp16", 1000.0)])
+@pytest.mark.parametrize("m,c", [(3, 64), (300, 256), (5, 640), (4, 1024), (2, 8192), (2, 16384), (8200, 256)])
+def test_layer_norm_gradients_of_rows_with_exact_means(ops, dt, at, m, c):
+    """Rows of one value: the mean is that value (all sums are whole numbers below 2^24, c a divisor), so
+    x - mean is zero, y is the bias, and the weight's gradient, a sum of dy 0, is zero exactly; dx is
+    rstd (g - mean g), a sum of c terms and three roundings."""
+    x = torch.full((m, c), at, dtype=DT[dt], device="cuda")
+    w, b, dy = rn(c, std=0.1) + 1, rn(c, seed=1), rn(m, c, dt=dt, seed=2)
+    y, mean, rstd = ops.layer_norm(x, w, b, return_stats=True)
+    assert torch.equal(y, b.to(DT[dt]).expand(m, c))
+    dx, dw, db = ops.layer_norm_backward(dy, x, w, mean, rstd)
+    assert not dw.any()
+    g, r = dy.double() * w.double(), rstd.double()[:, None]
+    want = r * (g - g.mean(1, keepdim=True))
+    R.check(dx, want, R._final(want, r * ((c + 8) * R.F * g.abs().mean(1, keepdim=True) + 8 * R.F * (g.abs() + g.mean(1, keepdim=True).abs())),
+                               DT[dt]), "dx")
+    R.check(db, dy.double().sum(0), (m + 8) * R.F * dy.double().abs().sum(0), "db")
 
 
 # ---- refusals ------------------------------------------------------------------------------------

@@ -11,7 +11,7 @@
 // to scratch as one float32 row per workgroup, and a second kernel adds those rows in a fixed order
 // (no atomics: equal calls give equal bits).
 //
-// 163840 x 640 bf16: forward 78 us, 5.4 TB/s, backward 121 us, 5.2 TB/s (what a large copy reaches here),
+// 163840 x 640 bf16: forward 78 us, 5.4 TB/s, backward 122 us, 5.1 TB/s (what a large copy reaches here),
 // and 4.6 for the rows of partial sums.  10001 x 1027 fp16, rows aligned to 2 bytes: 16 and 31 us.
 // 320 x 320 float32: 3.4 us, a launch and one row's latency.
 #include "token_common.h"
@@ -248,7 +248,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_grad_kernel(NormGrad
   for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.m; row0 += step) {
     const int64_t row = row0 + sub;
     const bool live = row < a.m;
-    const float rstd = rstd_n, shift = -mean_n * rstd;
+    const float rstd = rstd_n, mean = mean_n;
     float h[NV * kEpc], g[NV * kEpc];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_grad_kernel(NormGrad
       for (int e = 0; e < kEpc; ++e) {
         const int k = i * kEpc + e;
         const float d = elem<Tr>(gn[i], e);
-        h[k] = fmaf(elem<Tr>(xn[i], e), rstd, shift);
+        h[k] = (elem<Tr>(xn[i], e) - mean) * rstd;  // (as forward: x rstd - mean rstd would round the offset's product)
         g[k] = d * (own_w ? elem<Tr>(w[i], e) : wf[e]);
         s1 += g[k];
         s2 = fmaf(g[k], h[k], s2);
