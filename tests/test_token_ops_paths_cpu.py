@@ -1,9 +1,14 @@
 """What the token operators refuse, where that shows without a GPU."""
+import ctypes as C
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 from conftest import pkg
+
+L = pkg()._lib
+CTX = C.create_string_buffer(64)  # never read: every call here is refused
 
 
 def test_forward_mode_tangents_are_refused():
@@ -21,3 +26,21 @@ def test_tracing_is_refused():
     for f in (lambda t: ops.linear(t, t), lambda t: ops.layer_norm(t)):
         with pytest.raises(pkg().YKError, match="jit.trace"):
             torch.jit.trace(f, (x,))
+
+
+@pytest.mark.parametrize("fn,args", [
+    ("yk_linear", dict(dtype=0, m=1 << 28, n=1 << 13, k=8, x=64, w=64, y=64, x_stride=8, w_stride=8, y_stride=1 << 13)),
+    ("yk_linear_backward", dict(dtype=0, m=1 << 28, n=8, k=1 << 13, dy=64, x=64, w=64, dx=64, dy_stride=8, x_stride=1 << 13,
+                                w_stride=1 << 13, dx_stride=1 << 13, ws=64, ws_bytes=1 << 50)),
+    ("yk_attention", dict(dtype=0, b=1 << 24, h_q=1, h_kv=1, d=8, nq=1, nk=9, scale=1.0, q=64, k=64, v=64, o=64)),
+    ("yk_attention", dict(dtype=1, b=1 << 20, h_q=2, h_kv=2, d=8, nq=513, nk=9, scale=1.0, q=64, k=64, v=64, o=64)),
+    ("yk_attention_backward", dict(dtype=0, b=1 << 20, h_q=2, h_kv=2, d=8, nq=129, nk=9, scale=1.0, q=64, k=64, v=64, o=64, go=64,
+                                   lse=64, dq=64, dk=64, dv=64, ws=64, ws_bytes=1 << 50)),
+    ("yk_attention_backward", dict(dtype=0, b=1 << 20, h_q=2, h_kv=2, d=8, nq=1, nk=513, scale=1.0, q=64, k=64, v=64, o=64, go=64,
+                                   lse=64, dq=64, dk=64, dv=64, ws=64, ws_bytes=1 << 50)),
+])
+def test_more_workgroups_than_a_launch_holds(fn, args):
+    """A launch holds fewer than 2^32 threads: refused with nothing launched."""
+    a = L.TOKEN_ARGS[fn](**args)
+    assert getattr(L.lib(), fn)(C.addressof(CTX), C.byref(a), None) == L.YK_ERR_ARG
+    assert b"than a launch holds" in L.lib().yk_last_error()

@@ -1,5 +1,6 @@
 """The token operators (ops.py) on the GPU where their other tests do not reach: gradients at the ends of
-fp16's range, rows with exact means, refusals.  Element by element against float64 within the bounds of token_helpers.py."""
+fp16's range, rows with exact means, more
+rows than one launch holds, refusals.  Element by element against float64 within the bounds of token_helpers.py."""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -63,6 +64,37 @@ def test_layer_norm_gradients_of_rows_with_exact_means(ops, dt, at, m, c):
     R.check(dx, want, R._final(want, r * ((c + 8) * R.F * g.abs().mean(1, keepdim=True) + 8 * R.F * (g.abs() + g.mean(1, keepdim=True).abs())),
                                DT[dt]), "dx")
     R.check(db, dy.double().sum(0), (m + 8) * R.F * dy.double().abs().sum(0), "db")
+
+
+# ---- more workgroups than one launch holds ---------------------------------------------------------
+def test_layer_norm_of_more_rows_than_a_launch_holds(ops):
+    """2^28 rows of 16 per workgroup of 256 threads: parts, each row the bits of a smaller call."""
+    m, c = 2 ** 28 + 37, 8
+    x = rn(2 ** 16 + 3, c, dt="bf16").repeat(m // (2 ** 16 + 3) + 1, 1)[:m]
+    w, b = rn(c, seed=1), rn(c, seed=2)
+    y, mean, rstd = ops.layer_norm(x, w, b, return_stats=True)
+    for lo, hi in ((0, 2 ** 20), (2 ** 28 - 5000, m)):
+        got = ops.layer_norm(x[lo:hi], w, b, return_stats=True)
+        for g, t in zip(got, (y, mean, rstd)):
+            assert torch.equal(g, t[lo:hi])
+    want, e = R.layer_norm(x[-99:], w, b, 1e-5)
+    R.check(y[-99:], want, e, "y")
+
+
+def test_residual_gradient_of_more_rows_than_a_launch_holds(ops):
+    r, n = 2 ** 24 + 3, 16
+    dy = rn(2 ** 16 + 1, n, dt="bf16").repeat(r // (2 ** 16 + 1) + 1, 1)[:r + 5]
+    x, w = torch.zeros(r + 5, 1, dtype=dy.dtype, device="cuda"), rn(n, 1, dt="bf16")
+    dres = ops.linear_backward(dy, x, w, residual=dy[:r])[3]
+    assert torch.equal(dres[5:], dy[5:r])
+    assert torch.equal(dres[:5], (dy[:5].float() + dy[r:].float()).to(dy.dtype))
+
+
+def test_few_rows_of_more_columns_than_a_launch_holds(ops):
+    n = 2 ** 27 + 5
+    x, w = rn(2, 1, dt="bf16"), rn(2 ** 16 + 1, 1, dt="bf16").repeat(n // (2 ** 16 + 1) + 1, 1)[:n]
+    y = ops.linear(x, w)
+    assert torch.equal(y, (x.float() * w[:, 0].float()).to(y.dtype))  # (a product of two bf16 is exact in float32)
 
 
 # ---- refusals ------------------------------------------------------------------------------------

@@ -1110,6 +1110,16 @@ inline int range_splits(int bytes, int64_t bh, int64_t n, int64_t over) {
 }
 inline int64_t stat_words(int64_t bh, int64_t rows) { return cdiv(2 * bh * rows, 4) * 4; }
 
+// Whether a launch holds the workgroups of every kernel of a call.  Forward: of 16 rows, or of 64 (128
+// where two_tiles takes them); joins are of calls with few workgroups only.  Backward: 16 rows' statistics, 64 (128)
+// rows and 64 keys.
+inline bool fits_launch(const AttnArgs& a, int bytes, bool bwd) {
+  const int64_t bh = (int64_t)a.b * a.hk, most = most_groups(256);
+  const bool two = bytes == 2 && two_tiles(bh, a.rows) && feed_async(a.k, a.ks, a.d, 1, bytes) && feed_async(a.v, a.vs, a.d, 1, bytes);
+  if (!bwd) return bh * cdiv(a.rows, a.rows <= kFewRows ? 16 : two ? 128 : 64) <= most;
+  return cdiv(bh * a.rows, 16) <= most && bh * cdiv(a.rows, two ? 128 : 64) <= most && bh * cdiv(a.nk, 64) <= most;
+}
+
 template <class Tr, int kDP>
 void run_split(const AttnArgs& a, hipStream_t st) {
   const int64_t bh = (int64_t)a.b * a.hk;
@@ -1253,6 +1263,7 @@ int yk_attention(yk_ctx* ctx, const yk_attention_args* a, void* stream) {
   k.lse = a->lse;
   k.splits = split_count(tok_bytes(a->dtype), (int64_t)k.b * k.hk, k.rows, k.nk);
   if (k.splits > 1 && !a->ws) k.splits = 1;
+  YK_CHECK_ARG(fits_launch(k, tok_bytes(a->dtype), false), "yk_attention: more work items than a launch holds");
   const hipStream_t st = (hipStream_t)stream;
   if (a->dtype == YK_ACT_F32) run_attn<F32>(k, false, st);
   else if (a->dtype == YK_ACT_BF16) run_attn<B16>(k, false, st);
@@ -1288,6 +1299,7 @@ int yk_attention_backward(yk_ctx* ctx, const yk_attention_grad_args* a, void* st
   k.o = (const char*)a->o, k.go = (const char*)a->go;
   k.dq = (char*)a->dq, k.dk = (char*)a->dk, k.dv = (char*)a->dv;
   k.lse = (float*)a->lse;
+  YK_CHECK_ARG(fits_launch(k, tok_bytes(a->dtype), true), "yk_attention_backward: more work items than a launch holds");
   const int64_t bh = (int64_t)k.b * k.hk;
   k.splits = range_splits(tok_bytes(a->dtype), bh, k.nk, k.rows);
   k.key_splits = range_splits(tok_bytes(a->dtype), bh, k.rows, k.nk);

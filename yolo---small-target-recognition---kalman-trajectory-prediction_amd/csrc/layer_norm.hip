@@ -419,24 +419,38 @@ constexpr int kGradGroups = 768;          // workgroups (and rows of partial sum
 
 constexpr int kNarrowRows = 8192;
 
+// launch(part, its workgroups) for the parts of a call's rows that a launch holds each, `per` rows per workgroup
+template <class F>
+void for_rows(const NormArgs& a, int64_t per, int bytes, F&& launch) {
+  const int64_t most = most_groups(256) * per;
+  for (int64_t r0 = 0; r0 < a.m; r0 += most) {
+    NormArgs p = a;
+    p.x += r0 * a.x_stride * bytes, p.y += r0 * a.y_stride * bytes;
+    if (p.mean) p.mean += r0;
+    if (p.rstd) p.rstd += r0;
+    p.m = a.m - r0 < most ? a.m - r0 : most;
+    launch(p, dim3((unsigned)cdiv(p.m, per)));
+  }
+}
 template <class Tr, int NT>
-void launch_norm(const NormArgs& a, int nv, hipStream_t st) {
-  const dim3 grid((unsigned)cdiv(a.m, 256 / NT));
-  if constexpr (NT == 16) {
-    switch (nv) {
-      case 5: hipLaunchKernelGGL((norm_kernel<Tr, NT, 5>), grid, dim3(256), 0, st, a); return;
-      case 6: hipLaunchKernelGGL((norm_kernel<Tr, NT, 6>), grid, dim3(256), 0, st, a); return;
-      case 7: hipLaunchKernelGGL((norm_kernel<Tr, NT, 7>), grid, dim3(256), 0, st, a); return;
-      case 8: hipLaunchKernelGGL((norm_kernel<Tr, NT, 8>), grid, dim3(256), 0, st, a); return;
-      default: break;
+void launch_norm(const NormArgs& all, int nv, hipStream_t st) {
+  for_rows(all, 256 / NT, Tr::kBytes, [&](const NormArgs& a, dim3 grid) {
+    if constexpr (NT == 16) {
+      switch (nv) {
+        case 5: hipLaunchKernelGGL((norm_kernel<Tr, NT, 5>), grid, dim3(256), 0, st, a); return;
+        case 6: hipLaunchKernelGGL((norm_kernel<Tr, NT, 6>), grid, dim3(256), 0, st, a); return;
+        case 7: hipLaunchKernelGGL((norm_kernel<Tr, NT, 7>), grid, dim3(256), 0, st, a); return;
+        case 8: hipLaunchKernelGGL((norm_kernel<Tr, NT, 8>), grid, dim3(256), 0, st, a); return;
+        default: break;
+      }
     }
-  }
-  switch (nv) {
-    case 1: hipLaunchKernelGGL((norm_kernel<Tr, NT, 1>), grid, dim3(256), 0, st, a); break;
-    case 2: hipLaunchKernelGGL((norm_kernel<Tr, NT, 2>), grid, dim3(256), 0, st, a); break;
-    case 3: hipLaunchKernelGGL((norm_kernel<Tr, NT, 3>), grid, dim3(256), 0, st, a); break;
-    default: hipLaunchKernelGGL((norm_kernel<Tr, NT, 4>), grid, dim3(256), 0, st, a); break;
-  }
+    switch (nv) {
+      case 1: hipLaunchKernelGGL((norm_kernel<Tr, NT, 1>), grid, dim3(256), 0, st, a); break;
+      case 2: hipLaunchKernelGGL((norm_kernel<Tr, NT, 2>), grid, dim3(256), 0, st, a); break;
+      case 3: hipLaunchKernelGGL((norm_kernel<Tr, NT, 3>), grid, dim3(256), 0, st, a); break;
+      default: hipLaunchKernelGGL((norm_kernel<Tr, NT, 4>), grid, dim3(256), 0, st, a); break;
+    }
+  });
 }
 template <class Tr>
 void run_norm(const NormArgs& a, hipStream_t st) {
@@ -445,7 +459,7 @@ void run_norm(const NormArgs& a, hipStream_t st) {
   if (chunks <= 16 || (chunks <= 8 * 16 && a.m >= kNarrowRows)) launch_norm<Tr, 16>(a, (int)cdiv(chunks, 16), st);
   else if (chunks <= 4 * 64) launch_norm<Tr, 64>(a, (int)cdiv(chunks, 64), st);
   else if (chunks <= kMaxChunks) launch_norm<Tr, 256>(a, (int)cdiv(chunks, 256), st);
-  else hipLaunchKernelGGL(norm_wide_kernel<Tr>, dim3((unsigned)a.m), dim3(256), 0, st, a);
+  else for_rows(a, 1, Tr::kBytes, [&](const NormArgs& p, dim3 grid) { hipLaunchKernelGGL(norm_wide_kernel<Tr>, grid, dim3(256), 0, st, p); });
 }
 
 template <class Tr, int NT>
@@ -474,7 +488,13 @@ void run_norm_grad(const NormGradArgs& a, hipStream_t st) {
   const int chunks = (int)cdiv(a.c, 16 / Tr::kBytes);
   const int groups = grad_groups(a.m, a.c, Tr::kBytes);
   if (chunks > kMaxChunks) {
-    if (a.dx) hipLaunchKernelGGL(norm_grad_wide_kernel<Tr>, dim3((unsigned)a.m), dim3(256), 0, st, a);
+    for (int64_t r0 = 0; a.dx && r0 < a.m; r0 += most_groups(256)) {
+      NormGradArgs p = a;
+      p.x += r0 * a.x_stride * Tr::kBytes, p.dy += r0 * a.dy_stride * Tr::kBytes, p.dx += r0 * a.dx_stride * Tr::kBytes;
+      p.mean += r0, p.rstd += r0;
+      hipLaunchKernelGGL(norm_grad_wide_kernel<Tr>, dim3((unsigned)(a.m - r0 < most_groups(256) ? a.m - r0 : most_groups(256))), dim3(256), 0,
+                         st, p);
+    }
     if (a.part)
       hipLaunchKernelGGL(norm_cols_kernel<Tr>, dim3((unsigned)cdiv(chunks, 64), groups), dim3(256), 0, st, a);
     return;

@@ -725,6 +725,7 @@ struct ColArgs {
   float* part;     // [groups][r][n]
   int64_t dy_stride, z_stride, out_stride;
   int m, n, r, groups, act, out_f32, dtype, chunk_blocks;
+  int r0;          // residue of the launch's first workgroups
 };
 
 // Sums over the rows m % r == residue, for each column; a workgroup holds 32 chunks of columns x 8
@@ -736,7 +737,7 @@ __global__ __launch_bounds__(256) void cols_kernel(ColArgs a) {
   constexpr int kEpc = 16 / Tr::kBytes;
   __shared__ float lds[8][32 * kEpc];
   const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
-  const int res = blockIdx.x / a.chunk_blocks, cb = blockIdx.x - res * a.chunk_blocks;
+  const int sub_res = blockIdx.x / a.chunk_blocks, cb = blockIdx.x - sub_res * a.chunk_blocks, res = a.r0 + sub_res;
   const int c0 = (cb * 32 + lane) * kEpc;
   const int n = a.n - c0;
   float acc[kEpc];
@@ -843,6 +844,7 @@ inline Plan plan_gemm(int64_t m, int64_t n, int64_t k, int bytes, int trans, boo
   for (int i = bytes == 2 && !async ? 1 : 0; i < (bytes == 2 ? 3 : 2); ++i) {  // (256: no variant through registers)
     const TileTime& t = times[i];
     const int64_t tiles = cdiv(m, t.tile) * cdiv(n, t.tile);
+    if (tiles > most_groups(t.tile == 256 ? 512 : 256)) continue;  // (128-tiles are never: check_linear)
     for (int64_t s = 1; s == 1 || (s <= 64 && steps >= 4 * s && tiles * s <= kCUs * t.per_cu); s += s < 4 ? 1 : s / 2) {
       const int64_t per = cdiv(steps, s), wgs = cdiv(tiles * cdiv(steps, per), kCUs);
       auto turn = [&](int64_t r) {  // r workgroups at once on a CU
@@ -922,7 +924,7 @@ void launch_gemm(GemmArgs a, void* part, int64_t room, hipStream_t st) {
 
 template <class Tr>
 void run_linear(const GemmArgs& a, void* part, int64_t room, hipStream_t st) {
-  if (a.m <= kFewRows) {
+  if (a.m <= kFewRows && cdiv(a.n, 16) <= most_groups(512)) {
     const dim3 grid((unsigned)cdiv(a.n, 16));
     if (a.m <= 16) hipLaunchKernelGGL((rows_kernel<Tr, 1>), grid, dim3(512), 0, st, a);
     else if (a.m <= 32) hipLaunchKernelGGL((rows_kernel<Tr, 2>), grid, dim3(512), 0, st, a);
@@ -944,12 +946,16 @@ void run_cols(ColArgs c, float* part, hipStream_t st) {
   c.groups = col_groups(c.m, c.n, c.r, Tr::kBytes);
   c.chunk_blocks = (int)cdiv(c.n, 32 * (16 / Tr::kBytes));
   c.part = c.out && c.groups > 1 ? part : nullptr;
-  const dim3 grid((unsigned)(c.chunk_blocks * (int64_t)c.r), (unsigned)c.groups);
-  switch (c.act) {
-    case YK_TOK_GELU: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_GELU>), grid, dim3(256), 0, st, c); break;
-    case YK_TOK_SILU: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_SILU>), grid, dim3(256), 0, st, c); break;
-    case YK_TOK_RELU: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_RELU>), grid, dim3(256), 0, st, c); break;
-    default: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_NONE>), grid, dim3(256), 0, st, c);
+  const int64_t per = most_groups(256) / c.chunk_blocks;  // residues of a launch
+  for (int64_t r0 = 0; r0 < c.r; r0 += per) {
+    c.r0 = (int)r0;
+    const dim3 grid((unsigned)(c.chunk_blocks * (c.r - r0 < per ? c.r - r0 : per)), (unsigned)c.groups);
+    switch (c.act) {
+      case YK_TOK_GELU: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_GELU>), grid, dim3(256), 0, st, c); break;
+      case YK_TOK_SILU: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_SILU>), grid, dim3(256), 0, st, c); break;
+      case YK_TOK_RELU: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_RELU>), grid, dim3(256), 0, st, c); break;
+      default: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_NONE>), grid, dim3(256), 0, st, c);
+    }
   }
   if (c.part)
     hipLaunchKernelGGL(cols_sum_kernel, dim3((unsigned)cdiv((int64_t)c.r * c.n, 64)), dim3(1024), 0, st, c);
@@ -1001,8 +1007,8 @@ int check_linear(const char* fn, int dtype, int act, int64_t m, int64_t n, int64
   YK_CHECK_ARG(act >= YK_TOK_NONE && act <= YK_TOK_RELU, std::string(fn) + ": bad activation");
   YK_CHECK_ARG(m >= 0 && m < (1 << 30) && n >= 1 && n < (1 << 30) && k >= 1 && k < (1 << 30),
                std::string(fn) + ": sizes out of range (m in [0, 2^30), n and k in [1, 2^30))");
-  YK_CHECK_ARG(cdiv(m, 64) * cdiv(n, 64) < (int64_t(1) << 31) && cdiv(m, 64) * cdiv(k, 64) < (int64_t(1) << 31) &&
-                   cdiv(n, 64) * cdiv(k, 64) < (int64_t(1) << 31),
+  YK_CHECK_ARG(cdiv(m, 128) * cdiv(n, 128) <= most_groups(256) && cdiv(m, 128) * cdiv(k, 128) <= most_groups(256) &&
+                   cdiv(n, 128) * cdiv(k, 128) <= most_groups(256),
                std::string(fn) + ": more tiles than a launch holds");
   return YK_OK;
 }

@@ -237,6 +237,8 @@ inline int tok_bytes(int dtype) {
   return dtype == YK_ACT_F32 ? 4 : dtype == YK_ACT_BF16 || dtype == YK_ACT_F16 ? 2 : 0;
 }
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// Workgroups of `threads` that one launch holds along x: HIP takes fewer than 2^32 threads there.
+inline int64_t most_groups(int threads) { return 0xffffffffll / threads; }
 
 inline int launched(const char* what) {
   const hipError_t e = hipGetLastError();
