@@ -27,6 +27,10 @@ int yk_model_graph_count(yk_model* m, int32_t* n_graphs, int32_t* cap);
 /* Diagnostics: detector stores found outside every detector allocation so far (store-check build,
  * csrc/build.py YK_DEFINES=-DYK_STORE_CHECK=1); -1 from the product library. */
 int yk_store_check_count(int64_t* out);
+/* Diagnostics: the kernels that a token operator's call would launch, a line each as profilers name
+ * them; nothing is launched and no pointer is followed.  which: yk_struct_size's id of `args`
+ * (tests/test_token_ops_paths_cpu.py). */
+int yk_token_kernels(int which, const void* args, char* buf, int len);
 #ifdef __cplusplus
 }
 #endif

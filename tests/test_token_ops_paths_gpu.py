@@ -123,3 +123,31 @@ def test_tracing_is_refused(ops):
     x, w = rn(4, 8), rn(6, 8)
     with pytest.raises(pkg().YKError, match="jit.trace"):
         torch.jit.trace(lambda t: ops.linear(t, w), (x,))
+
+
+# ---- the detector's report ------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_profile_names_the_kernels_of_an_aifi_row(dtype):
+    """profile() names what its batch launches: 80 cells of 2 images are above the few rows' 64 and
+    one image's attention below its 128; a batch of 20-cell images takes the few-rows kernel."""
+    import importlib
+
+    import numpy as np
+
+    from aifi_helpers import aifi_dict
+
+    P = pkg()
+    A, W, M = (importlib.import_module(f"{P.__name__}.{n}") for n in ("arch", "weights", "model"))
+    ar = A.parse_arch(aifi_dict("n"))
+    sd = W.synthetic_state_dict(ar, 0)
+    t = {"fp32": "F32", "bf16": "B16"}[dtype]
+    many = "gemm_f32_kernel<false, false, 64>" if dtype == "fp32" else f"gemm_kernel<yk::tok::{t}, false, false, "
+    for hw, linear, attention in (((256, 320), many, "attn_split_kernel<yk::tok::" + t), ((128, 160), "rows_kernel<yk::tok::" + t, "attn_split_"),
+                                  ((384, 640), many, "attn_kernel<yk::tok::" + t)):
+        dm = M.DeviceModel(M.Program(ar, sd, hw[0], hw[1], max(hw), 2, dtype))
+        frames = torch.from_numpy(np.zeros((2, *hw, 3), np.uint8)).cuda()
+        dm.detect(frames, 0.25, 0.7, 300)
+        names = {kind: [n for _, k, n, _ in dm.profile(frames) if k == kind] for kind in (M.YK_K_LINEAR, M.YK_K_LAYER_NORM, M.YK_K_ATTENTION)}
+        assert len(names[M.YK_K_LINEAR]) == 4 and all(n.startswith(linear) for n in names[M.YK_K_LINEAR]), names
+        assert all(n.startswith("norm_kernel<yk::tok::" + t) for n in names[M.YK_K_LAYER_NORM]), names
+        assert all(n.startswith(attention) for n in names[M.YK_K_ATTENTION]), names

@@ -1127,35 +1127,35 @@ void run_split(const AttnArgs& a, hipStream_t st) {
   constexpr int kWaves = kDP * Tr::kBytes > 256 ? 2 : 4;  // (as many as have their slabs in 160 KB)
   const dim3 grid((unsigned)(bh * rb), a.splits);
   if (feed_async(a.k, a.ks, a.d, 1, Tr::kBytes) && feed_async(a.v, a.vs, a.d, 1, Tr::kBytes))
-    hipLaunchKernelGGL((attn_split_kernel<Tr, kDP, kWaves, true>), grid, dim3(64 * kWaves), 0, st, a, rb);
+    launch((attn_split_kernel<Tr, kDP, kWaves, true>), grid, dim3(64 * kWaves), 0, st, a, rb);
   else
-    hipLaunchKernelGGL((attn_split_kernel<Tr, kDP, kWaves, false>), grid, dim3(64 * kWaves), 0, st, a, rb);
+    launch((attn_split_kernel<Tr, kDP, kWaves, false>), grid, dim3(64 * kWaves), 0, st, a, rb);
   if (a.splits > 1)
-    hipLaunchKernelGGL(attn_join_kernel<Tr>, dim3((unsigned)(bh * a.rows)), dim3(256), 0, st, a, rb, kDP);
+    launch(attn_join_kernel<Tr>, dim3((unsigned)(bh * a.rows)), dim3(256), 0, st, a, rb, kDP);
 }
 
 template <class Tr, int kDP, int kNT, bool kAsync = true>
 void launch_fwd(const AttnArgs& a, hipStream_t st) {
   const int rb = (int)cdiv(a.rows, 64 * kNT);
-  hipLaunchKernelGGL((attn_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * rb), a.splits), dim3(256), 0, st, a, rb);
+  launch((attn_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * rb), a.splits), dim3(256), 0, st, a, rb);
   if (a.splits > 1)
-    hipLaunchKernelGGL(attn_join_rows_kernel<Tr>, dim3((unsigned)cdiv((int64_t)a.b * a.hk * a.rows, 256 / (kDP / 4))), dim3(256), 0, st,
+    launch(attn_join_rows_kernel<Tr>, dim3((unsigned)cdiv((int64_t)a.b * a.hk * a.rows, 256 / (kDP / 4))), dim3(256), 0, st,
                        a, kDP);
 }
 template <class Tr, int kDP, int kNT, bool kAsync = true>
 void launch_dkv(const AttnArgs& a, hipStream_t st) {
   const int kb = (int)cdiv(a.nk, 64 * kNT), s = a.splits;
-  hipLaunchKernelGGL((attn_dkv_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * kb), s), dim3(256), 0, st, a, kb);
+  launch((attn_dkv_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * kb), s), dim3(256), 0, st, a, kb);
   if (s > 1)
-    hipLaunchKernelGGL(attn_dkv_sum_kernel<Tr>, dim3((unsigned)cdiv((int64_t)a.b * a.hk * a.nk, 256 / (kDP / 2))), dim3(256), 0, st,
+    launch(attn_dkv_sum_kernel<Tr>, dim3((unsigned)cdiv((int64_t)a.b * a.hk * a.nk, 256 / (kDP / 2))), dim3(256), 0, st,
                        a, kDP, s);
 }
 template <class Tr, int kDP, int kNT, bool kAsync = true>
 void launch_dq(const AttnArgs& a, hipStream_t st) {
   const int rb = (int)cdiv(a.rows, 64 * kNT), s = a.key_splits;
-  hipLaunchKernelGGL((attn_dq_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * rb), s), dim3(256), 0, st, a, rb);
+  launch((attn_dq_kernel<Tr, kDP, kNT, kAsync>), dim3((unsigned)((int64_t)a.b * a.hk * rb), s), dim3(256), 0, st, a, rb);
   if (s > 1)
-    hipLaunchKernelGGL(attn_dq_sum_kernel<Tr>, dim3((unsigned)cdiv((int64_t)a.b * a.hk * a.rows, 256 / (kDP / 4))), dim3(256), 0, st,
+    launch(attn_dq_sum_kernel<Tr>, dim3((unsigned)cdiv((int64_t)a.b * a.hk * a.rows, 256 / (kDP / 4))), dim3(256), 0, st,
                        a, kDP, s);
 }
 
@@ -1171,7 +1171,7 @@ void run_fwd(const AttnArgs& a, hipStream_t st) {
 template <class Tr, int kDP>
 void run_bwd(const AttnArgs& a, hipStream_t st) {
   const int64_t bh = (int64_t)a.b * a.hk;
-  hipLaunchKernelGGL(attn_delta_kernel<Tr>, dim3((unsigned)cdiv(bh * a.rows, 16)), dim3(256), 0, st, a);
+  launch(attn_delta_kernel<Tr>, dim3((unsigned)cdiv(bh * a.rows, 16)), dim3(256), 0, st, a);
   const bool rows = feed_async(a.q, a.qs, a.d, a.group, Tr::kBytes) && feed_async(a.go, a.gos, a.d, a.group, Tr::kBytes);
   const bool keys = feed_async(a.k, a.ks, a.d, 1, Tr::kBytes) && feed_async(a.v, a.vs, a.d, 1, Tr::kBytes);
   constexpr int kTwo = Tr::kBytes == 2 ? 2 : 1, kTwoKeys = kDP == 96 ? kTwo : 1;

@@ -4413,7 +4413,7 @@ int launch_any(yk_model* m, const yk_op& op, const uint8_t* frames, int B, float
 }
 
 // Name of the kernel instantiation an op launches (matches rocprofv3's demangled names).
-const char* op_kernel_name(const yk_model* m, const yk_op& op) {
+const char* op_kernel_name(yk_model* m, const yk_op& op) {
   const int dt = m->desc.act_dtype;
   const bool f = dt == YK_ACT_F32;
   const char* tn = tr_name(dt);  // (F32S for a split-MFMA table conv below)
@@ -4433,10 +4433,14 @@ const char* op_kernel_name(const yk_model* m, const yk_op& op) {
         snprintf(buf, sizeof buf, "sppf_pool_kernel<yk::det::%s>", tn);
       return buf;
     case YK_K_DETECT: snprintf(buf, sizeof buf, "detect_kernel<yk::det::%s>", tn); return buf;
-    // (the token operators pick their instantiation by shape: the kernel's own name)
-    case YK_K_LINEAR: return (int64_t)op.out_h * op.out_w * m->desc.max_batch <= 64 ? "rows_kernel" : "gemm_kernel";
-    case YK_K_LAYER_NORM: return "norm_kernel";
-    case YK_K_ATTENTION: return "attn_kernel";
+    case YK_K_LINEAR:
+    case YK_K_LAYER_NORM:
+    case YK_K_ATTENTION: {
+      yk::KernelNames names;
+      if (launch_token_op(m, op, m->plan_batch, nullptr, 0) != YK_OK) return "unknown";
+      snprintf(buf, sizeof buf, "%s", names.text.substr(0, names.text.find('\n')).c_str());
+      return buf;
+    }
     default: break;
   }
   const ConvPlan cp = conv_plan(m, op, m->plan_batch);

@@ -419,9 +419,9 @@ constexpr int kGradGroups = 768;          // workgroups (and rows of partial sum
 
 constexpr int kNarrowRows = 8192;
 
-// launch(part, its workgroups) for the parts of a call's rows that a launch holds each, `per` rows per workgroup
+// run(part, its workgroups) for the parts of a call's rows that a launch holds each, `per` rows per workgroup
 template <class F>
-void for_rows(const NormArgs& a, int64_t per, int bytes, F&& launch) {
+void for_rows(const NormArgs& a, int64_t per, int bytes, F&& run) {
   const int64_t most = most_groups(256) * per;
   for (int64_t r0 = 0; r0 < a.m; r0 += most) {
     NormArgs p = a;
@@ -429,7 +429,7 @@ void for_rows(const NormArgs& a, int64_t per, int bytes, F&& launch) {
     if (p.mean) p.mean += r0;
     if (p.rstd) p.rstd += r0;
     p.m = a.m - r0 < most ? a.m - r0 : most;
-    launch(p, dim3((unsigned)cdiv(p.m, per)));
+    run(p, dim3((unsigned)cdiv(p.m, per)));
   }
 }
 template <class Tr, int NT>
@@ -437,18 +437,18 @@ void launch_norm(const NormArgs& all, int nv, hipStream_t st) {
   for_rows(all, 256 / NT, Tr::kBytes, [&](const NormArgs& a, dim3 grid) {
     if constexpr (NT == 16) {
       switch (nv) {
-        case 5: hipLaunchKernelGGL((norm_kernel<Tr, NT, 5>), grid, dim3(256), 0, st, a); return;
-        case 6: hipLaunchKernelGGL((norm_kernel<Tr, NT, 6>), grid, dim3(256), 0, st, a); return;
-        case 7: hipLaunchKernelGGL((norm_kernel<Tr, NT, 7>), grid, dim3(256), 0, st, a); return;
-        case 8: hipLaunchKernelGGL((norm_kernel<Tr, NT, 8>), grid, dim3(256), 0, st, a); return;
+        case 5: launch((norm_kernel<Tr, NT, 5>), grid, dim3(256), 0, st, a); return;
+        case 6: launch((norm_kernel<Tr, NT, 6>), grid, dim3(256), 0, st, a); return;
+        case 7: launch((norm_kernel<Tr, NT, 7>), grid, dim3(256), 0, st, a); return;
+        case 8: launch((norm_kernel<Tr, NT, 8>), grid, dim3(256), 0, st, a); return;
         default: break;
       }
     }
     switch (nv) {
-      case 1: hipLaunchKernelGGL((norm_kernel<Tr, NT, 1>), grid, dim3(256), 0, st, a); break;
-      case 2: hipLaunchKernelGGL((norm_kernel<Tr, NT, 2>), grid, dim3(256), 0, st, a); break;
-      case 3: hipLaunchKernelGGL((norm_kernel<Tr, NT, 3>), grid, dim3(256), 0, st, a); break;
-      default: hipLaunchKernelGGL((norm_kernel<Tr, NT, 4>), grid, dim3(256), 0, st, a); break;
+      case 1: launch((norm_kernel<Tr, NT, 1>), grid, dim3(256), 0, st, a); break;
+      case 2: launch((norm_kernel<Tr, NT, 2>), grid, dim3(256), 0, st, a); break;
+      case 3: launch((norm_kernel<Tr, NT, 3>), grid, dim3(256), 0, st, a); break;
+      default: launch((norm_kernel<Tr, NT, 4>), grid, dim3(256), 0, st, a); break;
     }
   });
 }
@@ -459,15 +459,15 @@ void run_norm(const NormArgs& a, hipStream_t st) {
   if (chunks <= 16 || (chunks <= 8 * 16 && a.m >= kNarrowRows)) launch_norm<Tr, 16>(a, (int)cdiv(chunks, 16), st);
   else if (chunks <= 4 * 64) launch_norm<Tr, 64>(a, (int)cdiv(chunks, 64), st);
   else if (chunks <= kMaxChunks) launch_norm<Tr, 256>(a, (int)cdiv(chunks, 256), st);
-  else for_rows(a, 1, Tr::kBytes, [&](const NormArgs& p, dim3 grid) { hipLaunchKernelGGL(norm_wide_kernel<Tr>, grid, dim3(256), 0, st, p); });
+  else for_rows(a, 1, Tr::kBytes, [&](const NormArgs& p, dim3 grid) { launch(norm_wide_kernel<Tr>, grid, dim3(256), 0, st, p); });
 }
 
 template <class Tr, int NT>
 void launch_norm_grad(const NormGradArgs& a, int nv, int groups, hipStream_t st) {
   const size_t lds = NT >= 256 ? NT / 64 * 4 : (size_t)(256 / NT) * a.c * 4;
   const dim3 block(NT < 256 ? 256 : NT);
-  if (nv == 1) hipLaunchKernelGGL((norm_grad_kernel<Tr, NT, 1>), dim3(groups), block, lds, st, a);
-  else hipLaunchKernelGGL((norm_grad_kernel<Tr, NT, 2>), dim3(groups), block, lds, st, a);
+  if (nv == 1) launch((norm_grad_kernel<Tr, NT, 1>), dim3(groups), block, lds, st, a);
+  else launch((norm_grad_kernel<Tr, NT, 2>), dim3(groups), block, lds, st, a);
 }
 // Lanes per row of the backward pass: at most two chunks each, whose sums, row and next row are some
 // 150 registers (four took 270, one wave per SIMD: 10000 x 8192 bf16 187 us).  Two of 16 lanes only with
@@ -492,11 +492,11 @@ void run_norm_grad(const NormGradArgs& a, hipStream_t st) {
       NormGradArgs p = a;
       p.x += r0 * a.x_stride * Tr::kBytes, p.dy += r0 * a.dy_stride * Tr::kBytes, p.dx += r0 * a.dx_stride * Tr::kBytes;
       p.mean += r0, p.rstd += r0;
-      hipLaunchKernelGGL(norm_grad_wide_kernel<Tr>, dim3((unsigned)(a.m - r0 < most_groups(256) ? a.m - r0 : most_groups(256))), dim3(256), 0,
+      launch(norm_grad_wide_kernel<Tr>, dim3((unsigned)(a.m - r0 < most_groups(256) ? a.m - r0 : most_groups(256))), dim3(256), 0,
                          st, p);
     }
     if (a.part)
-      hipLaunchKernelGGL(norm_cols_kernel<Tr>, dim3((unsigned)cdiv(chunks, 64), groups), dim3(256), 0, st, a);
+      launch(norm_cols_kernel<Tr>, dim3((unsigned)cdiv(chunks, 64), groups), dim3(256), 0, st, a);
     return;
   }
   switch (grad_lanes(a.m, chunks)) {
@@ -568,7 +568,7 @@ int yk_layer_norm_backward(yk_ctx* ctx, const yk_layer_norm_grad_args* a, void* 
     else run_norm_grad<H16>(k, st);
   }
   if (cols)
-    hipLaunchKernelGGL(norm_reduce_kernel, dim3((unsigned)cdiv(a->c, 32), 2), dim3(1024), 0, st, (const float*)a->ws,
+    launch(norm_reduce_kernel, dim3((unsigned)cdiv(a->c, 32), 2), dim3(1024), 0, st, (const float*)a->ws,
                        grad_groups(a->m, (int)a->c, tok_bytes(a->dtype)), (int)a->c, a->dw, a->db, f32, a->dtype);
   return launched("yk_layer_norm_backward");
 }

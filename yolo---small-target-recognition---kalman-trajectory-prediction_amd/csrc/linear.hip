@@ -875,18 +875,18 @@ template <class Tr, bool kXT, bool kWT, bool kAsync>
 void launch_tiles(const GemmArgs& a, int tile, int splits, hipStream_t st) {
   const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), (unsigned)splits);
   if constexpr (Tr::kBytes == 4) {
-    if (tile == 128) hipLaunchKernelGGL((gemm_f32_kernel<kXT, kWT, 128>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((gemm_f32_kernel<kXT, kWT, 64>), grid, dim3(256), 0, st, a);
+    if (tile == 128) launch((gemm_f32_kernel<kXT, kWT, 128>), grid, dim3(256), 0, st, a);
+    else launch((gemm_f32_kernel<kXT, kWT, 64>), grid, dim3(256), 0, st, a);
     return;
   } else {
   if constexpr (kAsync) {
     if (tile == 256) {
-      hipLaunchKernelGGL((gemm_kernel<Tr, kXT, kWT, 256, 256, 2, 4, 2, true>), grid, dim3(512), 0, st, a);
+      launch((gemm_kernel<Tr, kXT, kWT, 256, 256, 2, 4, 2, true>), grid, dim3(512), 0, st, a);
       return;
     }
   }
-  if (tile == 128) hipLaunchKernelGGL((gemm_kernel<Tr, kXT, kWT, 128, 128, 2, 2, 2, kAsync>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((gemm_kernel<Tr, kXT, kWT, 64, 64, 2, 2, 2, kAsync>), grid, dim3(256), 0, st, a);
+  if (tile == 128) launch((gemm_kernel<Tr, kXT, kWT, 128, 128, 2, 2, 2, kAsync>), grid, dim3(256), 0, st, a);
+  else launch((gemm_kernel<Tr, kXT, kWT, 64, 64, 2, 2, 2, kAsync>), grid, dim3(256), 0, st, a);
   }
 }
 
@@ -917,8 +917,8 @@ void launch_gemm(GemmArgs a, void* part, int64_t room, hipStream_t st) {
   else launch_tiles<Tr, kXT, kWT, false>(a, p.tile, p.splits, st);
   if (p.splits > 1) {
     const int64_t items = (int64_t)a.m * cdiv(a.n, 8);
-    if (p.splits >= 8) hipLaunchKernelGGL((split_sum_kernel<Tr, 8>), dim3((unsigned)cdiv(items, 32)), dim3(256), 0, st, a, p.splits);
-    else hipLaunchKernelGGL((split_sum_kernel<Tr, 1>), dim3((unsigned)cdiv(items, 256)), dim3(256), 0, st, a, p.splits);
+    if (p.splits >= 8) launch((split_sum_kernel<Tr, 8>), dim3((unsigned)cdiv(items, 32)), dim3(256), 0, st, a, p.splits);
+    else launch((split_sum_kernel<Tr, 1>), dim3((unsigned)cdiv(items, 256)), dim3(256), 0, st, a, p.splits);
   }
 }
 
@@ -926,9 +926,9 @@ template <class Tr>
 void run_linear(const GemmArgs& a, void* part, int64_t room, hipStream_t st) {
   if (a.m <= kFewRows && cdiv(a.n, 16) <= most_groups(512)) {
     const dim3 grid((unsigned)cdiv(a.n, 16));
-    if (a.m <= 16) hipLaunchKernelGGL((rows_kernel<Tr, 1>), grid, dim3(512), 0, st, a);
-    else if (a.m <= 32) hipLaunchKernelGGL((rows_kernel<Tr, 2>), grid, dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((rows_kernel<Tr, 4>), grid, dim3(512), 0, st, a);
+    if (a.m <= 16) launch((rows_kernel<Tr, 1>), grid, dim3(512), 0, st, a);
+    else if (a.m <= 32) launch((rows_kernel<Tr, 2>), grid, dim3(512), 0, st, a);
+    else launch((rows_kernel<Tr, 4>), grid, dim3(512), 0, st, a);
     return;
   }
   launch_gemm<Tr, false, false>(a, part, room, st);
@@ -951,14 +951,14 @@ void run_cols(ColArgs c, float* part, hipStream_t st) {
     c.r0 = (int)r0;
     const dim3 grid((unsigned)(c.chunk_blocks * (c.r - r0 < per ? c.r - r0 : per)), (unsigned)c.groups);
     switch (c.act) {
-      case YK_TOK_GELU: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_GELU>), grid, dim3(256), 0, st, c); break;
-      case YK_TOK_SILU: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_SILU>), grid, dim3(256), 0, st, c); break;
-      case YK_TOK_RELU: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_RELU>), grid, dim3(256), 0, st, c); break;
-      default: hipLaunchKernelGGL((cols_kernel<Tr, YK_TOK_NONE>), grid, dim3(256), 0, st, c);
+      case YK_TOK_GELU: launch((cols_kernel<Tr, YK_TOK_GELU>), grid, dim3(256), 0, st, c); break;
+      case YK_TOK_SILU: launch((cols_kernel<Tr, YK_TOK_SILU>), grid, dim3(256), 0, st, c); break;
+      case YK_TOK_RELU: launch((cols_kernel<Tr, YK_TOK_RELU>), grid, dim3(256), 0, st, c); break;
+      default: launch((cols_kernel<Tr, YK_TOK_NONE>), grid, dim3(256), 0, st, c);
     }
   }
   if (c.part)
-    hipLaunchKernelGGL(cols_sum_kernel, dim3((unsigned)cdiv((int64_t)c.r * c.n, 64)), dim3(1024), 0, st, c);
+    launch(cols_sum_kernel, dim3((unsigned)cdiv((int64_t)c.r * c.n, 64)), dim3(1024), 0, st, c);
 }
 
 template <class Tr>

@@ -4,6 +4,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "yk_internal.h"
 
@@ -240,7 +241,15 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Workgroups of `threads` that one launch holds along x: HIP takes fewer than 2^32 threads there.
 inline int64_t most_groups(int threads) { return 0xffffffffll / threads; }
 
+// Every launch of the token operators.
+template <class... P>
+inline void launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t st, std::common_type_t<P>... args) {
+  if (KernelNames* names = KernelNames::current()) return names->add((const void*)kernel);
+  void* ptrs[] = {(void*)&args...};
+  (void)hipLaunchKernel((const void*)kernel, grid, block, ptrs, lds, st);  // (launched() looks for its error)
+}
 inline int launched(const char* what) {
+  if (KernelNames::current()) return YK_OK;
   const hipError_t e = hipGetLastError();
   if (e == hipSuccess) return YK_OK;
   set_error(std::string(what) + ": launch failed: " + hipGetErrorString(e));

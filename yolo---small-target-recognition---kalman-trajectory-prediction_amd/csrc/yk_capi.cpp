@@ -1,4 +1,6 @@
 // Context handling, error reporting and the engine-file loader of the C ABI (include/yk.h).
+#include <cxxabi.h>
+#include <dlfcn.h>
 #include <execinfo.h>
 #include <signal.h>
 #include <unistd.h>
@@ -7,7 +9,32 @@
 #include <cstring>
 #include <vector>
 
+#include "yk_diag.h"
 #include "yk_internal.h"
+
+namespace yk {
+namespace {
+thread_local KernelNames* t_names = nullptr;
+}
+KernelNames::KernelNames() : outer_(t_names) { t_names = this; }
+KernelNames::~KernelNames() { t_names = outer_; }
+KernelNames* KernelNames::current() { return t_names; }
+void KernelNames::add(const void* kernel) {
+  Dl_info info;
+  std::string name = "unknown";
+  if (dladdr(kernel, &info) && info.dli_sname) {
+    int status = 0;
+    char* d = abi::__cxa_demangle(info.dli_sname, nullptr, nullptr, &status);
+    name = d ? d : info.dli_sname;
+    free(d);
+    name = name.substr(0, name.find('('));
+    const char* own = "yk::tok::";  // (the kernel's own, not its arguments')
+    const size_t at = name.find(own);
+    if (at <= 5) name = name.substr(at + strlen(own));
+  }
+  text += name + "\n";
+}
+}  // namespace yk
 
 extern "C" {
 
@@ -52,6 +79,24 @@ int yk_ctx_create(int device, yk_ctx** out) {
   YK_HIP(hipFree(nullptr));  // force runtime/context initialisation on this device
   *out = new yk_ctx{device};
   return YK_OK;
+}
+
+int yk_token_kernels(int which, const void* args, char* buf, int len) {
+  YK_CHECK_ARG(args && buf && len > 0, "yk_token_kernels: bad argument");
+  static yk_ctx ctx{0};
+  yk::KernelNames names;
+  int rc = YK_ERR_ARG;
+  switch (which) {
+    case 12: rc = yk_linear(&ctx, (const yk_linear_args*)args, nullptr); break;
+    case 13: rc = yk_linear_backward(&ctx, (const yk_linear_grad_args*)args, nullptr); break;
+    case 14: rc = yk_layer_norm(&ctx, (const yk_layer_norm_args*)args, nullptr); break;
+    case 15: rc = yk_layer_norm_backward(&ctx, (const yk_layer_norm_grad_args*)args, nullptr); break;
+    case 16: rc = yk_attention(&ctx, (const yk_attention_args*)args, nullptr); break;
+    case 17: rc = yk_attention_backward(&ctx, (const yk_attention_grad_args*)args, nullptr); break;
+    default: yk::set_error("yk_token_kernels: which must be in [12, 17]");
+  }
+  if (rc == YK_OK) snprintf(buf, (size_t)len, "%s", names.text.c_str());
+  return rc;
 }
 
 int64_t yk_struct_size(int which) {

@@ -38,4 +38,18 @@ struct DeviceGuard {
   }
 };
 
+// While one lives, the token operators' calls of its thread launch nothing: they add the name of each kernel that
+// they would launch to `text`, a line each, as profilers print it (what yk_token_kernels and yk_model_op_kernel report,
+// so that no second rule says what runs).
+struct KernelNames {
+  std::string text;
+  KernelNames();
+  ~KernelNames();
+  void add(const void* kernel);
+  static KernelNames* current();  // NULL: launches are made
+
+ private:
+  KernelNames* outer_;
+};
+
 }  // namespace yk
