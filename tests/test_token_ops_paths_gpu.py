@@ -125,6 +125,26 @@ def test_tracing_is_refused(ops):
         torch.jit.trace(lambda t: ops.linear(t, w), (x,))
 
 
+def test_an_earlier_error_of_the_runtime_is_not_the_calls(ops):
+    """A HIP call of the caller that failed leaves its code as the runtime's last error: the operators
+    neither report it as a launch of theirs nor take it away."""
+    import ctypes as C
+
+    x, w, q = rn(4, 8), rn(6, 8), rn(1, 4, 2, 8)
+    want = ops.linear(x, w), ops.layer_norm(x), ops.attention(q, q, q)
+    torch.cuda.synchronize()
+    loaded = {line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64" in line}
+    hip = C.CDLL(loaded.pop())
+    assert not loaded and hip.hipSetDevice(4096) != 0  # no such device
+    try:
+        got = ops.linear(x, w), ops.layer_norm(x), ops.attention(q, q, q)
+    finally:
+        left = hip.hipGetLastError()
+    assert left != 0
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 # ---- the detector's report ------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_profile_names_the_kernels_of_an_aifi_row(dtype):

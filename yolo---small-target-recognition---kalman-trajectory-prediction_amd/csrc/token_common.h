@@ -241,17 +241,21 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Workgroups of `threads` that one launch holds along x: HIP takes fewer than 2^32 threads there.
 inline int64_t most_groups(int threads) { return 0xffffffffll / threads; }
 
-// Every launch of the token operators.
+// Every launch of the token operators; a call's first error is kept for launched().  (The runtime's last
+// error may be another call's, of the caller's own, and is neither reported nor cleared here.)
+inline thread_local hipError_t t_launch_error = hipSuccess;
 template <class... P>
 inline void launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t st, std::common_type_t<P>... args) {
   if (KernelNames* names = KernelNames::current()) return names->add((const void*)kernel);
+  if (t_launch_error != hipSuccess) return;
   void* ptrs[] = {(void*)&args...};
-  (void)hipLaunchKernel((const void*)kernel, grid, block, ptrs, lds, st);  // (launched() looks for its error)
+  t_launch_error = hipLaunchKernel((const void*)kernel, grid, block, ptrs, lds, st);
 }
 inline int launched(const char* what) {
-  if (KernelNames::current()) return YK_OK;
-  const hipError_t e = hipGetLastError();
+  const hipError_t e = t_launch_error;
   if (e == hipSuccess) return YK_OK;
+  t_launch_error = hipSuccess;
+  (void)hipGetLastError();  // reported here
   set_error(std::string(what) + ": launch failed: " + hipGetErrorString(e));
   return YK_ERR_HIP;
 }
