@@ -119,6 +119,21 @@ def test_forward_mode_tangents_are_refused(ops):
                         f(*args, **{**kw, n: forward_ad.make_dual(t, torch.ones_like(t))})
 
 
+def test_values_outside_float32_are_refused(ops):
+    q, x = rn(1, 4, 2, 8), rn(4, 8)
+    for scale in (1e39, 1e-50, -1.0, float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            ops.attention(q, q, q, scale=scale)
+    for eps in (1e39, -1e-9, float("nan")):
+        with pytest.raises(ValueError, match="eps"):
+            ops.layer_norm(x, eps=eps)
+    y = ops.layer_norm(x, eps=torch.finfo(torch.float32).max)
+    R.check(y, *R.layer_norm(x, None, None, torch.finfo(torch.float32).max), "y")
+    many = q[:, :1].expand(2 ** 31, 1, 2, 8)
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.attention(many, many, many)
+
+
 def test_tracing_is_refused(ops):
     x, w = rn(4, 8), rn(6, 8)
     with pytest.raises(pkg().YKError, match="jit.trace"):

@@ -25,6 +25,7 @@ from . import _lib as L
 ACTS = {"none": 0, "silu": 1, "gelu": 2, "relu": 3}
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 3}  # yk_act_dtype
 _F32 = torch.float32
+_F32_MIN, _F32_MAX, _INF = 2.0 ** -149, torch.finfo(_F32).max, float("inf")
 _empty, _empty_like, _grad_enabled, _tracing = torch.empty, torch.empty_like, torch.is_grad_enabled, torch._C._is_tracing
 
 # The C argument structs as packed bytes (a ctypes struct costs three times as long to fill); the
@@ -244,8 +245,8 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, return_stats=False):
     dt, dev = _input(x, "x")
     m, c, xs = _rows(x, "x")
     w, b, pf = _norm_params(weight, bias, c, dev, x.dtype)
-    if not eps >= 0:
-        raise ValueError("eps must be >= 0")
+    if not eps >= 0 or _F32_MAX < eps < _INF:
+        raise ValueError("eps must be >= 0, in float32's range")
     y = _fresh(x)
     mean = rstd = None
     if return_stats:
@@ -305,8 +306,10 @@ def _attention_args(q, k, v, scale, causal, q_lengths, lengths):
     if not 1 <= d <= 128:
         raise ValueError(f"head size must be in [1, 128], got {d}")
     scale = d ** -0.5 if scale is None else float(scale)
-    if not 0 < scale < float("inf"):
-        raise ValueError("scale must be positive and finite")
+    if not _F32_MIN <= scale <= _F32_MAX:
+        raise ValueError("scale must be positive and finite, in float32's range")
+    if max(b, h) >= 1 << 31:
+        raise ValueError("more batch elements or heads than 2^31")
     lens = [0, 0]
     for i, (t, name) in enumerate(((q_lengths, "q_lengths"), (lengths, "lengths"))):
         if t is not None:
