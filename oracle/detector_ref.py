@@ -324,25 +324,6 @@ class RefDetectorFP8(RefDetector):
             y.append(self.conv(t, f"{p}.m.{j}.cv2", 3, 1, res=y[-1] if shortcut else None))
         return self.conv(torch.cat(y, 1), f"{p}.cv2", 1, 1)
 
-    def aifi(self, x, p, heads):
-        b, c, h, w = x.shape
-        W = {k[len(p) + 1:]: v.float() for k, v in self.sd.items() if k.startswith(p + ".")}
-        cols, rows = torch.meshgrid(torch.arange(w, dtype=torch.float32), torch.arange(h, dtype=torch.float32), indexing="ij")
-        freq = 10000.0 ** -(torch.arange(c // 4, dtype=torch.float32) / (c // 4))
-        cw, ch = torch.outer(cols.flatten(), freq), torch.outer(rows.flatten(), freq)
-        pos = torch.cat((cw.sin(), cw.cos(), ch.sin(), ch.cos()), 1)
-        t = x.flatten(2).transpose(1, 2)
-        wq, wk, wv = W["ma.in_proj_weight"].chunk(3)
-        bq, bk, bv = W["ma.in_proj_bias"].chunk(3)
-        q, k, v = (F.linear(i, j, l).view(b, h * w, heads, c // heads).transpose(1, 2)
-                   for i, j, l in ((t + pos, wq, bq), (t + pos, wk, bk), (t, wv, bv)))
-        a = ((q @ k.transpose(-1, -2)) / (c // heads) ** 0.5).softmax(-1) @ v
-        t = t + F.linear(a.transpose(1, 2).reshape(b, h * w, c), W["ma.out_proj.weight"], W["ma.out_proj.bias"])
-        t = F.layer_norm(t, (c,), W["norm1.weight"], W["norm1.bias"])
-        f = F.linear(F.gelu(F.linear(t, W["fc1.weight"], W["fc1.bias"])), W["fc2.weight"], W["fc2.bias"])
-        t = F.layer_norm(t + f, (c,), W["norm2.weight"], W["norm2.bias"])
-        return t.transpose(1, 2).reshape(b, c, h, w)
-
     def detect(self, xs, p, nc):
         outs = []
         for li, x in enumerate(xs):

@@ -67,26 +67,25 @@ __device__ __forceinline__ void bias8(const GemmArgs& a, int n, float* b) {
   }
 }
 
-// One operand's tile in LDS: kRows rows (of m or n) x 128 bytes of K, as 16-byte chunks.
+// One 16-bit operand's tile in LDS: kRows rows (of m or n) x 128 bytes of K, as 16-byte chunks.
 //   plain       [row][8 chunks of k]; chunk c of row r lies at c ^ (r & 7), so the 16 rows a
 //               fragment read touches fall on different banks
-//   transposed  [k][kRows]; the 16 rows of a fragment are one segment (32 / 64 bytes) of a k row;
+//   transposed  [k][kRows]; the 16 rows of a fragment are one segment (32 bytes) of a k row;
 //               segment s of k row kk lies at s ^ twist(kk), which spreads the k rows one read
-//               touches over the banks; 16-bit fragments come through ds_read_b64_tr_b16
+//               touches over the banks; fragments come through ds_read_b64_tr_b16
 template <class Tr, bool kTrans, int kRows>
 struct Tile {
   using T = typename Tr::T;
-  static constexpr int kK = 128 / Tr::kBytes;         // K elements of a tile
-  static constexpr int kEpc = 16 / Tr::kBytes;        // elements of a chunk
+  static_assert(Tr::kBytes == 2, "float32 operands: SplitTile");
+  static constexpr int kK = 64;                       // K elements of a tile
+  static constexpr int kEpc = 8;                      // elements of a chunk
   static constexpr int kChunks = kRows * 8;
   static constexpr int kPerRow = kTrans ? kRows / kEpc : 8;  // chunks of a stored row
   static constexpr int kSegs = kRows / 16;
-  static constexpr int kSegChunks = Tr::kBytes;       // 16 elements = 32 / 64 bytes
+  static constexpr int kSegChunks = 2;                // 16 elements = 32 bytes
   static constexpr int kBytesAll = kRows * 128;
 
-  static __device__ __forceinline__ int twist(int kk) {
-    return (Tr::kBytes == 4 ? kk >> 3 : (kk & 3) | ((kk >> 1) & 4)) & (kSegs - 1);
-  }
+  static __device__ __forceinline__ int twist(int kk) { return ((kk & 3) | ((kk >> 1) & 4)) & (kSegs - 1); }
   // stored row and first element of chunk j
   static __device__ __forceinline__ void locate(int j, int& row, int& col) {
     row = j / kPerRow;
@@ -99,15 +98,8 @@ struct Tile {
   static __device__ __forceinline__ typename Tr::V8 frag(const char* lds, int t, int step, int lane) {
     const int l = lane & 15, g = lane >> 4;
     if constexpr (!kTrans) {
-      const char* row = lds + (t * 16 + l) * 128;
-      if constexpr (Tr::kBytes == 2) {
-        return *(const typename Tr::V8*)(row + (((step * 4 + g) ^ (l & 7)) << 4));
-      } else {
-        const f32x4 lo = *(const f32x4*)(row + (((2 * g) ^ (l & 7)) << 4));
-        const f32x4 hi = *(const f32x4*)(row + (((2 * g + 1) ^ (l & 7)) << 4));
-        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      }
-    } else if constexpr (Tr::kBytes == 2) {
+      return *(const typename Tr::V8*)(lds + (t * 16 + l) * 128 + (((step * 4 + g) ^ (l & 7)) << 4));
+    } else {
       const int kk = step * 32 + g * 8 + (l >> 2);
       typedef __attribute__((address_space(3))) s16x4* lp;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -115,14 +107,6 @@ struct Tile {
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (lp)(lds + (kk + 4) * (kRows * 2) + ((t ^ twist(kk + 4)) << 5) + (l & 3) * 8));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    } else {
-      f32x8 v;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int kk = g * 8 + e;
-        v[e] = *(const float*)(lds + kk * (kRows * 4) + ((t ^ twist(kk)) << 6) + l * 4);
-      }
-      return v;
     }
   }
 };
