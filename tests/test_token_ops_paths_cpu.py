@@ -5,6 +5,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+import token_kernels as K
 from conftest import pkg
 
 L = pkg()._lib
@@ -44,3 +45,34 @@ def test_more_workgroups_than_a_launch_holds(fn, args):
     a = L.TOKEN_ARGS[fn](**args)
     assert getattr(L.lib(), fn)(C.addressof(CTX), C.byref(a), None) == L.YK_ERR_ARG
     assert b"than a launch holds" in L.lib().yk_last_error()
+
+
+# ---- the sizes of test_token_ops_paths_gpu.py reach the kernels that they are there for --------------
+@pytest.mark.parametrize("dt,form,m,k,n", K.PRODUCTS)
+def test_sizes_reach_the_products_of_large_tiles(dt, form, m, k, n):
+    names = {"ff": K.linear_kernels(dt, m, k, n), **dict(zip(("ft", "tt"), K.linear_grad_kernels(dt, m, k, n)))}
+    assert K.product_form(dt, names[form[:2]]) == form
+
+
+@pytest.mark.parametrize("dt", K.NORM_WIDTHS)
+def test_sizes_reach_every_norm_of_16_lanes(dt):
+    t, got = K.TRAIT[dt], set()
+    for c in K.NORM_WIDTHS[dt]:
+        fwd, bwd = K.norm_kernels(dt, K.NORM_ROWS, c)
+        got |= {fwd[0], bwd[0]}
+    assert {f"norm_kernel<{t}, 16, {i}>" for i in range(2, 9)} | {f"norm_grad_kernel<{t}, 16, 2>"} <= got
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("b,n,h,hk,d", K.TWO_TILES)
+def test_sizes_reach_two_tiles_a_wave(dt, b, n, h, hk, d):
+    t, dp = K.TRAIT[dt], (d + 31) // 32 * 32
+    fwd, bwd = K.attention_kernels(dt, b, n, n, h, hk, d)
+    assert fwd == [f"attn_kernel<{t}, {dp}, 2, true>"]
+    assert f"attn_dq_kernel<{t}, {dp}, 2, true>" in bwd
+    assert f"attn_dkv_kernel<{t}, {dp}, {2 if dp == 96 else 1}, true>" in bwd
+
+
+def test_kernels_are_reported_for_good_arguments_only():
+    with pytest.raises(pkg().YKError, match="activation"):
+        K.kernels("yk_linear", "bf16", **{"m": 4, "n": 4, "k": 4, "act": 9})

@@ -1,12 +1,15 @@
 """The token operators (ops.py) on the GPU where their other tests do not reach: gradients at the ends of
 fp16's range, rows with exact means, more
-rows than one launch holds, refusals.  Element by element against float64 within the bounds of token_helpers.py."""
+rows than one launch holds, sizes that take the kernels of large calls (which those are,
+test_token_ops_paths_cpu.py checks), refusals.  Element by element against float64 within the bounds of token_helpers.py."""
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 import token_helpers as R
+import token_kernels as K
 from conftest import pkg
+from test_token_ops_gpu import run_attention
 
 pytestmark = pytest.mark.gpu
 DT = R.DTYPES
@@ -186,3 +189,63 @@ def test_profile_names_the_kernels_of_an_aifi_row(dtype):
         assert len(names[M.YK_K_LINEAR]) == 4 and all(n.startswith(linear) for n in names[M.YK_K_LINEAR]), names
         assert all(n.startswith("norm_kernel<yk::tok::" + t) for n in names[M.YK_K_LAYER_NORM]), names
         assert all(n.startswith(attention) for n in names[M.YK_K_ATTENTION]), names
+
+
+# ---- kernels that large calls take ------------------------------------------------------------------
+@pytest.mark.parametrize("dt,form,m,k,n", K.PRODUCTS)
+def test_products_of_large_tiles(ops, dt, form, m, k, n):
+    """Whole tiles and remainders of every tile size and operand order, split or not."""
+    x, w, b = rn(m, k, dt=dt), rn(n, k, dt=dt, std=k ** -0.5), rn(n, dt=dt)
+    if form.startswith("ff"):
+        for act, res, bias in (("none", None, None), ("gelu", rn(77, n, dt=dt, seed=2), b)):
+            y, z = ops.linear(x, w, bias, act=act, residual=res, return_preact=True)
+            want, ey, wz, ez = R.linear(x, w, bias, act, res)
+            R.check(y, want, ey, f"y {act}")
+            R.check(z, wz, ez, f"z {act}")
+            assert torch.equal(y, ops.linear(x, w, bias, act=act, residual=res))
+        return
+    dy, z = rn(m, n, dt=dt, seed=1), rn(m, n, dt=dt, seed=3)
+    for act in ("none", "silu"):
+        got = ops.linear_backward(dy, x, w, b, act=act, preact=z)
+        again = ops.linear_backward(dy, x, w, b, act=act, preact=z)
+        for (want, e), g, a, name in zip(R.linear_grads(dy, x, w, act, z), got, again, ("dx", "dw", "db")):
+            R.check(g, want, R._final(want, e, b.dtype) if name == "db" else e, f"{name} {act}")
+            assert torch.equal(g, a)
+
+
+@pytest.mark.parametrize("dt,c", [(dt, c) for dt, cs in K.NORM_WIDTHS.items() for c in cs])
+def test_layer_norm_of_many_rows(ops, dt, c):
+    """Rows of 16 lanes at every number of chunks per lane, whole and with ragged ends."""
+    m = K.NORM_ROWS
+    x = rn(m, c, dt=dt) * 2 + rn(m, 1, dt=dt, seed=1) * 4
+    w, b, dy = rn(c, dt=dt) * 0.1 + 1, rn(c, dt=dt, seed=2), rn(m, c, dt=dt, seed=3)
+    for wt, bt in ((w, b), (w.float(), b.float()), (None, None)):
+        y, mean, rstd = ops.layer_norm(x, wt, bt, return_stats=True)
+        want, e = R.layer_norm(x, wt, bt, 1e-5)
+        R.check(y, want, e, "y")
+        grads = ops.layer_norm_backward(dy, x, wt, mean, rstd)
+        again = ops.layer_norm_backward(dy, x, wt, mean, rstd)
+        for (want, e), g, a, name in zip(R.layer_norm_grads(dy, x, wt, 1e-5), grads, again, ("dx", "dw", "db")):
+            R.check(g, want, e if name == "dx" else R._final(want, e, g.dtype), name)
+            assert torch.equal(g, a)
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_layer_norm_of_many_turns(ops, dt):
+    """A workgroup of the backward pass walks many rows, each fetched while one is worked on."""
+    for m, c in ((60001, 24), (20003, 600)):
+        x, w, dy = rn(m, c, dt=dt) + 1, rn(c, dt=dt), rn(m, c, dt=dt, seed=3)
+        y, mean, rstd = ops.layer_norm(x, w, return_stats=True)
+        for (want, e), g, name in zip(R.layer_norm_grads(dy, x, w, 1e-5), ops.layer_norm_backward(dy, x, w, mean, rstd), ("dx", "dw", "db")):
+            R.check(g, want, e if name == "dx" else R._final(want, e, g.dtype), name)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("b,n,h,hk,d", K.TWO_TILES)
+def test_attention_of_two_tiles_a_wave(ops, dt, causal, b, n, h, hk, d):
+    """Blocks of 128 rows with a remainder, whole batches and ragged ones, with gradients."""
+    run_attention(ops, dt, b, n, n, h, hk, d, causal)
+    lens = [n, 0, 1, 129, n - 1, 64, 300, 257] + [n] * (b - 8)
+    run_attention(ops, dt, b, n, n, h, hk, d, causal, lengths=lens, q_lengths=lens)
+    run_attention(ops, dt, b, n, n, h, hk, d, causal, lengths=[n - 3, 17, 0, 200] * (b // 4) + [n] * (b % 4))
