@@ -76,3 +76,16 @@ def test_sizes_reach_two_tiles_a_wave(dt, b, n, h, hk, d):
 def test_kernels_are_reported_for_good_arguments_only():
     with pytest.raises(pkg().YKError, match="activation"):
         K.kernels("yk_linear", "bf16", **{"m": 4, "n": 4, "k": 4, "act": 9})
+
+
+@pytest.mark.parametrize("args", [[64, 8, 0, "nn.ReLU"], [64, 8, 0, "nn.GELU", True], [64, 0], [64, -8], [0, 8], [64.5, 8], ["64", 8]])
+def test_aifi_arguments_that_change_the_layer_are_refused(args):
+    """An activation or a norm order that the layer does not have, sizes that no layer has."""
+    import importlib
+
+    from aifi_helpers import aifi_dict
+
+    d = aifi_dict("s")
+    d["backbone"][10][3] = args
+    with pytest.raises(ValueError, match="AIFI"):
+        importlib.import_module(pkg().__name__ + ".arch").parse_arch(d)

@@ -138,12 +138,16 @@ def parse_arch(d: dict, ch: int = 3) -> Arch:
             else:
                 L = Layer(i, f, m, c1, c2, {"k": args[1] if len(args) > 1 else 5})
         elif m == "AIFI":
-            c, heads = chs[f], args[1] if len(args) > 1 else 8
+            c, hidden, heads = chs[f], args[0] if args else 2048, args[1] if len(args) > 1 else 8
+            if len(args) > 2:
+                raise ValueError(f"AIFI: arguments are [hidden, heads] (post-norm, GELU), got {args}")
+            if not all(isinstance(v, int) and v >= 1 for v in (hidden, heads)):
+                raise ValueError(f"AIFI: hidden and heads must be whole numbers >= 1, got {hidden} and {heads}")
             if n != 1:
                 raise ValueError("AIFI: one layer per row (repeats must be 1)")
             if c % 8 or c % heads or c // heads > 128:
                 raise ValueError(f"AIFI: {c} channels must be a multiple of 8 and of the {heads} heads, at most 128 each")
-            L = Layer(i, f, m, c, c, {"hidden": args[0] if args else 2048, "heads": heads})
+            L = Layer(i, f, m, c, c, {"hidden": hidden, "heads": heads})
         elif m == "Upsample":
             L = Layer(i, f, m, chs[f], chs[f], {"scale": args[1]})
         elif m == "Concat":
