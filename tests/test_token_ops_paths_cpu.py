@@ -87,5 +87,8 @@ def test_aifi_arguments_that_change_the_layer_are_refused(args):
 
     d = aifi_dict("s")
     d["backbone"][10][3] = args
+    parse = importlib.import_module(pkg().__name__ + ".arch").parse_arch
     with pytest.raises(ValueError, match="AIFI"):
-        importlib.import_module(pkg().__name__ + ".arch").parse_arch(d)
+        parse(d)
+    d["backbone"][10][3] = [64, 8, 0.1]  # a dropout is of training only
+    assert parse(d).layers[10].args == {"hidden": 64, "heads": 8}

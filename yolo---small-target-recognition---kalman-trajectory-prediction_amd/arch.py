@@ -139,7 +139,7 @@ def parse_arch(d: dict, ch: int = 3) -> Arch:
                 L = Layer(i, f, m, c1, c2, {"k": args[1] if len(args) > 1 else 5})
         elif m == "AIFI":
             c, hidden, heads = chs[f], args[0] if args else 2048, args[1] if len(args) > 1 else 8
-            if len(args) > 2:
+            if len(args) > 3:  # (the third is a dropout, of training only)
                 raise ValueError(f"AIFI: arguments are [hidden, heads] (post-norm, GELU), got {args}")
             if not all(isinstance(v, int) and v >= 1 for v in (hidden, heads)):
                 raise ValueError(f"AIFI: hidden and heads must be whole numbers >= 1, got {hidden} and {heads}")
