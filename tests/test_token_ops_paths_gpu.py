@@ -163,6 +163,21 @@ def test_an_earlier_error_of_the_runtime_is_not_the_calls(ops):
         assert torch.equal(a, b)
 
 
+def test_the_first_call_may_be_a_captured_one(ops, monkeypatch):
+    """The device's context is made by the first call: inside a capture too."""
+    x, w, q = rn(300, 64), rn(40, 64), rn(2, 200, 4, 64, dt="fp16")
+    want = ops.linear(x, w, act="gelu"), ops.attention(q, q, q)
+    monkeypatch.setattr(pkg()._lib, "_ctx", {})
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y, o = ops.linear(x, w, act="gelu"), ops.attention(q, q, q)
+    for _ in range(3):
+        y.zero_(), o.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[0]) and torch.equal(o, want[1])
+
+
 # ---- the detector's report ------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_profile_names_the_kernels_of_an_aifi_row(dtype):

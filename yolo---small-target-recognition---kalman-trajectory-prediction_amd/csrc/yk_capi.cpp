@@ -76,7 +76,14 @@ int yk_ctx_create(int device, yk_ctx** out) {
   YK_HIP(hipGetDeviceCount(&n));
   YK_CHECK_ARG(device >= 0 && device < n, "yk_ctx_create: device index out of range");
   yk::DeviceGuard g(device);
-  YK_HIP(hipFree(nullptr));  // force runtime/context initialisation on this device
+  // Force runtime / context initialisation on this device.  The first call may come while a stream is being
+  // captured (torch.cuda.graph: global mode), where hipFree would end the capture of a thread that has not
+  // said that its calls are its own affair.
+  hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+  YK_HIP(hipThreadExchangeStreamCaptureMode(&mode));
+  const hipError_t init = hipFree(nullptr);
+  YK_HIP(hipThreadExchangeStreamCaptureMode(&mode));
+  YK_HIP(init);
   *out = new yk_ctx{device};
   return YK_OK;
 }
