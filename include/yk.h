@@ -616,8 +616,11 @@ int yk_memcpy_d2h(void* host_dst, const void* dev_src, int64_t bytes);
  * program's YK_K_LINEAR / YK_K_LAYER_NORM / YK_K_ATTENTION ops call the same kernels.  Matrices
  * are rows of `dtype` elements (YK_ACT_BF16, YK_ACT_F32 or YK_ACT_F16) with a stride between
  * rows, in elements (an input's may be 0: one row for all); elements of a row are adjacent.  Any
- * size from 1, any alignment that is a multiple of the element.  Sums,
- * softmax statistics and norms are float32; an output is rounded once.
+ * size from 1 that a launch holds (fewer than 2^32 threads; beyond, a call is refused before anything
+ * runs), any alignment that is a multiple of the element.  Sums, softmax statistics and norms are
+ * float32; an output is rounded once.  The 16-bit types also round, to the type, the operands that a
+ * call makes for its own matrix products: attention's P (forward, and for dv) and dS, and
+ * yk_linear_backward's dz where there is an activation.
  *
  * Every call only enqueues kernels on `stream` (hipGraph-capturable); nothing is allocated, so
  * a call that needs scratch takes it from the caller: *_workspace returns the bytes for the same

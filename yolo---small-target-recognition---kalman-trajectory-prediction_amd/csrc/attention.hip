@@ -358,8 +358,8 @@ __device__ __forceinline__ void key_range(int& k_begin, int& k_stop) {
 // Forward: 4 waves of 16 kNT rows; with few row blocks, blockIdx.y a range of the keys, whose sums
 // attn_join_rows_kernel joins.  Bound by issue: per block and lane 32 kNT exponentials, their sums and
 // conversions next to the MFMAs, neither of which hides the other wholly with two waves per SIMD.
-// bf16, 4 x 5120 x 5120, 8 heads of 64: 260 us, 826 TFLOP/s; 8 x 1280 x 1280, 8 heads of 40 (computed as
-// 64): 39 us.
+// bf16, 4 x 5120 x 5120, 8 heads of 64: 242 us, 887 TFLOP/s (under the profiler 258-272); 8 x 1280 x 1280,
+// 8 heads of 40 (computed as 64): 39 us.
 template <class Tr, int kDP, int kNT, bool kAsync>
 __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_kernel(AttnArgs a, int row_blocks) {
   using T = typename Tr::T;
@@ -692,7 +692,7 @@ constexpr float kShiftP<H16> = 15.f;
 // is rounded to fp16 is off by half a step of itself or 2^-34 of the column's largest so far.  It begins
 // at 2^64: |dS| 2^15 <= 2^15 128 65504^2 < 2^55 of fp16 operands stays finite times that, and what never
 // reaches 2^15 needs no less.  The other types' range is float32's, and nothing of this is compiled.
-// 4 x 5120 x 5120, 8 heads of 64, backward: 869 us, 819 without it (bf16 787).
+// 4 x 5120 x 5120, 8 heads of 64, backward: 869-880 us, 819 without it (bf16 787-796).
 template <class Tr>
 struct GradScale {
   static constexpr bool kOn = Tr::kBytes == 2 && kShiftP<Tr> != 0.f;
@@ -755,7 +755,8 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs a) {
 // dk and dv: 4 waves of 16 kNT keys, blocks of packed rows (q, do and their statistics) through LDS;
 // with few keys, blockIdx.y a range of the rows, whose float32 sums attn_dkv_sum_kernel adds.  S and dP are
 // computed here and once more for dq, instead of sums that several workgroups add to: 14 products' work
-// for 10, but no atomics and equal bits.  bf16, 4 x 5120 x 5120, 8 heads of 64: 470 us, 914 TFLOP/s.
+// for 10, but no atomics and equal bits.  bf16, 4 x 5120 x 5120, 8 heads of 64: 471-497 us under the
+// profiler, 864-912 TFLOP/s; fp16, whose dS is scaled, 513-535.
 template <class Tr, int kDP, int kNT, bool kAsync>
 __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_dkv_kernel(AttnArgs a, int key_blocks) {
   using T = typename Tr::T;
@@ -948,7 +949,8 @@ __global__ __launch_bounds__(256) void attn_dq_sum_kernel(AttnArgs a, int dp, in
 }
 
 // dq: 4 waves of 16 kNT rows, key blocks (k, v) through LDS; with few rows, blockIdx.y a range of the keys,
-// whose float32 sums attn_dq_sum_kernel adds.  bf16, 4 x 5120 x 5120, 8 heads of 64: 330 us, 976 TFLOP/s.
+// whose float32 sums attn_dq_sum_kernel adds.  bf16, 4 x 5120 x 5120, 8 heads of 64: 325-345 us under the
+// profiler, 934-991 TFLOP/s; fp16 337-350.
 template <class Tr, int kDP, int kNT, bool kAsync>
 __global__ __launch_bounds__(256, kWavesPerSimd<Tr>) void attn_dq_kernel(AttnArgs a, int row_blocks) {
   using T = typename Tr::T;

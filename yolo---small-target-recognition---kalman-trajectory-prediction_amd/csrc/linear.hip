@@ -322,9 +322,9 @@ __device__ __forceinline__ void loads_landed() {
   __builtin_amdgcn_s_barrier();
 }
 
-// kTM x kTN tile of C by kWM x kWN waves.  256-tiles, bf16: 8192^3 820 us (1340 TFLOP/s; a wave's LDS reads and
-// the loads into LDS take about the cycles its MFMAs do), 40960 x 4096 x 1024 320 us, of which some 65
-// are first loads and epilogues that one workgroup per CU hides behind nothing; with GELU 377.  Three or four
+// kTM x kTN tile of C by kWM x kWN waves.  256-tiles, bf16: 8192^3 820-850 us (1290-1340 TFLOP/s; a wave's LDS reads
+// and the loads into LDS take about the cycles its MFMAs do), 40960 x 4096 x 1024 313 us, of which some 65
+// are first loads and epilogues that one workgroup per CU hides behind nothing; with GELU 365-385.  Three or four
 // stages: 4096 x 1024 x 2048 in 128-tiles 26 -> 23 us, but the LDS they take leaves one workgroup
 // per CU where two fit (10240 x 512 x 2048: 30 -> 40), and so do fragments read a half tile ahead: no gain.
 // Rows that are not 16-byte aligned go through registers (4097 x 777 x 1111 fp16: 31 us), bound by the
@@ -426,7 +426,7 @@ __global__ __launch_bounds__(64 * kWM * kWN) void gemm_kernel(GemmArgs a) {
 // summed: w0x0, w0x1, w1x0, w1x1, w0x2, w2x0.  bf16 products are exact in float32 and what is left out
 // is below 2^-25 |w x|, less than one float32 rounding; six 16-cycle MFMAs per 32 of K replace eight
 // 32-cycle float32 ones.  (A part below bf16's normal range, of an operand below some 2^-110, may be
-// flushed.)  4096 x 1024 x 4096: 188 us, 267 on v_mfma_f32_16x16x4_f32.
+// flushed.)  4096 x 1024 x 4096: 181-198 us, 267 on v_mfma_f32_16x16x4_f32.
 //
 // The parts are made once per tile, between the global loads' registers and LDS (three planes a
 // side), not by every wave that reads them.  A tile is 32 of K:
@@ -886,7 +886,8 @@ Plan plan_for(const GemmArgs& a, bool& async) {
   return plan_gemm(a.m, a.n, a.k, Tr::kBytes, kXT + kWT, async);
 }
 
-// part: `room` bytes of scratch; without enough of it K is not split
+// part: `room` bytes of scratch; without enough of it K is not split, and the tile stays the one planned with
+// the split (float32 2560 x 512 x 2048: 47 us, without scratch 116; 320 x 320 x 1024: 13 and 28)
 template <class Tr, bool kXT, bool kWT>
 void launch_gemm(GemmArgs a, void* part, int64_t room, hipStream_t st) {
   bool async;

@@ -7,7 +7,9 @@ the tensors' device's current stream, allocate their outputs and scratch from to
 synchronise, so they can be captured into a graph.  No autograd graph is built: a call whose
 inputs require gradients (while gradients are enabled) or carry a forward-mode tangent raises, and so
 does one under torch.jit.trace, which would record its empty outputs; the ``*_backward`` functions
-return the gradients.  Sums are float32 and outputs are rounded once; equal calls give equal bits.
+return the gradients.  Sums are float32 and an output is rounded once; what else a 16-bit type rounds are
+operands of its matrix products (attention's P and dS, linear's dz) and the preactivation that linear
+returns.  Equal calls give equal bits.
 
 A tensor's last dimension must be contiguous; what precedes it must step evenly from row to row
 (any row stride, so a channel slice of a wider tensor is fine).  Anything else raises ValueError.
@@ -327,7 +329,8 @@ def attention(q, k, v, *, scale=None, causal=False, lengths=None, q_lengths=None
     lengths / q_lengths (int32 [B] on the device): keys / queries in use, the rest of a padded
     batch; keys behind a length are never read, queries behind one give 0.  causal: query i
     sees keys j <= i + length - q_length, so one new token sees its whole cache.  A query that sees
-    no key gives 0.  Returns o like q, with return_lse also ln of the softmax's denominators,
+    no key gives 0.  (What causality alone hides takes part as a factor of 0: a NaN or infinity in v, or
+    in k, q or do backward, may show as NaN there; behind the lengths none does.)  Returns o like q, with return_lse also ln of the softmax's denominators,
     float32 [B, H, Nq] (-inf where no key is seen), for attention_backward."""
     dev, head, qkv, lens, strides = _attention_args(q, k, v, scale, causal, q_lengths, lengths)
     o = _fresh(q)
